@@ -55,6 +55,7 @@ class LevelDesc(C.Structure):
 
 _P = C.c_void_p
 _I = C.c_int32
+_L = C.c_int64
 _F = C.c_float
 _MD = C.POINTER(ModelDesc)
 _BC = C.POINTER(BatchCounts)
@@ -103,6 +104,14 @@ SIGNATURES = {
     "dvae_decode": (_I, [_MD, _I, _P, _P, _P, _I, _P, _P, _P, _P, _P, _P]),
     "dvae_decode_static_max_floats": (C.c_int64, []),
     "dvae_decode_static": (_I, [_MD, _I, _P, _P, _I, _P, _P, _P, _P, _P, _P]),
+    "dvae_embed_fwd": (_I, [_P, _L, _P, _I, _P, _L, _L, _I, _F, _I, _P]),
+    "dvae_embed_bwd_ws_bytes": (_L, [_L, _L, _I]),
+    "dvae_embed_bwd": (_I, [_P, _L, _P, _I, _P, _P, _L, _L, _I, _F, _I, _P]),
+    "dvae_scan_state_floats": (_L, [_L, _I]),
+    "dvae_scan_ws_bytes": (_L, [_L, _I]),
+    "dvae_scan_fwd": (_I, [_P, _L, _P, _L, _P, _I, _P, _P, _P, _P, _P, _L, _L, _I, _I, _P]),
+    "dvae_scan_bwd": (_I, [_P, _L, _P, _L, _P, _I, _P, _P, _P, _L, _P, _P, _P, _P, _P, _L, _L, _I, _I, _P]),
+    "dvae_scan_step": (_I, [_P, _L, _P, _L, _P, _L, _L, _P, _I, _P, _I, _I, _I, _P]),
     "dvae_encode_ws_floats": (C.c_int64, [_MD, _BC]),
     "dvae_loss_ws_floats": (C.c_int64, [_MD, _BC]),
     "dvae_debug_side_stream": (_I, [_P, C.POINTER(_P)]),

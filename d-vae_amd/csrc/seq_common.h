@@ -1,0 +1,61 @@
+// Shared by the sequence operators (embed.hip, scan.hip): element types, vector accesses and their widest legal width.
+#pragma once
+#include "common.h"
+#include "dvae_hip.h"
+
+namespace dvae {
+
+// V consecutive elements of T as one access (V * sizeof(T) <= 16 bytes, aligned to that)
+template <typename T, int V> struct alignas(sizeof(T) * V) Pack { T e[V]; };
+
+template <typename T, int V> __device__ __forceinline__ Pack<T, V> load_pack(const T* p) {
+    return *reinterpret_cast<const Pack<T, V>*>(p);
+}
+template <typename T, int V> __device__ __forceinline__ void store_pack(T* p, const Pack<T, V>& v) {
+    *reinterpret_cast<Pack<T, V>*>(p) = v;
+}
+// one rounding, to nearest even
+template <typename T, int V> __device__ __forceinline__ void store_floats(T* p, const float (&f)[V]) {
+    Pack<T, V> o;
+#pragma unroll
+    for (int i = 0; i < V; ++i) o.e[i] = (T)f[i];
+    store_pack<T, V>(p, o);
+}
+
+static inline int elem_size(int dtype) { return dtype == DVAE_F32 ? 4 : 2; }
+static inline bool known_dtype(int dtype) { return dtype == DVAE_F32 || dtype == DVAE_BF16 || dtype == DVAE_F16; }
+
+// The widest vector (in elements, at most `bytes` bytes) that divides every listed extent / stride and to which every
+// base pointer is aligned.  An odd row length leaves single elements, which a wave still reads as one 128- or 256-byte run.
+template <size_t NE, size_t NP>
+static inline int widest(int es, int bytes, const int64_t (&extents)[NE], const void* const (&ptrs)[NP]) {
+    for (int v = bytes / es; v > 1; v /= 2) {
+        bool ok = true;
+        for (int64_t x : extents) ok = ok && x % v == 0;
+        for (const void* p : ptrs) ok = ok && (uintptr_t)p % (uintptr_t)(v * es) == 0;
+        if (ok) return v;
+    }
+    return 1;
+}
+
+// CALL(T, V) for the element type and vector width picked at run time
+#define DVAE_BY_TYPE(dtype, vec, CALL)                                        \
+    do {                                                                      \
+        if ((dtype) == DVAE_F32) {                                            \
+            if ((vec) >= 4) { CALL(float, 4); }                               \
+            else if ((vec) == 2) { CALL(float, 2); }                          \
+            else { CALL(float, 1); }                                          \
+        } else if ((dtype) == DVAE_BF16) {                                    \
+            if ((vec) >= 8) { CALL(__bf16, 8); }                              \
+            else if ((vec) == 4) { CALL(__bf16, 4); }                         \
+            else if ((vec) == 2) { CALL(__bf16, 2); }                         \
+            else { CALL(__bf16, 1); }                                         \
+        } else {                                                              \
+            if ((vec) >= 8) { CALL(_Float16, 8); }                            \
+            else if ((vec) == 4) { CALL(_Float16, 4); }                       \
+            else if ((vec) == 2) { CALL(_Float16, 2); }                       \
+            else { CALL(_Float16, 1); }                                       \
+        }                                                                     \
+    } while (0)
+
+}  // namespace dvae

@@ -446,6 +446,50 @@ int dvae_decode_static(const dvae_model_desc* m, int32_t B, const float* pw, con
                        const float* u_type, const float* u_edge, int32_t* types, uint64_t* pred_mask,
                        int32_t* n_vertices, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Sequence operators: a token table and a gated linear recurrence over packed
+ * sequences, for sequence encoders beside the DAG model (the reference's own
+ * ones, models.py:18-338, run on stock nn.GRU and one-hot inputs).
+ *
+ * Element types of the matrices (the states of the recurrence are always fp32).
+ * ------------------------------------------------------------------------- */
+enum { DVAE_F32 = 0, DVAE_BF16 = 1, DVAE_F16 = 2 };
+
+/* out[t][0:D] = scale * w[ids[t]][0:D] (w [vocab] rows of stride ld_w elements, out [n][D] contiguous; rounded once).
+ * ids: int32, or int64 with ids_i64 = 1; a token outside [0, vocab) gives a row of zeros. */
+int dvae_embed_fwd(const void* w, int64_t ld_w, const void* ids, int32_t ids_i64, void* out, int64_t n, int64_t vocab,
+                   int32_t D, float scale, int32_t dtype, void* stream);
+/* dw[v][0:D] = scale * sum over t with ids[t] = v of dout[t][0:D] (dw [vocab][D] contiguous, every row written; dout rows
+ * of stride ld_dout, 0 = one row for all; tokens outside [0, vocab) take no part).  Sums in fp32 over the sorted tokens,
+ * rounded once; the result does not vary from run to run.  ws: dvae_embed_bwd_ws_bytes() bytes, 16-byte aligned. */
+int64_t dvae_embed_bwd_ws_bytes(int64_t n, int64_t vocab, int32_t D);
+int dvae_embed_bwd(const void* dout, int64_t ld_dout, const void* ids, int32_t ids_i64, void* dw, void* ws, int64_t n,
+                   int64_t vocab, int32_t D, float scale, int32_t dtype, void* stream);
+
+/* h[t] = z[t] h[t-1] + (1 - z[t]) x[t], z = sigmoid(gate), along `seqs` sequences packed into `rows` rows of D channels:
+ * sequence s is the rows [off[s], off[s+1]) (off: seqs + 1 values that do not decrease, int32 or int64; NULL: sequences of
+ * rows / seqs rows each); values outside [0, rows] count as the nearer end.  The state before a sequence is h0[s] (fp32
+ * [seqs][D]; NULL: zeros).  gate, x: row strides ld_* in elements (halves of one projection's output are allowed; 0 = one
+ * row for all); h [rows][D] contiguous, rounded once; last [seqs][D] fp32: the state after each sequence (h0 where it is
+ * empty).  Rows of no sequence give zeros.  states: dvae_scan_state_floats() floats that the backward pass reads (NULL if
+ * there is none); ws: dvae_scan_ws_bytes() bytes, 16-byte aligned, for this call alone. */
+int64_t dvae_scan_state_floats(int64_t rows, int32_t D);
+int64_t dvae_scan_ws_bytes(int64_t rows, int32_t D);
+int dvae_scan_fwd(const void* gate, int64_t ld_gate, const void* x, int64_t ld_x, const void* off, int32_t off_i64,
+                  const float* h0, void* h, float* last, float* states, void* ws, int64_t rows, int64_t seqs, int32_t D,
+                  int32_t dtype, void* stream);
+/* autograd of the above.  dh (NULL: zeros) and dlast (NULL: zeros) are the upstream gradients; dgate, dx [rows][D]
+ * contiguous, every row written (zeros in rows of no sequence); dh0 [seqs][D] fp32, nullable. */
+int dvae_scan_bwd(const void* gate, int64_t ld_gate, const void* x, int64_t ld_x, const void* off, int32_t off_i64,
+                  const float* h0, const float* states, const void* dh, int64_t ld_dh, const float* dlast, void* dgate, void* dx,
+                  float* dh0, void* ws, int64_t rows, int64_t seqs, int32_t D, int32_t dtype, void* stream);
+/* One token of each of `rows` sequences: state[slots[b]] = h[b] = z[b] state[slots[b]] + (1 - z[b]) x[b], in place in a
+ * pool of fp32 states (row stride ld_state).  slots: int32 / int64, NULL: row b has state b.  A slot outside [0, pool)
+ * marks a padding row: h[b] = 0, no state changes.  Rows with the same slot advance it one after the other in their order. */
+int dvae_scan_step(const void* gate, int64_t ld_gate, const void* x, int64_t ld_x, float* state, int64_t ld_state,
+                   int64_t pool, const void* slots, int32_t slots_i64, void* h, int32_t rows, int32_t D, int32_t dtype,
+                   void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,375 @@
+"""The sequence operators (d-vae_amd/sequence.py) against plain implementations in 64 bits.
+
+Tolerances: u = 2^-24 is half a step of float32, r = eps / 2 of the output's type; M bounds the values of x and h0 (and so
+of every state, a convex combination of them).  A step of the recurrence rounds a few times (gate and its complement about
+3 u each relative, two products, one sum: 8 u M together) and passes older errors on times z <= zmax, so they add up to at most
+8 u M min(T, 1 / (1 - zmax)); the exponential's argument adds 16 u |g| / 10 relative to z (1 - z), which sums to 32 u M."""
+import numpy as np
+import pytest
+import torch
+
+from _dvae_pkg import dvae_amd
+
+S = dvae_amd.sequence
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+DT = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}
+
+
+def half_step(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def close(got, want, tol, what=""):
+    """|got - want| <= tol + half a step of got's type, element by element (tol: number or array)"""
+    got64 = got.detach().double().cpu()
+    err = (got64 - want).abs()
+    lim = tol + want.abs() * half_step(got.dtype) * (1 + 1e-6)
+    if got.dtype == torch.float16:
+        lim = lim + 2.0 ** -25  # half a step among its subnormal numbers
+    assert torch.isfinite(got64).all(), what
+    bad = err > lim
+    assert not bad.any(), "%s: %d of %d off, worst %.3g where %.3g is allowed" % (
+        what, int(bad.sum()), bad.numel(), float((err - lim).max() + lim.max()), float(lim.max()))
+
+
+def gen(seed):
+    g = torch.Generator()
+    g.manual_seed(seed)
+    return g
+
+
+# ------------------------------------------------------------------------------------------------------------------ embed
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("n,vocab,dim", [(1, 1, 1), (5, 3, 7), (31, 8, 501), (33, 255, 64), (64, 256, 96), (257, 40, 1024), (1500, 70000, 33),
+                                         (8192, 8, 130), (8193, 8, 130), (9001, 300, 256), (20011, 66000, 20), (70001, 5, 16)])
+def test_embed_and_its_gradient(dtype, n, vocab, dim):
+    dt, g = DT[dtype], gen(n + vocab)
+    w = torch.randn(vocab, dim, generator=g).to(dt)
+    ids = torch.randint(0, vocab, (n,), generator=g)
+    ids[torch.rand(n, generator=g) < 0.3] = min(2, vocab - 1)  # a hot row
+    ids[torch.rand(n, generator=g) < 0.1] = -1
+    if n > 2:
+        ids[1] = vocab
+    dout = torch.randn(n, dim, generator=g).to(dt)
+    scale = 2.5
+    wd = w.cuda().requires_grad_(True)
+    out = S.embed(wd, ids.to(torch.int32).cuda() if n % 2 else ids.cuda(), scale)
+    ok = (ids >= 0) & (ids < vocab)
+    want = w.double()[ids.clamp(0, vocab - 1)] * scale * ok[:, None]
+    close(out, want, want.abs() * U, "out")  # one product in fp32, then the rounding to the type
+    dw, = torch.autograd.grad(out, [wd], dout.cuda())
+    want = torch.zeros(vocab, dim, dtype=torch.float64).index_add_(0, ids[ok], dout.double()[ok])
+    size = torch.zeros(vocab, dim, dtype=torch.float64).index_add_(0, ids[ok], dout.double()[ok].abs())
+    # additions on any one path: 32 in a chunk, the partials of a wave, the eight waves; each is off by u of a partial sum
+    depth = 32 + (n // 32 // 8 + 2) + 8 + 2
+    close(dw, want * scale, size * scale * depth * U, "dw")
+    again, = torch.autograd.grad(S.embed(wd, ids.cuda(), scale), [wd], dout.cuda())
+    assert torch.equal(dw, again)
+
+
+def test_embed_shapes_strides_and_no_tokens():
+    g = gen(1)
+    big = torch.randn(9, 40, generator=g).cuda()
+    w = big[:, 3:24].requires_grad_(True)  # rows of stride 40 that begin at an odd element
+    ids = torch.randint(-1, 10, (4, 3, 2), generator=g).cuda()
+    out = S.embed(w, ids, 1.0)
+    assert out.shape == (4, 3, 2, 21)
+    ok = ((ids >= 0) & (ids < 9))[..., None]
+    assert torch.equal(out, w[ids.clamp(0, 8)] * ok)
+    one = torch.ones(21, device="cuda").expand(4, 3, 2, 21)  # a gradient of stride 0, as sum() gives it
+    dw, = torch.autograd.grad(out, [w], one)
+    count = torch.stack([(ids == v).sum() for v in range(9)]).float()
+    assert torch.equal(dw, count[:, None].expand(9, 21))
+    out = S.embed(w, ids, 1.0)
+    turned = torch.randn(21, 24, generator=g).cuda().t().reshape(4, 3, 2, 21)
+    dw, = torch.autograd.grad(out, [w], turned)
+    want = torch.zeros(9, 21, dtype=torch.float64)
+    flat, t64 = ids.reshape(-1).cpu(), turned.reshape(-1, 21).double().cpu()
+    for t in range(24):
+        if 0 <= flat[t] < 9:
+            want[flat[t]] += t64[t]
+    close(dw, want, 24 * 24 * U, "dw of a turned gradient")
+    none = S.embed(w, torch.empty(0, dtype=torch.int64, device="cuda"))
+    assert none.shape == (0, 21)
+    dw, = torch.autograd.grad(none, [w], torch.empty(0, 21, device="cuda"))
+    assert torch.equal(dw, torch.zeros(9, 21, device="cuda"))
+
+
+def test_embed_padding_rows_do_not_spread_what_they_hold():
+    w = torch.randn(4, 65).cuda().requires_grad_(True)
+    ids = torch.tensor([1, -1, 3, 4, 1, -7], device="cuda")
+    dout = torch.ones(6, 65, device="cuda")
+    dout[1], dout[3], dout[5] = float("nan"), float("inf"), float("nan")
+    dw, = torch.autograd.grad(S.embed(w, ids), [w], dout)
+    assert torch.equal(dw, torch.tensor([0.0, 2.0, 0.0, 1.0], device="cuda")[:, None].expand(4, 65))
+    all_pad = torch.full((70,), -1, device="cuda")
+    dw, = torch.autograd.grad(S.embed(w, all_pad), [w], torch.full((70, 65), float("nan"), device="cuda"))
+    assert torch.equal(dw, torch.zeros(4, 65, device="cuda"))
+
+
+# ------------------------------------------------------------------------------------------------------------------- scan
+
+def plain_scan(gate, x, off, h0, dh=None, dlast=None):
+    """row by row in 64 bits; off: list of S + 1 row numbers"""
+    N, D = x.shape
+    Sn = len(off) - 1
+    z = torch.sigmoid(gate)
+    omz = torch.sigmoid(-gate)
+    h, prev = torch.zeros(N, D, dtype=torch.float64), torch.zeros(N, D, dtype=torch.float64)
+    init = torch.zeros(Sn, D, dtype=torch.float64) if h0 is None else h0
+    last = init.clone()
+    for s in range(Sn):
+        for t in range(off[s], off[s + 1]):
+            prev[t] = last[s]
+            last[s] = z[t] * last[s] + omz[t] * x[t]
+            h[t] = last[s]
+    if dh is None:
+        return h, last
+    dg, dx, dh0, big = torch.zeros_like(h), torch.zeros_like(h), torch.zeros_like(last), 0.0
+    for s in range(Sn):
+        c = dlast[s].clone()
+        for t in reversed(range(off[s], off[s + 1])):
+            G = dh[t] + c
+            big = max(big, float(G.abs().max()))
+            dx[t] = omz[t] * G
+            dg[t] = G * (prev[t] - x[t]) * z[t] * omz[t]
+            c = z[t] * G
+        dh0[s] = c
+    return h, last, dg, dx, dh0, big
+
+
+def offsets_of(lengths, front=0):
+    return [front + int(v) for v in np.concatenate([[0], np.cumsum(lengths)])]
+
+
+SHAPES = [  # (lengths, rows before the first sequence, rows behind the last)
+    ([1], 0, 0), ([0], 0, 0), ([0, 0, 3], 0, 0), ([5, 0, 0, 1, 64, 65, 0], 0, 0), ([200], 0, 0), ([63, 1, 64, 128, 2], 7, 70),
+    ([7] * 40, 0, 1), ([0, 0], 3, 0), ([700, 1, 1, 1000], 65, 0)]
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("dim", [1, 6, 64, 501, 516])
+@pytest.mark.parametrize("k", range(len(SHAPES)))
+def test_gated_scan_and_its_gradient(dtype, dim, k):
+    lengths, front, behind = SHAPES[k]
+    dt, g = DT[dtype], gen(100 * k + dim)
+    off = offsets_of(lengths, front)
+    N, Sn = off[-1] + behind, len(lengths)
+    gate = (torch.randn(N, dim, generator=g) * 2 + 1).clamp(-5, 5).to(dt)
+    x = torch.randn(N, dim, generator=g).clamp(-3, 3).to(dt)
+    h0 = torch.randn(Sn, dim, generator=g).clamp(-3, 3) if k % 2 else None
+    dh, dlast = torch.randn(N, dim, generator=g).to(dt), torch.randn(Sn, dim, generator=g)
+    mem = min(max(lengths + [1]), 1 + np.exp(5.0))
+    M = 3.0
+    ref = plain_scan(gate.double(), x.double(), off, None if h0 is None else h0.double(), dh.double(), dlast.double())
+    both = torch.cat([gate, x], 1).cuda()  # the two halves of one projection: rows of stride 2 D
+    gd, xd = both[:, :dim].detach().requires_grad_(True), both[:, dim:].detach().requires_grad_(True)
+    hd = None if h0 is None else h0.cuda().requires_grad_(True)
+    o = torch.tensor(off, dtype=torch.int64 if k % 2 else torch.int32, device="cuda")
+    h, last = S.gated_scan(gd, xd, o, hd)
+    tol_h = (8 * mem + 32) * U * M
+    close(h, ref[0], tol_h, "h")
+    close(last, ref[1], tol_h, "last")
+    got = torch.autograd.grad([h, last], [gd, xd] + ([hd] if h0 is not None else []), [dh.cuda(), dlast.cuda()])
+    big = max(ref[5], 1.0)
+    tol_G = (8 * mem + 32) * U * big
+    close(got[1], ref[3], tol_G + 4 * U * big, "dx")
+    # G, h_{t-1} - x (at most 2 M, off by tol_h) and z (1 - z) <= 1 / 4, each a few roundings of its own
+    close(got[0], ref[2], (tol_G * 2 * M + big * tol_h + 32 * U * big * 2 * M) / 4, "dgate")
+    if h0 is not None:
+        close(got[2], ref[4], tol_G, "dh0")
+    if behind:
+        assert not h[off[-1]:].any() and not got[0][off[-1]:].any() and not got[1][off[-1]:].any()
+    h2, last2 = S.gated_scan(gd, xd, o, hd)
+    assert torch.equal(h, h2) and torch.equal(last, last2)
+
+
+def test_gated_scan_gradient_against_differences():
+    g = gen(5)
+    off, D, N = [0, 3, 70, 75], 5, 75
+    gate, x, h0 = torch.randn(N, D, generator=g) + 1, torch.randn(N, D, generator=g), torch.randn(3, D, generator=g)
+    a, b = torch.randn(N, D, generator=g), torch.randn(3, D, generator=g)
+    leaves = [t.cuda().requires_grad_(True) for t in (gate, x, h0)]
+    h, last = S.gated_scan(leaves[0], leaves[1], torch.tensor(off).cuda(), leaves[2])
+    got = torch.autograd.grad((h * a.cuda()).sum() + (last * b.cuda()).sum(), leaves)
+
+    def loss(v):
+        hh, ll = plain_scan(v[0], v[1], off, v[2])
+        return float((hh * a.double()).sum() + (ll * b.double()).sum())
+
+    for i in range(3):
+        for _ in range(4):
+            d = [torch.zeros_like(t).double() for t in (gate, x, h0)]
+            d[i] = torch.randn(d[i].shape, generator=g).double()
+            step = 1e-4
+            up = [t.double() + step * e for t, e in zip((gate, x, h0), d)]
+            down = [t.double() - step * e for t, e in zip((gate, x, h0), d)]
+            diff = (loss(up) - loss(down)) / (2 * step)
+            mine = float((got[i].double().cpu() * d[i]).sum())
+            # differences: third derivatives times step^2 (below 1e-6 in all); the kernel: about 1e3 terms of fp32 accuracy
+            assert abs(diff - mine) < 1e-6 * 100 + 1000 * 32 * U, (i, diff, mine)
+
+
+def test_gated_scan_equal_lengths_and_layouts():
+    g = gen(6)
+    B, T, D = 3, 70, 36
+    base = torch.randn(B, T, 2 * D, generator=g).cuda()
+    gate, x = base[..., :D], base[..., D:]
+    h, last = S.gated_scan(gate, x)
+    off = torch.arange(0, B * T + 1, T).cuda()
+    h2, last2 = S.gated_scan(gate.reshape(B * T, D), x.reshape(B * T, D), off)
+    assert torch.equal(h.reshape(B * T, D), h2) and torch.equal(last, last2)
+    for view in (lambda t: t.transpose(0, 1).contiguous().transpose(0, 1), lambda t: t.transpose(1, 2).contiguous().transpose(1, 2)):
+        h3, last3 = S.gated_scan(view(gate), view(x))
+        assert torch.equal(h, h3) and torch.equal(last, last3)
+    one, last4 = S.gated_scan(gate[:, :1], x[:, :1])  # length one, rows of stride T 2 D
+    assert torch.equal(one, h[:, :1]) and torch.equal(last4, h[:, 0])
+    none, last5 = S.gated_scan(gate[:, :0], x[:, :0], h0=torch.ones(B, D, device="cuda"))
+    assert none.shape == (B, 0, D) and torch.equal(last5, torch.ones(B, D, device="cuda"))
+    gl, xl = gate.detach().requires_grad_(True), x.detach().requires_grad_(True)
+    dg, dx = torch.autograd.grad(S.gated_scan(gl, xl)[0].sum(), [gl, xl])  # dh of stride 0, no dlast
+    dg2, dx2 = torch.autograd.grad(S.gated_scan(gl, xl)[0], [gl, xl], torch.ones(B, T, D, device="cuda"))
+    assert torch.equal(dg, dg2) and torch.equal(dx, dx2)
+    h0 = torch.randn(B, D, generator=g).cuda().requires_grad_(True)
+    dh0, = torch.autograd.grad(S.gated_scan(gl, xl, h0=h0)[1].sum(), [h0])  # dlast alone
+    want = torch.sigmoid(gate.double()).prod(1)
+    close(dh0, want.cpu(), 8 * T * U, "dh0 of the last state")
+
+
+def test_gated_scan_extreme_gates():
+    inf = float("inf")
+    gate = torch.tensor([[inf, -inf, 200.0, -200.0, 100.0, 0.0]] * 3, device="cuda")
+    x = torch.tensor([[1.0, 2.0, 3.0, 4.0, 5.0, 6.0]] * 3, device="cuda")
+    h0 = torch.full((1, 6), 7.0, device="cuda")
+    h, last = S.gated_scan(gate[None], x[None], h0=h0)
+    assert torch.equal(h[0, -1].cpu(), torch.tensor([7.0, 2.0, 7.0, 4.0, 7.0, 6.125]))
+    bad = x.clone()
+    bad[1, 0] = float("nan")  # a NaN stays in its own sequence and channel
+    two = torch.cat([bad, x])
+    h, _ = S.gated_scan(torch.zeros_like(two), two, torch.tensor([0, 3, 6]).cuda())
+    assert torch.isnan(h[1:3, 0]).all() and torch.isfinite(h[3:]).all() and torch.isfinite(h[:, 1:]).all() and torch.isfinite(h[0]).all()
+
+
+def test_gated_scan_offsets_outside_the_rows_count_as_the_nearer_end():
+    g = gen(8)
+    gate, x = torch.randn(90, 8, generator=g).cuda(), torch.randn(90, 8, generator=g).cuda()
+    h, last = S.gated_scan(gate, x, torch.tensor([-5, 40, 200]).cuda())
+    h2, last2 = S.gated_scan(gate, x, torch.tensor([0, 40, 90]).cuda())
+    assert torch.equal(h, h2) and torch.equal(last, last2)
+
+
+# ------------------------------------------------------------------------------------------------------------------- step
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("rows,pool,dim", [(1, 1, 1), (5, 9, 7), (64, 64, 501), (65, 300, 256), (300, 200, 68)])
+def test_gated_step(dtype, rows, pool, dim):
+    dt, g = DT[dtype], gen(rows + dim)
+    gate, x = (torch.randn(rows, dim, generator=g) * 2).to(dt), torch.randn(rows, dim, generator=g).clamp(-3, 3).to(dt)
+    state = torch.randn(pool, dim, generator=g).clamp(-3, 3)
+    slots = torch.randint(-2, pool + 2, (rows,), generator=g)  # padding rows and repeated slots among them
+    ref, want = state.double().clone(), torch.zeros(rows, dim, dtype=torch.float64)
+    longest = 1
+    for b in range(rows):
+        k = int(slots[b])
+        if 0 <= k < pool:
+            z, omz = torch.sigmoid(gate[b].double()), torch.sigmoid(-gate[b].double())
+            ref[k] = z * ref[k] + omz * x[b].double()
+            want[b] = ref[k]
+            longest = max(longest, int((slots == k).sum()))
+    both, sd = torch.cat([gate, x], 1).cuda(), state.cuda()
+    h = S.gated_step(both[:, :dim], both[:, dim:], sd, slots.cuda() if dim % 2 else slots.to(torch.int32).cuda())
+    tol = (8 * longest + 32) * U * 3
+    close(h, want, tol, "h")
+    close(sd, ref, tol, "state")
+    untouched = torch.ones(pool, dtype=torch.bool)
+    untouched[slots[(slots >= 0) & (slots < pool)]] = False
+    assert torch.equal(sd.cpu()[untouched], state[untouched])
+
+
+def test_gated_step_continues_a_scan():
+    """a prompt read in at once and then token by token gives what the scan over all of it gives"""
+    g = gen(9)
+    lengths, D, more = [5, 1, 130, 0], 96, 3
+    Sn = len(lengths)
+    full = [torch.randn(n + more, 2 * D, generator=g).cuda() for n in lengths]
+    prompt = torch.cat([f[:n] for f, n in zip(full, lengths)])
+    h, last = S.gated_scan(prompt[:, :D], prompt[:, D:], torch.tensor(offsets_of(lengths)).cuda())
+    pool = torch.zeros(9, D, device="cuda")
+    slots = torch.tensor([7, 0, 3, 4]).cuda()
+    pool[slots] = last
+    outs = [S.gated_step(t[:, :D], t[:, D:], pool, slots) for t in (torch.stack([f[n + i] for f, n in zip(full, lengths)]) for i in range(more))]
+    allrows = torch.cat(full)
+    off = offsets_of([n + more for n in lengths])
+    ref, _ = plain_scan(allrows[:, :D].double().cpu(), allrows[:, D:].double().cpu(), off, None)
+    tol = (8 * 133 + 32) * U * float(allrows.abs().max())
+    for i in range(more):
+        close(outs[i], torch.stack([ref[off[s] + lengths[s] + i] for s in range(Sn)]), tol, "token %d" % i)
+
+
+# ------------------------------------------------------------------------------------------------------ streams and graphs
+
+def test_sequence_operators_on_two_streams_at_once():
+    g = gen(11)
+    jobs = []
+    for k in range(2):
+        w = torch.randn(50, 64, generator=g).cuda().requires_grad_(True)
+        ids = torch.randint(0, 50, (9000,), generator=g).cuda()
+        gate, x = (torch.randn(9000, 64, generator=g).cuda().requires_grad_(True) for _ in range(2))
+        off = torch.tensor([0, 10, 4000 + k, 9000]).cuda()
+        jobs.append((w, ids, gate, x, off))
+
+    def work(w, ids, gate, x, off):
+        e = S.embed(w, ids, 2.0)
+        h, last = S.gated_scan(gate, e, off)
+        return [h.detach(), last.detach()] + list(torch.autograd.grad([h, last], [w, gate], [torch.ones_like(h), torch.ones_like(last)]))
+
+    want = [work(*j) for j in jobs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in jobs]
+    got = [None, None]
+    for _ in range(3):
+        for k, j in enumerate(jobs):
+            with torch.cuda.stream(streams[k]):
+                got[k] = work(*j)
+    torch.cuda.synchronize()
+    for a, b in zip(want, got):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_sequence_operators_captured_and_replayed():
+    g = gen(12)
+    D, N = 72, 9000
+    w = torch.randn(40, D, generator=g).cuda().requires_grad_(True)
+    gate = torch.randn(N, D, generator=g).cuda().requires_grad_(True)
+    ids, off = torch.randint(-1, 40, (N,), generator=g).cuda(), torch.tensor([0, 100, 100, 8000, N]).cuda()
+    state, slots = torch.zeros(6, D, device="cuda"), torch.tensor([3, 1, 3]).cuda()
+
+    def work():
+        h, last = S.gated_scan(gate, S.embed(w, ids, 2.0), off)
+        dw, dg = torch.autograd.grad([h, last], [w, gate], [torch.ones_like(h), torch.ones_like(last)])
+        step = S.gated_step(gate.detach()[:3], h.detach()[:3], state, slots)
+        return [h.detach(), last.detach(), dw, dg, step, state]
+
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        work()
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        out = work()
+    for k in range(4):
+        with torch.no_grad():
+            gate.copy_(torch.randn(N, D, generator=g))
+            ids.copy_(torch.randint(-1, 40, (N,), generator=g))
+            off.copy_(torch.tensor([0, 5 * k, 700, 7000 + k, N]))
+            state.fill_(float(k))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in out]
+        with torch.no_grad():
+            state.fill_(float(k))
+        want = work()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), k

@@ -1,0 +1,66 @@
+"""What the sequence operators refuse, on the CPU: nothing here launches a kernel."""
+import ctypes as C
+
+import pytest
+import torch
+
+from _dvae_pkg import dvae_amd
+
+S, L = dvae_amd.sequence, dvae_amd._lib
+
+
+def test_cpu_tensors_are_refused():
+    with pytest.raises(L.DvaeHipError, match="no CPU fallback"):
+        S.embed(torch.zeros(3, 4), torch.zeros(2, dtype=torch.int64))
+    with pytest.raises(L.DvaeHipError, match="no CPU fallback"):
+        S.gated_scan(torch.zeros(1, 3, 4), torch.zeros(1, 3, 4))
+    with pytest.raises(L.DvaeHipError, match="no CPU fallback"):
+        S.gated_step(torch.zeros(3, 4), torch.zeros(3, 4), torch.zeros(3, 4))
+
+
+def test_wrong_types_and_ranks_are_refused():
+    with pytest.raises(ValueError, match="2 dimensions"):
+        S.embed(torch.zeros(4), torch.zeros(2, dtype=torch.int64))
+    with pytest.raises(ValueError, match="float32, bfloat16 or float16"):
+        S.embed(torch.zeros(3, 4, dtype=torch.float64), torch.zeros(2, dtype=torch.int64))
+    with pytest.raises(ValueError, match="3 dimensions"):
+        S.gated_scan(torch.zeros(3, 4), torch.zeros(3, 4))
+    with pytest.raises(ValueError, match="2 dimensions"):
+        S.gated_scan(torch.zeros(1, 3, 4), torch.zeros(1, 3, 4), torch.zeros(2, dtype=torch.int32))
+
+
+def rc(name, *args):
+    lib = L.load()
+    code = getattr(lib, name)(*args)
+    assert code < 0, "%s was not refused" % name
+    return lib.dvae_last_error().decode()
+
+
+def test_the_c_entries_refuse_bad_sizes_before_any_launch():
+    p = C.c_void_p(4096)  # never read: every call below is refused on the host
+    assert "element type" in rc("dvae_embed_fwd", p, 8, p, 0, p, 4, 4, 8, 1.0, 7, None)
+    assert "row stride" in rc("dvae_embed_fwd", p, 7, p, 0, p, 4, 4, 8, 1.0, 0, None)
+    assert "null" in rc("dvae_embed_fwd", None, 8, p, 0, p, 4, 4, 8, 1.0, 0, None)
+    assert "tokens" in rc("dvae_embed_fwd", p, 8, p, 0, p, -1, 4, 8, 1.0, 0, None)
+    assert "table" in rc("dvae_embed_fwd", p, 8, p, 0, p, 4, 0, 8, 1.0, 0, None)
+    assert "row length" in rc("dvae_embed_fwd", p, 8, p, 0, p, 4, 4, 0, 1.0, 0, None)
+    assert "null" in rc("dvae_embed_bwd", p, 8, p, 0, None, p, 4, 4, 8, 1.0, 0, None)
+    assert "aligned" in rc("dvae_embed_bwd", p, 8, p, 0, p, C.c_void_p(4097), 4, 4, 8, 1.0, 0, None)
+    assert "table" in rc("dvae_embed_bwd_ws_bytes", 4, 0, 8)
+    assert "one length" in rc("dvae_scan_fwd", p, 8, p, 8, None, 0, None, p, p, None, p, 7, 2, 8, 0, None)
+    assert "null" in rc("dvae_scan_fwd", p, 8, p, 8, None, 0, None, p, None, None, p, 8, 2, 8, 0, None)
+    assert "row stride" in rc("dvae_scan_fwd", p, 8, p, 4, None, 0, None, p, p, None, p, 8, 2, 8, 0, None)
+    assert "channels" in rc("dvae_scan_fwd", p, 8, p, 8, None, 0, None, p, p, None, p, 8, 2, 0, 0, None)
+    assert "null" in rc("dvae_scan_bwd", p, 8, p, 8, None, 0, None, None, p, 8, p, p, p, p, p, 8, 2, 8, 0, None)
+    assert "element type" in rc("dvae_scan_bwd", p, 8, p, 8, None, 0, None, p, p, 8, p, p, p, p, p, 8, 2, 8, 3, None)
+    assert "rows" in rc("dvae_scan_ws_bytes", -1, 8)
+    assert "pool" in rc("dvae_scan_step", p, 8, p, 8, p, 8, 3, None, 0, p, 4, 8, 0, None)
+    assert "row stride" in rc("dvae_scan_step", p, 8, p, 8, p, 7, 4, None, 0, p, 4, 8, 0, None)
+    assert "null" in rc("dvae_scan_step", p, 8, p, 8, None, 8, 4, None, 0, p, 4, 8, 0, None)
+
+
+def test_workspace_sizes_grow_with_the_work():
+    lib = L.load()
+    assert lib.dvae_scan_state_floats(0, 8) == 0 and lib.dvae_scan_state_floats(1, 8) == 8
+    assert lib.dvae_scan_state_floats(1 << 39, 8) > 1 << 32  # 64 bits all the way
+    assert lib.dvae_embed_bwd_ws_bytes(1 << 20, 1 << 20, 1 << 12) > 1 << 30
