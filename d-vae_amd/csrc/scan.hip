@@ -75,12 +75,58 @@ __device__ __forceinline__ long seq_of(const Marks& m, int i) {
     return ((long)hi << 32) | (unsigned)lo;
 }
 
-// z = sigmoid(g) and 1 - z, neither by a subtraction
+// z = sigmoid(g) and 1 - z.  The smaller of the two (at most 1/2) is exp(-|g|) / (1 + exp(-|g|)), good to a few ulp; the
+// other is 1 minus it, good to half an ulp of 1 and unbiased, so that products of hundreds of z near 1 do not drift.
 __device__ __forceinline__ void gate_of(float g, float& z, float& omz) {
-    const float t = __expf(-fabsf(g)), r = __builtin_amdgcn_rcpf(1.f + t), u = t * r;
-    z = g >= 0.f ? r : u;
-    omz = g >= 0.f ? u : r;
-    if (g != g) z = omz = g;
+    const float t = __expf(-fabsf(g));
+    const float less = t * __builtin_amdgcn_rcpf(1.f + t), more = 1.f - less;
+    z = g >= 0.f ? more : less;
+    omz = g >= 0.f ? less : more;
+}
+
+// A run of rows as a map of the state (or of the gradient that flows back) before it: s -> A s + B.  A = 0 says that a
+// sequence begins inside, so that nothing of s is left, not even a NaN; a product of gates is kept above 0 for that.
+__device__ __forceinline__ float through(float A, float B, float s) { return A == 0.f ? B : fmaf(A, s, B); }
+constexpr float A_MIN = 1.17549435e-38f;
+
+// Carries between the tiles of a slab.  Every tile publishes its (A, B) per channel as soon as it has it, and then the
+// state behind it as (0, state), which is the same map with everything before it folded in.  A tile looks back over up to
+// LOOK published maps to the nearest whose A is 0 and applies the ones in between in order, oldest first: the sums are
+// those of walking the tiles one by one, whatever the timing, so results do not vary.  64-bit relaxed atomics at device
+// scope; a word that still holds the fill pattern has not been published, so no fences are needed.
+constexpr int LOOK = 16;
+constexpr unsigned long long UNSET = ~0ull;
+__device__ __forceinline__ void publish(unsigned long long* at, float A, float B) {
+    const unsigned long long w = ((unsigned long long)__float_as_uint(A) << 32) | __float_as_uint(B);
+    __hip_atomic_store(at, w == UNSET ? w ^ 1 : w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+// `ahead`: the words of the tiles before this one in walking order, nearest first, `step` apart; `count` of them exist.
+__device__ __forceinline__ float look_back(const unsigned long long* nearest, long step, long count) {
+    const int n = (int)min(count, (long)LOOK);
+    for (int spin = 0; spin < (1 << 20); ++spin) {
+        unsigned long long w[LOOK];
+#pragma unroll
+        for (int i = 0; i < LOOK; ++i)
+            w[i] = i < n ? __hip_atomic_load(nearest + i * step, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
+        int from = -1;  // the nearest whole state, if everything nearer is published
+        bool open = true;
+#pragma unroll
+        for (int i = 0; i < LOOK; ++i) {
+            if (w[i] == UNSET) open = false;
+            // (past the first tile of all the state is zero)
+            if (open && from < 0 && (i >= n ? count <= LOOK : (w[i] >> 32) == 0)) from = i;
+        }
+        if (open && from < 0 && count <= LOOK && n == LOOK) from = LOOK;
+        if (__all(from >= 0)) {
+            float s = 0.f;
+#pragma unroll
+            for (int i = LOOK - 1; i >= 0; --i)
+                if (i <= from && i < n) s = through(__uint_as_float((unsigned)(w[i] >> 32)), __uint_as_float((unsigned)w[i]), s);
+            return s;
+        }
+        __builtin_amdgcn_s_sleep(1);
+    }
+    return __uint_as_float(0x7FC00000u);  // not reached: every tile waits for earlier tickets only; NaN rather than a hang
 }
 
 struct ScanParams {
@@ -90,8 +136,8 @@ struct ScanParams {
     const float *h0, *dlast;        // [S][D] or nullptr
     float *last, *dh0;              // [S][D]
     float *states;                  // [tiles][D]: the state before each tile
-    float2 *agg;                    // [tiles][D]: a tile's (A, B)
-    float *carry;                   // [tiles][D]: backward: what flows into a tile from behind
+    unsigned long long* words;      // [tiles][D]: a tile's map, as published
+    unsigned* ticket;
     Rows q;
     int D, slabs;
 };
@@ -101,14 +147,22 @@ template <int V> __device__ __forceinline__ void load_init(float (&h)[V], const 
     for (int j = 0; j < V; ++j) h[j] = p && live ? p[seq * D + c + j] : 0.f;
 }
 
-// Forward.  APPLY = false: the tile's (A, B); true: h, given the state before the tile.
-template <typename T, int V, int RW, int W, bool APPLY>
+// Tiles are taken by ticket, in walking order: a tile's predecessors have always begun, so every wait ends.
+__device__ __forceinline__ unsigned take_ticket(unsigned* ticket) {
+    __shared__ unsigned mine;
+    if (threadIdx.x == 0) mine = atomicAdd(ticket, 1u);
+    __syncthreads();
+    return mine;
+}
+
+template <typename T, int V, int RW, int W>
 __global__ __launch_bounds__(W * 64) void scan_fwd_kernel(ScanParams p) {
-    static_assert(RW * W == TR, "");
-    __shared__ float As[W][64 * V], Bs[W][64 * V];
+    static_assert(RW * W == TR && W >= V, "");
+    __shared__ float As[W][64 * V], Bs[W][64 * V], Cs[64 * V];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int c = (int)(blockIdx.x % (unsigned)p.slabs) * 64 * V + lane * V;
-    const long tile = blockIdx.x / (unsigned)p.slabs, t0 = tile * TR + wave * RW;
+    const unsigned unit = __builtin_amdgcn_readfirstlane(take_ticket(p.ticket));
+    const int c0 = (int)(unit % (unsigned)p.slabs) * 64 * V, c = c0 + lane * V;
+    const long tile = unit / (unsigned)p.slabs, t0 = tile * TR + wave * RW;
     const bool live = c < p.D;
     Pack<T, V> g[RW], x[RW];
 #pragma unroll
@@ -118,50 +172,50 @@ __global__ __launch_bounds__(W * 64) void scan_fwd_kernel(ScanParams p) {
             x[i] = load_pack<T, V>((const T*)p.x + (t0 + i) * p.ld_x + c);
         }
     const Marks m = mark_rows<RW>(p.q, t0);
-    float A[V], h[V];
+    float A[V], h[V], z[RW][V], b[RW][V];
 #pragma unroll
     for (int j = 0; j < V; ++j) { A[j] = 1.f; h[j] = 0.f; }
-    if (t0 < p.q.N) {
 #pragma unroll
-        for (int i = 0; i < RW; ++i) {
-            if ((m.start >> i) & 1) {
-                load_init<V>(h, p.h0, seq_of(m, i), p.D, c, live);
+    for (int i = 0; i < RW; ++i) {
+        if ((m.start >> i) & 1) {
+            load_init<V>(h, p.h0, seq_of(m, i), p.D, c, live);
 #pragma unroll
-                for (int j = 0; j < V; ++j) A[j] = 0.f;
-            }
-            if ((m.cover >> i) & 1)
-#pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    float z, omz;
-                    gate_of((float)g[i].e[j], z, omz);
-                    h[j] = fmaf(z, h[j], omz * (float)x[i].e[j]);
-                    A[j] *= z;
-                }
+            for (int j = 0; j < V; ++j) A[j] = 0.f;
         }
+        if ((m.cover >> i) & 1)
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                float omz;
+                gate_of((float)g[i].e[j], z[i][j], omz);
+                b[i][j] = omz * (float)x[i].e[j];
+                h[j] = fmaf(z[i][j], h[j], b[i][j]);
+                A[j] = A[j] == 0.f ? 0.f : fmaxf(A[j] * z[i][j], A_MIN);
+            }
     }
 #pragma unroll
     for (int j = 0; j < V; ++j) { As[wave][lane * V + j] = A[j]; Bs[wave][lane * V + j] = h[j]; }
     __syncthreads();
-    if (!APPLY) {
-        if (wave == 0 && live) {
+    if (wave < V && c0 + (int)threadIdx.x < p.D) {  // one thread per channel from here to the barrier
+        const int k = threadIdx.x;
+        float a = 1.f, y = 0.f;
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                float a = 1.f, b = 0.f;
-#pragma unroll
-                for (int w = 0; w < W; ++w) {
-                    b = fmaf(As[w][lane * V + j], b, Bs[w][lane * V + j]);
-                    a *= As[w][lane * V + j];
-                }
-                p.agg[tile * p.D + c + j] = make_float2(a, b);
-            }
+        for (int w = 0; w < W; ++w) {
+            y = through(As[w][k], Bs[w][k], y);
+            a = As[w][k] == 0.f ? 0.f : a == 0.f ? 0.f : fmaxf(a * As[w][k], A_MIN);
         }
-        return;
+        unsigned long long* word = p.words + tile * p.D + c0 + k;
+        publish(word, a, y);
+        const float s = tile == 0 ? 0.f : look_back(word - p.D, -(long)p.D, tile);
+        if (a != 0.f) publish(word, 0.f, through(a, y, s));
+        if (p.states) p.states[tile * p.D + c0 + k] = s;
+        Cs[k] = s;
     }
-    if (!live || t0 >= p.q.N) return;
+    __syncthreads();
+    if (!live) return;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        float s = p.states[tile * p.D + c + j];
-        for (int w = 0; w < wave; ++w) s = fmaf(As[w][lane * V + j], s, Bs[w][lane * V + j]);
+        float s = Cs[lane * V + j];
+        for (int w = 0; w < wave; ++w) s = through(As[w][lane * V + j], Bs[w][lane * V + j], s);
         h[j] = s;
     }
 #pragma unroll
@@ -172,9 +226,7 @@ __global__ __launch_bounds__(W * 64) void scan_fwd_kernel(ScanParams p) {
         float o[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            float z, omz;
-            gate_of((float)g[i].e[j], z, omz);
-            if (cover) h[j] = fmaf(z, h[j], omz * (float)x[i].e[j]);
+            if (cover) h[j] = fmaf(z[i][j], h[j], b[i][j]);
             o[j] = cover ? h[j] : 0.f;
         }
         store_floats<T, V>((T*)p.h + (t0 + i) * p.D + c, o);
@@ -186,14 +238,15 @@ __global__ __launch_bounds__(W * 64) void scan_fwd_kernel(ScanParams p) {
     }
 }
 
-// Backward.  APPLY = false: the tile's (A, B) from its end to its begin; true: the gradients.
-template <typename T, int V, int RW, int W, bool APPLY>
+// Backward: the tiles are walked from the last; what flows from a tile to the one before it is z_t G_t of its first row.
+template <typename T, int V, int RW, int W>
 __global__ __launch_bounds__(W * 64) void scan_bwd_kernel(ScanParams p) {
-    static_assert(RW * W == TR, "");
-    __shared__ float As[W][64 * V], Bs[W][64 * V], Fs[W][64 * V];
+    static_assert(RW * W == TR && W >= V, "");
+    __shared__ float As[W][64 * V], Bs[W][64 * V], Fs[W][64 * V], Cs[64 * V];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int c = (int)(blockIdx.x % (unsigned)p.slabs) * 64 * V + lane * V;
-    const long tile = blockIdx.x / (unsigned)p.slabs, t0 = tile * TR + wave * RW;
+    const unsigned unit = __builtin_amdgcn_readfirstlane(take_ticket(p.ticket));
+    const int c0 = (int)(unit % (unsigned)p.slabs) * 64 * V, c = c0 + lane * V;
+    const long tiles = (p.q.N + TR - 1) / TR, tile = tiles - 1 - unit / (unsigned)p.slabs, t0 = tile * TR + wave * RW;
     const bool live = c < p.D;
     Pack<T, V> g[RW], x[RW], d[RW];
 #pragma unroll
@@ -201,7 +254,7 @@ __global__ __launch_bounds__(W * 64) void scan_bwd_kernel(ScanParams p) {
         if (live && t0 + i < p.q.N) {
             g[i] = load_pack<T, V>((const T*)p.gate + (t0 + i) * p.ld_gate + c);
             if (p.dh) d[i] = load_pack<T, V>((const T*)p.dh + (t0 + i) * p.ld_dh + c);
-            if (APPLY) x[i] = load_pack<T, V>((const T*)p.x + (t0 + i) * p.ld_x + c);
+            x[i] = load_pack<T, V>((const T*)p.x + (t0 + i) * p.ld_x + c);
         }
     const Marks m = mark_rows<RW>(p.q, t0);
     auto row_grad = [&](int i, float (&e)[V]) {  // dh of row i, and dlast where the sequence ends
@@ -213,81 +266,71 @@ __global__ __launch_bounds__(W * 64) void scan_bwd_kernel(ScanParams p) {
             for (int j = 0; j < V; ++j) e[j] += live ? p.dlast[s * p.D + c + j] : 0.f;
         }
     };
-    float A[V], B[V], h[V];
+    float A[V], B[V], h[V], z[RW][V], omz[RW][V];
 #pragma unroll
     for (int j = 0; j < V; ++j) { A[j] = 1.f; B[j] = 0.f; h[j] = 0.f; }
-    if (t0 < p.q.N) {
 #pragma unroll
-        for (int i = RW - 1; i >= 0; --i) {
-            if (!((m.cover >> i) & 1)) continue;
-            float e[V];
-            row_grad(i, e);
+    for (int i = 0; i < RW; ++i) {  // this wave's part of the forward scan
+        if ((m.start >> i) & 1) load_init<V>(h, p.h0, seq_of(m, i), p.D, c, live);
+        if ((m.cover >> i) & 1)
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                float z, omz;
-                gate_of((float)g[i].e[j], z, omz);
-                const bool first = (m.start >> i) & 1;
-                B[j] = first ? 0.f : z * (e[j] + B[j]);
-                A[j] = first ? 0.f : A[j] * z;
+                gate_of((float)g[i].e[j], z[i][j], omz[i][j]);
+                h[j] = fmaf(z[i][j], h[j], omz[i][j] * (float)x[i].e[j]);
             }
-        }
-        if (APPLY) {  // this wave's part of the forward scan (its A is the same product)
-#pragma unroll
-            for (int i = 0; i < RW; ++i) {
-                if ((m.start >> i) & 1) load_init<V>(h, p.h0, seq_of(m, i), p.D, c, live);
-                if ((m.cover >> i) & 1)
-#pragma unroll
-                    for (int j = 0; j < V; ++j) {
-                        float z, omz;
-                        gate_of((float)g[i].e[j], z, omz);
-                        h[j] = fmaf(z, h[j], omz * (float)x[i].e[j]);
-                    }
-            }
-        }
     }
+#pragma unroll
+    for (int i = RW - 1; i >= 0; --i)
+        if ((m.cover >> i) & 1) {
+            float e[V];
+            row_grad(i, e);
+            const bool first = (m.start >> i) & 1;
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                B[j] = first ? 0.f : z[i][j] * (e[j] + B[j]);
+                A[j] = first || A[j] == 0.f ? 0.f : fmaxf(A[j] * z[i][j], A_MIN);
+            }
+        }
 #pragma unroll
     for (int j = 0; j < V; ++j) {
         As[wave][lane * V + j] = A[j];
         Bs[wave][lane * V + j] = B[j];
-        if (APPLY) Fs[wave][lane * V + j] = h[j];
+        Fs[wave][lane * V + j] = h[j];
     }
     __syncthreads();
-    if (!APPLY) {
-        if (wave == 0 && live) {
+    if (wave < V && c0 + (int)threadIdx.x < p.D) {
+        const int k = threadIdx.x;
+        float a = 1.f, y = 0.f;
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                float a = 1.f, b = 0.f;
-#pragma unroll
-                for (int w = W - 1; w >= 0; --w) {
-                    b = fmaf(As[w][lane * V + j], b, Bs[w][lane * V + j]);
-                    a *= As[w][lane * V + j];
-                }
-                p.agg[tile * p.D + c + j] = make_float2(a, b);
-            }
+        for (int w = W - 1; w >= 0; --w) {
+            y = through(As[w][k], Bs[w][k], y);
+            a = As[w][k] == 0.f ? 0.f : a == 0.f ? 0.f : fmaxf(a * As[w][k], A_MIN);
         }
-        return;
+        unsigned long long* word = p.words + tile * p.D + c0 + k;
+        publish(word, a, y);
+        const float s = tile == tiles - 1 ? 0.f : look_back(word + p.D, p.D, tiles - 1 - tile);
+        if (a != 0.f) publish(word, 0.f, through(a, y, s));
+        Cs[k] = s;
     }
+    __syncthreads();
     if (!live || t0 >= p.q.N) return;
-    float C[V];
+    float C[V], prev[RW][V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
         float s = p.states[tile * p.D + c + j];
-        for (int w = 0; w < wave; ++w) s = fmaf(As[w][lane * V + j], s, Fs[w][lane * V + j]);
+        for (int w = 0; w < wave; ++w) s = through(As[w][lane * V + j], Fs[w][lane * V + j], s);
         h[j] = s;
-        s = p.carry[tile * p.D + c + j];
-        for (int w = W - 1; w > wave; --w) s = fmaf(As[w][lane * V + j], s, Bs[w][lane * V + j]);
+        s = Cs[lane * V + j];
+        for (int w = W - 1; w > wave; --w) s = through(As[w][lane * V + j], Bs[w][lane * V + j], s);
         C[j] = s;
     }
-    float prev[RW][V];
 #pragma unroll
     for (int i = 0; i < RW; ++i) {
         if ((m.start >> i) & 1) load_init<V>(h, p.h0, seq_of(m, i), p.D, c, live);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             prev[i][j] = h[j];
-            float z, omz;
-            gate_of((float)g[i].e[j], z, omz);
-            if ((m.cover >> i) & 1) h[j] = fmaf(z, h[j], omz * (float)x[i].e[j]);
+            if ((m.cover >> i) & 1) h[j] = fmaf(z[i][j], h[j], omz[i][j] * (float)x[i].e[j]);
         }
     }
 #pragma unroll
@@ -298,12 +341,10 @@ __global__ __launch_bounds__(W * 64) void scan_bwd_kernel(ScanParams p) {
         row_grad(i, e);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            float z, omz;
-            gate_of((float)g[i].e[j], z, omz);
             const float G = e[j] + C[j];
-            og[j] = cover ? G * (prev[i][j] - (float)x[i].e[j]) * z * omz : 0.f;
-            ox[j] = cover ? G * omz : 0.f;
-            if (cover) C[j] = z * G;
+            og[j] = cover ? G * (prev[i][j] - (float)x[i].e[j]) * z[i][j] * omz[i][j] : 0.f;
+            ox[j] = cover ? G * omz[i][j] : 0.f;
+            if (cover) C[j] = z[i][j] * G;
         }
         store_floats<T, V>((T*)p.dgate + (t0 + i) * p.D + c, og);
         store_floats<T, V>((T*)p.dx + (t0 + i) * p.D + c, ox);
@@ -319,25 +360,19 @@ __global__ __launch_bounds__(W * 64) void scan_bwd_kernel(ScanParams p) {
     }
 }
 
-// the state before every tile, tile by tile (REV: what flows into a tile from behind)
-template <bool REV> __global__ __launch_bounds__(64) void scan_carry_kernel(const float2* __restrict__ agg, float* __restrict__ out, long tiles, int D) {
-    const int c = blockIdx.x * 64 + threadIdx.x;
-    if (c >= D) return;
-    float s = 0.f;
-    for (long k = 0; k < tiles; ++k) {
-        const long t = REV ? tiles - 1 - k : k;
-        const float2 ab = agg[t * D + c];
-        out[t * D + c] = s;
-        s = fmaf(ab.x, s, ab.y);
+// Before either pass: nothing is published yet, ticket 0 is next; and the sequences without rows, whose last state is the
+// first (and whose gradient goes straight through).  Workgroups behind `fill_blocks` take four sequences each.
+__global__ __launch_bounds__(256) void scan_begin_kernel(ulonglong2* __restrict__ words, long pairs, unsigned* __restrict__ ticket,
+                                                         int fill_blocks, Rows q, const float* __restrict__ from,
+                                                         float* __restrict__ to, int D) {
+    if ((int)blockIdx.x < fill_blocks) {
+        if (blockIdx.x == 0 && threadIdx.x == 0) *ticket = 0;
+        for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < pairs; i += (long)fill_blocks * 256) words[i] = make_ulonglong2(UNSET, UNSET);
+        return;
     }
-}
-
-// sequences without rows: the last state is the first, and its gradient goes straight through
-__global__ __launch_bounds__(256) void scan_empty_kernel(Rows q, const float* __restrict__ from, float* __restrict__ to, int D) {
-    const long s = blockIdx.x;
-    const long b = q.off ? q.at(s) : 0, e = q.off ? q.at(s + 1) : q.len;
-    if (b < e) return;
-    for (int c = threadIdx.x; c < D; c += 256) to[s * D + c] = from ? from[s * D + c] : 0.f;
+    const long s = ((long)blockIdx.x - fill_blocks) * 4 + (threadIdx.x >> 6);
+    if (s >= q.S || (q.off ? q.at(s) < q.at(s + 1) : q.len > 0)) return;
+    for (int c = threadIdx.x & 63; c < D; c += 64) to[s * D + c] = from ? from[s * D + c] : 0.f;
 }
 
 // ------------------------------------------------------------------------------------------------------- single tokens
@@ -403,15 +438,14 @@ static int scan_check(const char* who, int64_t rows, int64_t seqs, const void* o
 }
 
 struct ScanWs {
-    int64_t agg, carry, bytes;  // byte offsets
+    int64_t words, bytes;  // [16 bytes: the ticket][words, to a whole number of 16 bytes]
     int64_t tiles;
 };
 static ScanWs scan_ws(int64_t rows, int64_t D) {
     ScanWs w;
     w.tiles = (rows + TR - 1) / TR;
-    w.agg = 0;
-    w.carry = w.tiles * D * 8;
-    w.bytes = w.carry + w.tiles * D * 4;
+    w.words = 16;
+    w.bytes = w.words + (w.tiles * D + 1) / 2 * 16;
     return w;
 }
 
@@ -429,9 +463,16 @@ static ScanWs scan_ws(int64_t rows, int64_t D) {
         }                                                                                       \
     } while (0)
 
-static int scan_empty(const Rows& q, const float* from, float* to, int D, hipStream_t s) {
-    if (q.S == 0 || (!q.off && q.len > 0)) return DVAE_OK;
-    hipLaunchKernelGGL(scan_empty_kernel, dim3((unsigned)q.S), dim3(256), 0, s, q, from, to, D);
+static int scan_begin(ScanParams& p, void* ws, const ScanWs& L, const float* from, float* to, hipStream_t s) {
+    p.ticket = (unsigned*)ws;
+    p.words = (unsigned long long*)((char*)ws + L.words);
+    const long pairs = (L.tiles * p.D + 1) / 2;
+    const int fill = L.tiles == 0 ? 0 : (int)min((pairs + 255) / 256, 2048L);
+    const bool empties = to && p.q.S > 0 && (p.q.off || p.q.len == 0);
+    const long blocks = fill + (empties ? (p.q.S + 3) / 4 : 0);
+    if (blocks == 0) return DVAE_OK;
+    hipLaunchKernelGGL(scan_begin_kernel, dim3((unsigned)blocks), dim3(256), 0, s, (ulonglong2*)p.words, pairs, p.ticket, fill,
+                       p.q, from, to, p.D);
     DVAE_LAUNCH_CHECK();
     return DVAE_OK;
 }
@@ -459,28 +500,20 @@ extern "C" int dvae_scan_fwd(const void* gate, int64_t ld_gate, const void* x, i
     DVAE_REQUIRE(seqs == 0 || last, "scan_fwd: null pointer");
     DVAE_REQUIRE((uintptr_t)ws % 16 == 0, "scan_fwd: the workspace must be 16-byte aligned");
     hipStream_t s = (hipStream_t)stream;
-    const Rows q = {off, off_i64, seqs, seqs > 0 ? rows / seqs : 0, rows};
-    DVAE_TRY(scan_empty(q, h0, last, D, s));
-    if (rows == 0) return DVAE_OK;
-    const int vec = widest(elem_size(dtype), 8, {(int64_t)D, ld_gate, ld_x}, {gate, x, (const void*)h});
     const ScanWs L = scan_ws(rows, D);
+    const int vec = widest(elem_size(dtype), 8, {(int64_t)D, ld_gate, ld_x}, {gate, x, (const void*)h});
     ScanParams p = {};
-    p.gate = gate; p.x = x; p.ld_gate = ld_gate; p.ld_x = ld_x; p.h = h; p.h0 = h0; p.last = last;
-    p.agg = (float2*)((char*)ws + L.agg);
-    p.states = states ? states : (float*)((char*)ws + L.carry);
-    p.q = q; p.D = D; p.slabs = cdiv(D, 64 * vec);
+    p.gate = gate; p.x = x; p.ld_gate = ld_gate; p.ld_x = ld_x; p.h = h; p.h0 = h0; p.last = last; p.states = states;
+    p.q = {off, off_i64, seqs, seqs > 0 ? rows / seqs : 0, rows};
+    p.D = D; p.slabs = cdiv(D, 64 * vec);
     DVAE_REQUIRE(L.tiles * p.slabs < (1LL << 31), "scan_fwd: %lld rows of %d channels are too many", (long long)rows, D);
+    DVAE_TRY(scan_begin(p, ws, L, h0, last, s));
+    if (rows == 0) return DVAE_OK;
     const dim3 grid((unsigned)(L.tiles * p.slabs));
-#define SCAN_AGG(T, V, RW, W) hipLaunchKernelGGL((scan_fwd_kernel<T, V, RW, W, false>), grid, dim3(W * 64), 0, s, p)
-#define SCAN_APPLY(T, V, RW, W) hipLaunchKernelGGL((scan_fwd_kernel<T, V, RW, W, true>), grid, dim3(W * 64), 0, s, p)
-    SCAN_BY_TYPE(dtype, vec, SCAN_AGG);
+#define SCAN_FWD(T, V, RW, W) hipLaunchKernelGGL((scan_fwd_kernel<T, V, RW, W>), grid, dim3(W * 64), 0, s, p)
+    SCAN_BY_TYPE(dtype, vec, SCAN_FWD);
+#undef SCAN_FWD
     DVAE_LAUNCH_CHECK();
-    hipLaunchKernelGGL((scan_carry_kernel<false>), dim3(cdiv(D, 64)), dim3(64), 0, s, p.agg, p.states, (long)L.tiles, D);
-    DVAE_LAUNCH_CHECK();
-    SCAN_BY_TYPE(dtype, vec, SCAN_APPLY);
-    DVAE_LAUNCH_CHECK();
-#undef SCAN_AGG
-#undef SCAN_APPLY
     return DVAE_OK;
 }
 
@@ -494,30 +527,22 @@ extern "C" int dvae_scan_bwd(const void* gate, int64_t ld_gate, const void* x, i
     DVAE_REQUIRE(rows == 0 || (gate && x && states && dgate && dx && ws), "scan_bwd: null pointer");
     DVAE_REQUIRE((uintptr_t)ws % 16 == 0, "scan_bwd: the workspace must be 16-byte aligned");
     hipStream_t s = (hipStream_t)stream;
-    const Rows q = {off, off_i64, seqs, seqs > 0 ? rows / seqs : 0, rows};
-    if (dh0) DVAE_TRY(scan_empty(q, dlast, dh0, D, s));
-    if (rows == 0) return DVAE_OK;
+    const ScanWs L = scan_ws(rows, D);
     const int vec = widest(elem_size(dtype), 8, {(int64_t)D, ld_gate, ld_x, dh ? ld_dh : 0},
                            {gate, x, dh, (const void*)dgate, (const void*)dx});
-    const ScanWs L = scan_ws(rows, D);
     ScanParams p = {};
     p.gate = gate; p.x = x; p.dh = dh; p.ld_gate = ld_gate; p.ld_x = ld_x; p.ld_dh = ld_dh;
     p.dgate = dgate; p.dx = dx; p.h0 = h0; p.dlast = dlast; p.dh0 = dh0; p.states = const_cast<float*>(states);
-    p.agg = (float2*)((char*)ws + L.agg);
-    p.carry = (float*)((char*)ws + L.carry);
-    p.q = q; p.D = D; p.slabs = cdiv(D, 64 * vec);
+    p.q = {off, off_i64, seqs, seqs > 0 ? rows / seqs : 0, rows};
+    p.D = D; p.slabs = cdiv(D, 64 * vec);
     DVAE_REQUIRE(L.tiles * p.slabs < (1LL << 31), "scan_bwd: %lld rows of %d channels are too many", (long long)rows, D);
+    DVAE_TRY(scan_begin(p, ws, L, dlast, dh0, s));
+    if (rows == 0) return DVAE_OK;
     const dim3 grid((unsigned)(L.tiles * p.slabs));
-#define SCAN_AGG(T, V, RW, W) hipLaunchKernelGGL((scan_bwd_kernel<T, V, RW, W, false>), grid, dim3(W * 64), 0, s, p)
-#define SCAN_APPLY(T, V, RW, W) hipLaunchKernelGGL((scan_bwd_kernel<T, V, RW, W, true>), grid, dim3(W * 64), 0, s, p)
-    SCAN_BY_TYPE(dtype, vec, SCAN_AGG);
+#define SCAN_BWD(T, V, RW, W) hipLaunchKernelGGL((scan_bwd_kernel<T, V, RW, W>), grid, dim3(W * 64), 0, s, p)
+    SCAN_BY_TYPE(dtype, vec, SCAN_BWD);
+#undef SCAN_BWD
     DVAE_LAUNCH_CHECK();
-    hipLaunchKernelGGL((scan_carry_kernel<true>), dim3(cdiv(D, 64)), dim3(64), 0, s, p.agg, p.carry, (long)L.tiles, D);
-    DVAE_LAUNCH_CHECK();
-    SCAN_BY_TYPE(dtype, vec, SCAN_APPLY);
-    DVAE_LAUNCH_CHECK();
-#undef SCAN_AGG
-#undef SCAN_APPLY
     return DVAE_OK;
 }
 

@@ -252,6 +252,35 @@ def test_gated_scan_extreme_gates():
     assert torch.isnan(h[1:3, 0]).all() and torch.isfinite(h[3:]).all() and torch.isfinite(h[:, 1:]).all() and torch.isfinite(h[0]).all()
 
 
+def test_gated_scan_keeps_nan_and_inf_in_their_sequence():
+    """also where a sequence begins in the middle of a tile, at its first row, or many tiles later"""
+    g = gen(7)
+    off = [0, 130, 131, 300, 320, 1920, 1984, 2100]
+    N, D = off[-1], 70
+    gate, x = torch.randn(N, D, generator=g) * 3, torch.randn(N, D, generator=g)
+    dh, dlast = torch.randn(N, D, generator=g).cuda(), torch.randn(len(off) - 1, D, generator=g).cuda()
+    bad = x.clone()
+    bad[5, 0], bad[140, 1], bad[330, 2], bad[1930, 3] = float("nan"), float("inf"), float("nan"), float("-inf")
+    hit = {0: (0, 5), 1: (2, 140), 2: (4, 330), 3: (5, 1930)}  # channel -> (its sequence, the row)
+
+    def run(xx):
+        leaves = [gate.cuda().requires_grad_(True), xx.cuda().requires_grad_(True)]
+        h, last = S.gated_scan(leaves[0], leaves[1], torch.tensor(off).cuda())
+        return [h.detach(), last.detach()] + list(torch.autograd.grad([h, last], leaves, [dh, dlast]))
+
+    good, got = run(x), run(bad)
+    h, last, dg, dx = got
+    for c in range(D):
+        keep = torch.ones(N, dtype=torch.bool)
+        if c in hit:
+            s, row = hit[c]
+            keep[off[s]:off[s + 1]] = False
+            assert not torch.isfinite(h[row:off[s + 1], c]).any() and not torch.isfinite(last[s, c])
+            assert torch.equal(h[off[s]:row, c], good[0][off[s]:row, c])
+        assert torch.equal(h[keep, c], good[0][keep, c]) and torch.equal(dg[keep, c], good[2][keep, c])
+    assert torch.equal(dx, good[3])  # dx does not depend on x
+
+
 def test_gated_scan_offsets_outside_the_rows_count_as_the_nearer_end():
     g = gen(8)
     gate, x = torch.randn(90, 8, generator=g).cuda(), torch.randn(90, 8, generator=g).cuda()
