@@ -19,7 +19,7 @@
 
 namespace dvae {
 
-constexpr int EC = 32;              // sorted tokens per chunk
+constexpr int EC = 32;              // sorted tokens per chunk (a multiple of ER, at most 62)
 constexpr int ER = 8;               // rows in flight per wave
 constexpr int SORT_ITEMS = 8;       // items per lane of a sorting tile
 constexpr int SMALL_THREADS = 1024; // one workgroup sorts up to SMALL_THREADS * SORT_ITEMS tokens by itself
@@ -157,36 +157,39 @@ __global__ __launch_bounds__(SMALL_THREADS) void sort_small_kernel(const void* _
     }
 }
 
-// digit counts of the first pass per block, and zeros for those of the later ones (counted by the pass before)
-__global__ __launch_bounds__(TILE_THREADS) void sort_count_kernel(const void* __restrict__ ids, int i64, int n, int V, int passes,
-                                                                  int per_block, int* __restrict__ hist) {
+// digit counts of pass p per block
+__global__ __launch_bounds__(TILE_THREADS) void sort_count_kernel(const void* __restrict__ ids, int i64, const int* __restrict__ key_in,
+                                                                  int n, int V, int p, int per_block, int* __restrict__ hist) {
     __shared__ int cnt[256];
     const int tid = threadIdx.x;
     cnt[tid] = 0;
     __syncthreads();
     const long beg = (long)blockIdx.x * per_block;
     const int end = (int)min((long)n, beg + per_block);
-    for (long i = beg + tid; i < end; i += TILE_THREADS) atomicAdd(&cnt[token_key(ids, i64, i, V) & 255], 1);
+    for (long i = beg + tid; i < end; i += TILE_THREADS)
+        atomicAdd(&cnt[((p == 0 ? token_key(ids, i64, i, V) : key_in[i]) >> (8 * p)) & 255], 1);
     __syncthreads();
     hist[(long)blockIdx.x * 256 + tid] = cnt[tid];
-    for (int p = 1; p < passes; ++p) hist[((long)p * gridDim.x + blockIdx.x) * 256 + tid] = 0;
 }
 
 __global__ __launch_bounds__(TILE_THREADS) void sort_pass_kernel(const void* __restrict__ ids, int i64, const int* __restrict__ key_in,
-                                                                 const int* __restrict__ pos_in, int n, int V, int p, int passes,
-                                                                 int per_block, int* __restrict__ hist, int* __restrict__ key_out,
+                                                                 const int* __restrict__ pos_in, int n, int V, int p, int per_block,
+                                                                 const int* __restrict__ hist, int* __restrict__ key_out,
                                                                  int* __restrict__ pos_out) {
     constexpr int W = TILE_THREADS / 64;
     __shared__ int cnt[W][256];
     __shared__ int wave_tot[4];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int* mine = hist + (long)p * gridDim.x * 256;
-    int* next = hist + (long)(p + 1) * gridDim.x * 256;
     int before = 0, tot = 0;
-    for (int b = 0; b < (int)gridDim.x; ++b) {
-        const int h = mine[(long)b * 256 + tid];
-        before += b < (int)blockIdx.x ? h : 0;
-        tot += h;
+    for (int b0 = 0; b0 < (int)gridDim.x; b0 += 16) {
+        int h[16];
+#pragma unroll
+        for (int u = 0; u < 16; ++u) h[u] = hist[(long)min(b0 + u, (int)gridDim.x - 1) * 256 + tid];
+#pragma unroll
+        for (int u = 0; u < 16; ++u) {
+            before += b0 + u < (int)blockIdx.x ? h[u] : 0;
+            tot += b0 + u < (int)gridDim.x ? h[u] : 0;
+        }
     }
     int base = scan256(tot, wave_tot) + before;  // where this block's items with digit `tid` begin
     const long beg = (long)blockIdx.x * per_block;
@@ -216,8 +219,6 @@ __global__ __launch_bounds__(TILE_THREADS) void sort_pass_kernel(const void* __r
                 const int d = cnt[wave][(key[r] >> (8 * p)) & 255] + rank[r];
                 key_out[d] = key[r];
                 pos_out[d] = pos[r];
-                // integer counts: the sum does not depend on the order of the atomics
-                if (p + 1 < passes) atomicAdd(&next[(long)(d / per_block) * 256 + ((key[r] >> (8 * (p + 1))) & 255)], 1);
             }
         __syncthreads();
     }
@@ -249,12 +250,15 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const T* __restrict__ do
     if ((int)blockIdx.x >= sum_blocks) {
         __shared__ unsigned long long named;
         const int r0 = ((int)blockIdx.x - sum_blocks) * ZERO_ROWS, rows = min(ZERO_ROWS, vocab - r0);
-        if (threadIdx.x == 0) named = 0;
-        __syncthreads();
-        if (wave == 0) {
-            const int lo = wave_lower_bound(key, n, r0), hi = wave_lower_bound(key, n, r0 + rows);
-            for (int i = lo + lane; i < hi; i += 64)
-                if (i == lo || key[i] != key[i - 1]) atomicOr(&named, 1ull << (key[i] - r0));
+        if (wave == 0) {  // lane r looks for row r0 + r among the tokens of the range
+            int lo = wave_lower_bound(key, n, r0), hi = wave_lower_bound(key, n, r0 + rows);
+            const int end = hi;
+            while (lo < hi) {
+                const int mid = lo + (hi - lo) / 2;
+                if (key[mid] < r0 + lane) lo = mid + 1; else hi = mid;
+            }
+            const unsigned long long mask = __ballot(lo < end && key[min(lo, n - 1)] == r0 + lane);
+            if (lane == 0) named = mask;
         }
         __syncthreads();
         const unsigned long long skip = named;
@@ -269,83 +273,95 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const T* __restrict__ do
     const int chunk = (int)(unit / slabs), c = (int)(unit % slabs) * 64 * V + lane * V;
     const int s = chunk * EC, e = min(n, s + EC);
     const bool live = c < D;
-    int cur = key[s];
+    const T* col = dout + (live ? c : D - V);  // idle lanes read the last columns
+    // the chunk's tokens, one per lane; lanes 62 and 63 have the tokens on either side of it
+    const int at = lane < EC ? min(s + lane, n - 1) : lane == 62 ? max(s - 1, 0) : min(e, n - 1);
+    const int my_key = key[at], my_pos = pos[at];
+    int cur = __builtin_amdgcn_readlane(my_key, 0);
     if (cur >= vocab) return;
-    bool head = s > 0 && key[s - 1] == cur;  // the run began in an earlier chunk
+    bool head = s > 0 && __builtin_amdgcn_readlane(my_key, 62) == cur;  // the run began in an earlier chunk
     float acc[V] = {};
-    auto to_part = [&](int which) {
-        float* p = part + ((long)2 * chunk + which) * D + c;
+    auto flush = [&](int which) {  // to the table's row, or to partial 0 (a run's continuation) or 1 (its begin)
+        if (!live) return;
+        if (which < 0) {
+            float f[V];
 #pragma unroll
-        for (int j = 0; j < V; ++j) p[j] = acc[j];
-    };
-    auto to_row = [&]() {
-        float f[V];
+            for (int j = 0; j < V; ++j) f[j] = acc[j] * scale;
+            store_floats<T, V>(dw + (long)cur * D + c, f);
+        } else {
+            float* p = part + ((long)2 * chunk + which) * D + c;
 #pragma unroll
-        for (int j = 0; j < V; ++j) f[j] = acc[j] * scale;
-        store_floats<T, V>(dw + (long)cur * D + c, f);
+            for (int j = 0; j < V; ++j) p[j] = acc[j];
+        }
     };
     for (int i0 = s; i0 < e; i0 += ER) {
         Pack<T, V> row[ER];
         int k[ER];
 #pragma unroll
         for (int u = 0; u < ER; ++u) {
-            const int i = min(i0 + u, e - 1);
-            k[u] = key[i];
-            if (live) row[u] = load_pack<T, V>(dout + (long)pos[i] * ldo + c);
+            k[u] = i0 + u < e ? __builtin_amdgcn_readlane(my_key, i0 + u - s) : -1;
+            row[u] = load_pack<T, V>(col + (long)__builtin_amdgcn_readlane(my_pos, i0 + u - s) * ldo);
         }
 #pragma unroll
+        for (int u = 0; u < ER; ++u) hold(row[u]);  // all ER rows are under way before the first is added
+#pragma unroll
         for (int u = 0; u < ER; ++u) {
-            if (i0 + u >= e) break;
-            if (k[u] != cur) {
-                if (live) { if (head) to_part(0); else to_row(); }
+            if (k[u] != cur && k[u] >= 0) {
+                flush(head ? 0 : -1);
                 if (k[u] >= vocab) return;  // tokens outside the table sort last
                 cur = k[u];
                 head = false;
 #pragma unroll
                 for (int j = 0; j < V; ++j) acc[j] = 0.f;
             }
-            if (live)
 #pragma unroll
-                for (int j = 0; j < V; ++j) acc[j] += (float)row[u].e[j];
+            for (int j = 0; j < V; ++j) acc[j] += k[u] >= 0 ? (float)row[u].e[j] : 0.f;
         }
     }
-    if (!live) return;
-    if (head) to_part(0);
-    else if (e < n && key[e] == cur) to_part(1);
-    else to_row();
+    flush(head ? 0 : e < n && __builtin_amdgcn_readlane(my_key, 63) == cur ? 1 : -1);
 }
 
-// The run that begins in this chunk and goes on in the next: its partials, in chunk order per wave, waves in order.
+// The run that begins in this chunk and goes on in the next: its partials are summed per wave in chunk order, then the
+// waves' sums in wave order.  The eight waves are G groups of 256 columns times 8 / G shares of the partials.
 template <typename T>
 __global__ __launch_bounds__(512) void embed_join_kernel(const int* __restrict__ key, int n, int vocab, int D, float scale,
-                                                         T* __restrict__ dw, const float* __restrict__ part) {
-    constexpr int W = 8, U = 8;
-    __shared__ float sums[W][64];
+                                                         T* __restrict__ dw, const float* __restrict__ part, int G) {
+    constexpr int U = 8;
+    __shared__ float sums[8][256];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int chunk = blockIdx.x, s = chunk * EC, e = s + EC;
     if (e >= n) return;
     const int k = key[e - 1];
     if (k >= vocab || key[e] != k || (s > 0 && key[s - 1] == k)) return;
     const int last = (wave_lower_bound(key, n, k + 1) - 1) / EC;
-    const int c = blockIdx.y * 64 + lane;
-    float acc = 0.f;
-    if (c < D) {
-        if (wave == 0) acc = part[((long)2 * chunk + 1) * D + c];
-        for (int q = chunk + 1 + wave; q <= last; q += W * U) {
-            float v[U];
+    const int shares = 8 / G, share = wave / G;
+    for (int c0 = 0; c0 < D; c0 += G * 256) {
+        const int c = c0 + (wave % G) * 256 + lane;
+        float acc[4];
 #pragma unroll
-            for (int u = 0; u < U; ++u) v[u] = part[(long)2 * min(q + u * W, last) * D + c];
+        for (int j = 0; j < 4; ++j) acc[j] = share == 0 ? part[((long)2 * chunk + 1) * D + min(c + 64 * j, D - 1)] : 0.f;
+        for (int q = chunk + 1 + share; q <= last; q += shares * U) {
+            float v[U][4];
 #pragma unroll
-            for (int u = 0; u < U; ++u) acc += q + u * W <= last ? v[u] : 0.f;
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[u][j] = part[(long)2 * min(q + u * shares, last) * D + min(c + 64 * j, D - 1)];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[j] += q + u * shares <= last ? v[u][j] : 0.f;
         }
-    }
-    sums[wave][lane] = acc;
-    __syncthreads();
-    if (wave == 0 && c < D) {
-        float t = 0.f;
+        __syncthreads();
 #pragma unroll
-        for (int w = 0; w < W; ++w) t += sums[w][lane];
-        dw[(long)k * D + c] = (T)(t * scale);
+        for (int j = 0; j < 4; ++j) sums[wave][lane + 64 * j] = acc[j];
+        __syncthreads();
+        if (share == 0)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float t = acc[j];
+                for (int w = wave + G; w < 8; w += G) t += sums[w][lane + 64 * j];
+                if (c + 64 * j < D) dw[(long)k * D + c + 64 * j] = (T)(t * scale);
+            }
     }
 }
 
@@ -366,7 +382,7 @@ static EmbedWs embed_ws(int64_t n, int64_t vocab, int64_t D) {
     int64_t at = 0;
     for (int i = 0; i < 2; ++i) { w.key[i] = at; at += list; w.pos[i] = at; at += list; }
     w.hist = at;
-    at += n > SMALL_N ? (int64_t)w.passes * w.blocks * 1024 : 0;
+    at += n > SMALL_N ? (int64_t)w.blocks * 1024 : 0;
     w.part = at;
     at += (int64_t)w.chunks * 2 * D * 4;
     w.bytes = at;
@@ -426,14 +442,14 @@ extern "C" int dvae_embed_bwd(const void* dout, int64_t ld_dout, const void* ids
                            (int*)(b + L.key[0]), (int*)(b + L.pos[0]));
         DVAE_LAUNCH_CHECK();
     } else if (n > 0) {
-        hipLaunchKernelGGL(sort_count_kernel, dim3(L.blocks), dim3(TILE_THREADS), 0, s, ids, ids_i64, (int)n, (int)vocab,
-                           L.passes, L.per_block, (int*)(b + L.hist));
-        DVAE_LAUNCH_CHECK();
         for (int p = 0; p < L.passes; ++p) {
             at = p & 1;
-            hipLaunchKernelGGL(sort_pass_kernel, dim3(L.blocks), dim3(TILE_THREADS), 0, s, ids, ids_i64,
-                               (const int*)(b + L.key[1 - at]), (const int*)(b + L.pos[1 - at]), (int)n, (int)vocab, p, L.passes,
-                               L.per_block, (int*)(b + L.hist), (int*)(b + L.key[at]), (int*)(b + L.pos[at]));
+            const int *key_in = (const int*)(b + L.key[1 - at]), *pos_in = (const int*)(b + L.pos[1 - at]);
+            hipLaunchKernelGGL(sort_count_kernel, dim3(L.blocks), dim3(TILE_THREADS), 0, s, ids, ids_i64, key_in, (int)n, (int)vocab, p,
+                               L.per_block, (int*)(b + L.hist));
+            DVAE_LAUNCH_CHECK();
+            hipLaunchKernelGGL(sort_pass_kernel, dim3(L.blocks), dim3(TILE_THREADS), 0, s, ids, ids_i64, key_in, pos_in, (int)n,
+                               (int)vocab, p, L.per_block, (const int*)(b + L.hist), (int*)(b + L.key[at]), (int*)(b + L.pos[at]));
             DVAE_LAUNCH_CHECK();
         }
     }
@@ -453,9 +469,10 @@ extern "C" int dvae_embed_bwd(const void* dout, int64_t ld_dout, const void* ids
 #undef EMBED_SUM
     DVAE_LAUNCH_CHECK();
     if (L.chunks > 1) {
-        const dim3 grid(L.chunks, cdiv(D, 64));
-#define EMBED_JOIN(T) \
-    hipLaunchKernelGGL((embed_join_kernel<T>), grid, dim3(512), 0, s, key, (int)n, (int)vocab, D, scale, (T*)dw, (const float*)part)
+        const int groups = D <= 256 ? 1 : D <= 512 ? 2 : D <= 1024 ? 4 : 8;
+#define EMBED_JOIN(T)                                                                                                        \
+    hipLaunchKernelGGL((embed_join_kernel<T>), dim3(L.chunks), dim3(512), 0, s, key, (int)n, (int)vocab, D, scale, (T*)dw, \
+                       (const float*)part, groups)
         if (dtype == DVAE_F32) EMBED_JOIN(float);
         else if (dtype == DVAE_BF16) EMBED_JOIN(__bf16);
         else EMBED_JOIN(_Float16);

@@ -19,7 +19,7 @@
 
 namespace dvae {
 
-constexpr int TR = 64;  // rows of a tile: the state before every tile is kept for the backward pass
+constexpr int TR = 128;  // rows of a tile: the state before every tile is kept for the backward pass
 
 struct Rows {  // where the sequences lie
     const void* off;  // [S + 1] int32 / int64, or nullptr: S sequences of `len` rows each
@@ -75,13 +75,19 @@ __device__ __forceinline__ long seq_of(const Marks& m, int i) {
     return ((long)hi << 32) | (unsigned)lo;
 }
 
-// z = sigmoid(g) and 1 - z.  The smaller of the two (at most 1/2) is exp(-|g|) / (1 + exp(-|g|)), good to a few ulp; the
-// other is 1 minus it, good to half an ulp of 1 and unbiased, so that products of hundreds of z near 1 do not drift.
-__device__ __forceinline__ void gate_of(float g, float& z, float& omz) {
+// z = sigmoid(g) and 1 - z in one register: the smaller of the two (at most 1/2), negative where that is z.  It is
+// exp(-|g|) / (1 + exp(-|g|)), good to a few ulp; the other is 1 minus it, good to half an ulp of 1 and unbiased, so that
+// products of hundreds of z near 1 do not drift.
+__device__ __forceinline__ float gate_code(float g) {
     const float t = __expf(-fabsf(g));
-    const float less = t * __builtin_amdgcn_rcpf(1.f + t), more = 1.f - less;
-    z = g >= 0.f ? more : less;
-    omz = g >= 0.f ? less : more;
+    const float less = t * __builtin_amdgcn_rcpf(1.f + t);
+    return g >= 0.f ? less : -less;
+}
+__device__ __forceinline__ void gate_of_code(float code, float& z, float& omz) {
+    const float less = fabsf(code), more = 1.f - less;
+    const bool open = !(__float_as_uint(code) >> 31);
+    z = open ? more : less;
+    omz = open ? less : more;
 }
 
 // A run of rows as a map of the state (or of the gradient that flows back) before it: s -> A s + B.  A = 0 says that a
@@ -94,39 +100,48 @@ constexpr float A_MIN = 1.17549435e-38f;
 // LOOK published maps to the nearest whose A is 0 and applies the ones in between in order, oldest first: the sums are
 // those of walking the tiles one by one, whatever the timing, so results do not vary.  64-bit relaxed atomics at device
 // scope; a word that still holds the fill pattern has not been published, so no fences are needed.
-constexpr int LOOK = 16;
+constexpr int LOOK = 8;
 constexpr unsigned long long UNSET = ~0ull;
+constexpr int SPINS = 1 << 22;  // never reached: every tile waits for earlier tickets only; then NaN rather than a hang
 __device__ __forceinline__ void publish(unsigned long long* at, float A, float B) {
     const unsigned long long w = ((unsigned long long)__float_as_uint(A) << 32) | __float_as_uint(B);
     __hip_atomic_store(at, w == UNSET ? w ^ 1 : w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-// `ahead`: the words of the tiles before this one in walking order, nearest first, `step` apart; `count` of them exist.
+__device__ __forceinline__ unsigned long long read_word(const unsigned long long* at) {
+    return __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+// The state that flows into a tile.  `nearest`: the word of the tile before it in walking order, the others `step` apart,
+// `count` of them.  All words in reach are read at once; where none is whole yet, the farthest one is the next to become
+// so, and only that one is polled.
 __device__ __forceinline__ float look_back(const unsigned long long* nearest, long step, long count) {
     const int n = (int)min(count, (long)LOOK);
-    for (int spin = 0; spin < (1 << 20); ++spin) {
-        unsigned long long w[LOOK];
+    unsigned long long w[LOOK];
+    int spins = 0;
+    bool open;
+    do {
+        open = true;
 #pragma unroll
-        for (int i = 0; i < LOOK; ++i)
-            w[i] = i < n ? __hip_atomic_load(nearest + i * step, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
-        int from = -1;  // the nearest whole state, if everything nearer is published
-        bool open = true;
+        for (int i = 0; i < LOOK; ++i) w[i] = i < n ? read_word(nearest + i * step) : 0;  // 0: before the first tile the state is 0
 #pragma unroll
         for (int i = 0; i < LOOK; ++i) {
-            if (w[i] == UNSET) open = false;
-            // (past the first tile of all the state is zero)
-            if (open && from < 0 && (i >= n ? count <= LOOK : (w[i] >> 32) == 0)) from = i;
+            open = open && w[i] != UNSET;
+            if ((w[i] >> 32) == 0) break;  // whole: nothing farther matters
         }
-        if (open && from < 0 && count <= LOOK && n == LOOK) from = LOOK;
-        if (__all(from >= 0)) {
-            float s = 0.f;
+    } while (!__all(open) && ++spins < SPINS);
+    bool whole = count < LOOK;
 #pragma unroll
-            for (int i = LOOK - 1; i >= 0; --i)
-                if (i <= from && i < n) s = through(__uint_as_float((unsigned)(w[i] >> 32)), __uint_as_float((unsigned)w[i]), s);
-            return s;
-        }
+    for (int i = 0; i < LOOK; ++i) whole = whole || (w[i] >> 32) == 0;
+    if (count == LOOK) whole = true;
+    while (!__all(whole) && ++spins < SPINS) {
         __builtin_amdgcn_s_sleep(1);
+        const unsigned long long far = read_word(nearest + (LOOK - 1) * step);
+        if (!whole && (far >> 32) == 0) { w[LOOK - 1] = far; whole = true; }
     }
-    return __uint_as_float(0x7FC00000u);  // not reached: every tile waits for earlier tickets only; NaN rather than a hang
+    float s = spins < SPINS ? 0.f : __uint_as_float(0x7FC00000u);
+#pragma unroll
+    for (int i = LOOK - 1; i >= 0; --i)
+        if (i < n) s = through(__uint_as_float((unsigned)(w[i] >> 32)), __uint_as_float((unsigned)w[i]), s);
+    return s;
 }
 
 struct ScanParams {
@@ -155,6 +170,45 @@ __device__ __forceinline__ unsigned take_ticket(unsigned* ticket) {
     return mine;
 }
 
+// A wave's rows of one matrix: a buffer based at its first row, the lane's columns as the one vector offset, the row as a
+// scalar offset, so that no lane computes an address.  Rows beyond the last and columns beyond D are read from the nearest
+// inside and not used: loads without branches.
+template <typename T, int V> struct RowBuffer {
+    __amdgpu_buffer_rsrc_t rsrc;
+    unsigned col, pitch;  // bytes
+    int most;             // rows behind the first that may be touched
+    __device__ __forceinline__ RowBuffer(const void* base, long ld, long t0, long N, int c) {
+        const long first = min(t0, N - 1);
+        rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)((const T*)base + first * ld), 0, 0x7FFFFFFF, 0x00020000);
+        col = (unsigned)c * sizeof(T);
+        pitch = (unsigned)(ld * sizeof(T));
+        most = (int)min(N - 1 - first, 63L);
+    }
+    __device__ __forceinline__ Pack<T, V> load(int i) const {
+        const unsigned at = min(i, most) * pitch;
+        if constexpr (sizeof(T) * V == 4) return __builtin_bit_cast(Pack<T, V>, __builtin_amdgcn_raw_buffer_load_b32(rsrc, col, at, 0));
+        else return __builtin_bit_cast(Pack<T, V>, __builtin_amdgcn_raw_buffer_load_b16(rsrc, col, at, 0));
+    }
+    __device__ __forceinline__ void store(int i, const float (&f)[V]) const {
+        Pack<T, V> o;
+#pragma unroll
+        for (int j = 0; j < V; ++j) o.e[j] = (T)f[j];
+        if constexpr (sizeof(T) * V == 4) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, o), rsrc, col, i * pitch, 0);
+        else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, o), rsrc, col, i * pitch, 0);
+    }
+};
+template <typename T, int V, int RW>
+__device__ __forceinline__ void load_rows(Pack<T, V> (&r)[RW], const void* base, long ld, long t0, long N, int D, int c) {
+    const RowBuffer<T, V> b(base, ld, t0, N, min(c, D - V));
+#pragma unroll
+    for (int i = 0; i < RW; ++i) r[i] = b.load(i);
+}
+
+struct Yes { static constexpr bool value = true; };
+struct No { static constexpr bool value = false; };
+
+// Where a wave's rows all lie inside one sequence (PLAIN below) the row loops have no branches, so that the loads, the
+// exponentials and the chains of multiply-adds of several channels overlap.
 template <typename T, int V, int RW, int W>
 __global__ __launch_bounds__(W * 64) void scan_fwd_kernel(ScanParams p) {
     static_assert(RW * W == TR && W >= V, "");
@@ -165,35 +219,39 @@ __global__ __launch_bounds__(W * 64) void scan_fwd_kernel(ScanParams p) {
     const long tile = unit / (unsigned)p.slabs, t0 = tile * TR + wave * RW;
     const bool live = c < p.D;
     Pack<T, V> g[RW], x[RW];
-#pragma unroll
-    for (int i = 0; i < RW; ++i)
-        if (live && t0 + i < p.q.N) {
-            g[i] = load_pack<T, V>((const T*)p.gate + (t0 + i) * p.ld_gate + c);
-            x[i] = load_pack<T, V>((const T*)p.x + (t0 + i) * p.ld_x + c);
-        }
+    load_rows<T, V, RW>(g, p.gate, p.ld_gate, t0, p.q.N, p.D, c);
+    load_rows<T, V, RW>(x, p.x, p.ld_x, t0, p.q.N, p.D, c);
     const Marks m = mark_rows<RW>(p.q, t0);
-    float A[V], h[V], z[RW][V], b[RW][V];
+    const bool plain = m.start == 0 && m.end == 0 && m.cover == (unsigned)((1ull << RW) - 1);
+    float A[V], h[V], code[RW][V];
 #pragma unroll
     for (int j = 0; j < V; ++j) { A[j] = 1.f; h[j] = 0.f; }
 #pragma unroll
-    for (int i = 0; i < RW; ++i) {
-        if ((m.start >> i) & 1) {
-            load_init<V>(h, p.h0, seq_of(m, i), p.D, c, live);
+    for (int i = 0; i < RW; ++i)
 #pragma unroll
-            for (int j = 0; j < V; ++j) A[j] = 0.f;
-        }
-        if ((m.cover >> i) & 1)
+        for (int j = 0; j < V; ++j) code[i][j] = gate_code((float)g[i].e[j]);
+    auto local = [&](auto mixed) {
+#pragma unroll
+        for (int i = 0; i < RW; ++i) {
+            if (decltype(mixed)::value) {
+                if ((m.start >> i) & 1) load_init<V>(h, p.h0, seq_of(m, i), p.D, c, live);
+                if (!((m.cover >> i) & 1)) continue;
+            }
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                float omz;
-                gate_of((float)g[i].e[j], z[i][j], omz);
-                b[i][j] = omz * (float)x[i].e[j];
-                h[j] = fmaf(z[i][j], h[j], b[i][j]);
-                A[j] = A[j] == 0.f ? 0.f : fmaxf(A[j] * z[i][j], A_MIN);
+                float z, omz;
+                gate_of_code(code[i][j], z, omz);
+                h[j] = fmaf(z, h[j], omz * (float)x[i].e[j]);
+                A[j] *= z;
             }
-    }
+        }
+    };
+    if (plain) local(No()); else local(Yes());
 #pragma unroll
-    for (int j = 0; j < V; ++j) { As[wave][lane * V + j] = A[j]; Bs[wave][lane * V + j] = h[j]; }
+    for (int j = 0; j < V; ++j) {
+        As[wave][lane * V + j] = m.start ? 0.f : fmaxf(A[j], A_MIN);
+        Bs[wave][lane * V + j] = h[j];
+    }
     __syncthreads();
     if (wave < V && c0 + (int)threadIdx.x < p.D) {  // one thread per channel from here to the barrier
         const int k = threadIdx.x;
@@ -213,29 +271,44 @@ __global__ __launch_bounds__(W * 64) void scan_fwd_kernel(ScanParams p) {
     __syncthreads();
     if (!live) return;
 #pragma unroll
+    for (int i = 0; i < RW; ++i) {
+        hold(x[i]);
+#pragma unroll
+        for (int j = 0; j < V; ++j) hold(code[i][j]);
+    }
+#pragma unroll
     for (int j = 0; j < V; ++j) {
         float s = Cs[lane * V + j];
         for (int w = 0; w < wave; ++w) s = through(As[w][lane * V + j], Bs[w][lane * V + j], s);
         h[j] = s;
     }
+    const RowBuffer<T, V> out(p.h, p.D, t0, p.q.N, c);
+    auto apply = [&](auto mixed) {
 #pragma unroll
-    for (int i = 0; i < RW; ++i) {
-        if (t0 + i >= p.q.N) break;
-        if ((m.start >> i) & 1) load_init<V>(h, p.h0, seq_of(m, i), p.D, c, live);
-        const bool cover = (m.cover >> i) & 1;
-        float o[V];
+        for (int i = 0; i < RW; ++i) {
+            bool cover = true;
+            if (decltype(mixed)::value) {
+                if (t0 + i >= p.q.N) continue;
+                if ((m.start >> i) & 1) load_init<V>(h, p.h0, seq_of(m, i), p.D, c, live);
+                cover = (m.cover >> i) & 1;
+            }
+            float o[V];
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            if (cover) h[j] = fmaf(z[i][j], h[j], b[i][j]);
-            o[j] = cover ? h[j] : 0.f;
+            for (int j = 0; j < V; ++j) {
+                float z, omz;
+                gate_of_code(code[i][j], z, omz);
+                if (cover) h[j] = fmaf(z, h[j], omz * (float)x[i].e[j]);
+                o[j] = cover ? h[j] : 0.f;
+            }
+            out.store(i, o);
+            if (decltype(mixed)::value && ((m.end >> i) & 1)) {
+                const long s = seq_of(m, i);
+#pragma unroll
+                for (int j = 0; j < V; ++j) p.last[s * p.D + c + j] = h[j];
+            }
         }
-        store_floats<T, V>((T*)p.h + (t0 + i) * p.D + c, o);
-        if ((m.end >> i) & 1) {
-            const long s = seq_of(m, i);
-#pragma unroll
-            for (int j = 0; j < V; ++j) p.last[s * p.D + c + j] = h[j];
-        }
-    }
+    };
+    if (plain) apply(No()); else apply(Yes());
 }
 
 // Backward: the tiles are walked from the last; what flows from a tile to the one before it is z_t G_t of its first row.
@@ -249,51 +322,65 @@ __global__ __launch_bounds__(W * 64) void scan_bwd_kernel(ScanParams p) {
     const long tiles = (p.q.N + TR - 1) / TR, tile = tiles - 1 - unit / (unsigned)p.slabs, t0 = tile * TR + wave * RW;
     const bool live = c < p.D;
     Pack<T, V> g[RW], x[RW], d[RW];
+    load_rows<T, V, RW>(g, p.gate, p.ld_gate, t0, p.q.N, p.D, c);
+    load_rows<T, V, RW>(x, p.x, p.ld_x, t0, p.q.N, p.D, c);
+    if (p.dh) load_rows<T, V, RW>(d, p.dh, p.ld_dh, t0, p.q.N, p.D, c);
+    else
 #pragma unroll
-    for (int i = 0; i < RW; ++i)
-        if (live && t0 + i < p.q.N) {
-            g[i] = load_pack<T, V>((const T*)p.gate + (t0 + i) * p.ld_gate + c);
-            if (p.dh) d[i] = load_pack<T, V>((const T*)p.dh + (t0 + i) * p.ld_dh + c);
-            x[i] = load_pack<T, V>((const T*)p.x + (t0 + i) * p.ld_x + c);
-        }
+        for (int i = 0; i < RW; ++i)
+#pragma unroll
+            for (int j = 0; j < V; ++j) d[i].e[j] = (T)0.f;
     const Marks m = mark_rows<RW>(p.q, t0);
-    auto row_grad = [&](int i, float (&e)[V]) {  // dh of row i, and dlast where the sequence ends
+    const bool plain = m.start == 0 && m.end == 0 && m.cover == (unsigned)((1ull << RW) - 1);
+    auto row_grad = [&](auto mixed, int i, float (&e)[V]) {  // dh of row i, and dlast where the sequence ends
 #pragma unroll
-        for (int j = 0; j < V; ++j) e[j] = p.dh ? (float)d[i].e[j] : 0.f;
-        if (((m.end >> i) & 1) && p.dlast) {
+        for (int j = 0; j < V; ++j) e[j] = (float)d[i].e[j];
+        if (decltype(mixed)::value && ((m.end >> i) & 1) && p.dlast) {
             const long s = seq_of(m, i);
 #pragma unroll
             for (int j = 0; j < V; ++j) e[j] += live ? p.dlast[s * p.D + c + j] : 0.f;
         }
     };
-    float A[V], B[V], h[V], z[RW][V], omz[RW][V];
+    float A[V], B[V], h[V], code[RW][V];
 #pragma unroll
     for (int j = 0; j < V; ++j) { A[j] = 1.f; B[j] = 0.f; h[j] = 0.f; }
 #pragma unroll
-    for (int i = 0; i < RW; ++i) {  // this wave's part of the forward scan
-        if ((m.start >> i) & 1) load_init<V>(h, p.h0, seq_of(m, i), p.D, c, live);
-        if ((m.cover >> i) & 1)
+    for (int i = 0; i < RW; ++i)
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                gate_of((float)g[i].e[j], z[i][j], omz[i][j]);
-                h[j] = fmaf(z[i][j], h[j], omz[i][j] * (float)x[i].e[j]);
+        for (int j = 0; j < V; ++j) code[i][j] = gate_code((float)g[i].e[j]);
+    auto local = [&](auto mixed) {
+#pragma unroll
+        for (int i = 0; i < RW; ++i) {  // this wave's part of the forward scan
+            if (decltype(mixed)::value) {
+                if ((m.start >> i) & 1) load_init<V>(h, p.h0, seq_of(m, i), p.D, c, live);
+                if (!((m.cover >> i) & 1)) continue;
             }
-    }
-#pragma unroll
-    for (int i = RW - 1; i >= 0; --i)
-        if ((m.cover >> i) & 1) {
-            float e[V];
-            row_grad(i, e);
-            const bool first = (m.start >> i) & 1;
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                B[j] = first ? 0.f : z[i][j] * (e[j] + B[j]);
-                A[j] = first || A[j] == 0.f ? 0.f : fmaxf(A[j] * z[i][j], A_MIN);
+                float z, omz;
+                gate_of_code(code[i][j], z, omz);
+                h[j] = fmaf(z, h[j], omz * (float)x[i].e[j]);
             }
         }
 #pragma unroll
+        for (int i = RW - 1; i >= 0; --i) {
+            if (decltype(mixed)::value && !((m.cover >> i) & 1)) continue;
+            float e[V];
+            row_grad(mixed, i, e);
+            const bool first = decltype(mixed)::value && ((m.start >> i) & 1);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                float z, omz;
+                gate_of_code(code[i][j], z, omz);
+                B[j] = first ? 0.f : z * (e[j] + B[j]);
+                A[j] *= z;
+            }
+        }
+    };
+    if (plain) local(No()); else local(Yes());
+#pragma unroll
     for (int j = 0; j < V; ++j) {
-        As[wave][lane * V + j] = A[j];
+        As[wave][lane * V + j] = m.start ? 0.f : fmaxf(A[j], A_MIN);
         Bs[wave][lane * V + j] = B[j];
         Fs[wave][lane * V + j] = h[j];
     }
@@ -314,6 +401,13 @@ __global__ __launch_bounds__(W * 64) void scan_bwd_kernel(ScanParams p) {
     }
     __syncthreads();
     if (!live || t0 >= p.q.N) return;
+#pragma unroll
+    for (int i = 0; i < RW; ++i) {
+        hold(x[i]);
+        hold(d[i]);
+#pragma unroll
+        for (int j = 0; j < V; ++j) hold(code[i][j]);
+    }
     float C[V], prev[RW][V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
@@ -324,40 +418,48 @@ __global__ __launch_bounds__(W * 64) void scan_bwd_kernel(ScanParams p) {
         for (int w = W - 1; w > wave; --w) s = through(As[w][lane * V + j], Bs[w][lane * V + j], s);
         C[j] = s;
     }
+    const RowBuffer<T, V> out_gate(p.dgate, p.D, t0, p.q.N, c), out_x(p.dx, p.D, t0, p.q.N, c);
+    auto apply = [&](auto mixed) {
 #pragma unroll
-    for (int i = 0; i < RW; ++i) {
-        if ((m.start >> i) & 1) load_init<V>(h, p.h0, seq_of(m, i), p.D, c, live);
+        for (int i = 0; i < RW; ++i) {
+            if (decltype(mixed)::value && ((m.start >> i) & 1)) load_init<V>(h, p.h0, seq_of(m, i), p.D, c, live);
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            prev[i][j] = h[j];
-            if ((m.cover >> i) & 1) h[j] = fmaf(z[i][j], h[j], omz[i][j] * (float)x[i].e[j]);
-        }
-    }
-#pragma unroll
-    for (int i = RW - 1; i >= 0; --i) {
-        if (t0 + i >= p.q.N) continue;
-        const bool cover = (m.cover >> i) & 1;
-        float e[V], og[V], ox[V];
-        row_grad(i, e);
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const float G = e[j] + C[j];
-            og[j] = cover ? G * (prev[i][j] - (float)x[i].e[j]) * z[i][j] * omz[i][j] : 0.f;
-            ox[j] = cover ? G * omz[i][j] : 0.f;
-            if (cover) C[j] = z[i][j] * G;
-        }
-        store_floats<T, V>((T*)p.dgate + (t0 + i) * p.D + c, og);
-        store_floats<T, V>((T*)p.dx + (t0 + i) * p.D + c, ox);
-        if ((m.start >> i) & 1) {
-            if (p.dh0) {
-                const long s = seq_of(m, i);
-#pragma unroll
-                for (int j = 0; j < V; ++j) p.dh0[s * p.D + c + j] = C[j];
+            for (int j = 0; j < V; ++j) {
+                prev[i][j] = h[j];
+                float z, omz;
+                gate_of_code(code[i][j], z, omz);
+                if (!decltype(mixed)::value || ((m.cover >> i) & 1)) h[j] = fmaf(z, h[j], omz * (float)x[i].e[j]);
             }
-#pragma unroll
-            for (int j = 0; j < V; ++j) C[j] = 0.f;
         }
-    }
+#pragma unroll
+        for (int i = RW - 1; i >= 0; --i) {
+            if (decltype(mixed)::value && t0 + i >= p.q.N) continue;
+            const bool cover = !decltype(mixed)::value || ((m.cover >> i) & 1);
+            float e[V], og[V], ox[V];
+            row_grad(mixed, i, e);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                float z, omz;
+                gate_of_code(code[i][j], z, omz);
+                const float G = e[j] + C[j];
+                og[j] = cover ? G * (prev[i][j] - (float)x[i].e[j]) * z * omz : 0.f;
+                ox[j] = cover ? G * omz : 0.f;
+                if (cover) C[j] = z * G;
+            }
+            out_gate.store(i, og);
+            out_x.store(i, ox);
+            if (decltype(mixed)::value && ((m.start >> i) & 1)) {
+                if (p.dh0) {
+                    const long s = seq_of(m, i);
+#pragma unroll
+                    for (int j = 0; j < V; ++j) p.dh0[s * p.D + c + j] = C[j];
+                }
+#pragma unroll
+                for (int j = 0; j < V; ++j) C[j] = 0.f;
+            }
+        }
+    };
+    if (plain) apply(No()); else apply(Yes());
 }
 
 // Before either pass: nothing is published yet, ticket 0 is next; and the sequences without rows, whose last state is the
@@ -394,10 +496,19 @@ __global__ __launch_bounds__(256) void scan_step_kernel(const T* __restrict__ ga
         if (live) store_floats<T, V>(h + (long)b * D + c, zero);
         return;
     }
-    if (slots) {
-        for (int r0 = 0; r0 < b; r0 += 64)
-            if (__ballot(r0 + lane < b && slot(min(r0 + lane, b)) == k)) return;  // an earlier row advances this slot
-    }
+    bool again = false;  // a later row names the same slot
+    if (slots)
+        for (int r0 = 0; r0 < B; r0 += 64 * 8) {
+            bool same[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) same[u] = slot(min(r0 + 64 * u + lane, B - 1)) == k;
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const int r = r0 + 64 * u + lane;
+                if (__ballot(same[u] && r < b)) return;  // an earlier row advances this slot
+                again = again || __ballot(same[u] && r > b && r < B);
+            }
+        }
     float s[V];
     if (live)
 #pragma unroll
@@ -408,13 +519,13 @@ __global__ __launch_bounds__(256) void scan_step_kernel(const T* __restrict__ ga
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             float z, omz;
-            gate_of((float)g.e[j], z, omz);
+            gate_of_code(gate_code((float)g.e[j]), z, omz);
             s[j] = fmaf(z, s[j], omz * (float)y.e[j]);
         }
         store_floats<T, V>(h + (long)r * D + c, s);
     };
     advance(b);
-    if (slots)
+    if (again)
         for (int r0 = b + 1; r0 < B; r0 += 64) {
             unsigned long long more = __ballot(r0 + lane < B && slot(min(r0 + lane, B - 1)) == k);
             while (more) {
@@ -427,11 +538,13 @@ __global__ __launch_bounds__(256) void scan_step_kernel(const T* __restrict__ ga
         for (int j = 0; j < V; ++j) state[k * ld_state + c + j] = s[j];
 }
 
-static int scan_check(const char* who, int64_t rows, int64_t seqs, const void* off, int32_t D, int32_t dtype) {
+static int scan_check(const char* who, int64_t rows, int64_t seqs, const void* off, int64_t ld_most, int32_t D, int32_t dtype) {
     DVAE_REQUIRE(known_dtype(dtype), "%s: unknown element type %d", who, dtype);
     DVAE_REQUIRE(rows >= 0 && rows < (1LL << 40), "%s: %lld rows are not supported", who, (long long)rows);
     DVAE_REQUIRE(seqs >= 0 && seqs < (1LL << 31), "%s: %lld sequences are not supported", who, (long long)seqs);
     DVAE_REQUIRE(D >= 1 && D <= (1 << 20), "%s: %d channels are not in 1 .. 2^20", who, D);
+    // (a wave addresses its 32 rows with 32-bit byte offsets)
+    DVAE_REQUIRE(ld_most <= (1 << 23), "%s: a row stride of %lld elements is not supported", who, (long long)ld_most);
     DVAE_REQUIRE(off || (seqs > 0 ? rows % seqs == 0 : rows == 0), "%s: %lld rows are not %lld sequences of one length", who,
                  (long long)rows, (long long)seqs);
     return DVAE_OK;
@@ -449,18 +562,16 @@ static ScanWs scan_ws(int64_t rows, int64_t D) {
     return w;
 }
 
-// CALL(T, V, RW, W): V channels per lane, RW rows per wave (V * RW = 32 elements of every operand in registers), W waves
-#define SCAN_BY_TYPE(dtype, vec, CALL)                                                          \
-    do {                                                                                        \
-        if ((dtype) == DVAE_F32) {                                                              \
-            if ((vec) >= 2) { CALL(float, 2, 16, 4); } else { CALL(float, 1, 32, 2); }          \
-        } else if ((dtype) == DVAE_BF16) {                                                      \
-            if ((vec) >= 4) { CALL(__bf16, 4, 8, 8); }                                          \
-            else if ((vec) == 2) { CALL(__bf16, 2, 16, 4); } else { CALL(__bf16, 1, 32, 2); }   \
-        } else {                                                                                \
-            if ((vec) >= 4) { CALL(_Float16, 4, 8, 8); }                                        \
-            else if ((vec) == 2) { CALL(_Float16, 2, 16, 4); } else { CALL(_Float16, 1, 32, 2); } \
-        }                                                                                       \
+// CALL(T, V, RW, W): V channels per lane, RW rows per wave, W waves.  Two channels a lane for 16-bit types, so that a wave
+// reads 256 bytes of a row as with one fp32 channel; odd row lengths and strides fall back to one.
+#define SCAN_BY_TYPE(dtype, vec, CALL)                                                       \
+    do {                                                                                     \
+        if ((dtype) == DVAE_F32) { CALL(float, 1, 16, 8); }                                  \
+        else if ((dtype) == DVAE_BF16) {                                                     \
+            if ((vec) == 2) { CALL(__bf16, 2, 16, 8); } else { CALL(__bf16, 1, 16, 8); }     \
+        } else {                                                                             \
+            if ((vec) == 2) { CALL(_Float16, 2, 16, 8); } else { CALL(_Float16, 1, 16, 8); } \
+        }                                                                                    \
     } while (0)
 
 static int scan_begin(ScanParams& p, void* ws, const ScanWs& L, const float* from, float* to, hipStream_t s) {
@@ -481,12 +592,12 @@ static int scan_begin(ScanParams& p, void* ws, const ScanWs& L, const float* fro
 
 extern "C" int64_t dvae_scan_state_floats(int64_t rows, int32_t D) {
     using namespace dvae;
-    DVAE_TRY(scan_check("scan_state_floats", rows, 1, nullptr, D, DVAE_F32));
+    DVAE_TRY(scan_check("scan_state_floats", rows, 1, nullptr, 0, D, DVAE_F32));
     return scan_ws(rows, D).tiles * D;
 }
 extern "C" int64_t dvae_scan_ws_bytes(int64_t rows, int32_t D) {
     using namespace dvae;
-    DVAE_TRY(scan_check("scan_ws_bytes", rows, 1, nullptr, D, DVAE_F32));
+    DVAE_TRY(scan_check("scan_ws_bytes", rows, 1, nullptr, 0, D, DVAE_F32));
     return scan_ws(rows, D).bytes;
 }
 
@@ -494,14 +605,14 @@ extern "C" int dvae_scan_fwd(const void* gate, int64_t ld_gate, const void* x, i
                              const float* h0, void* h, float* last, float* states, void* ws, int64_t rows, int64_t seqs,
                              int32_t D, int32_t dtype, void* stream) {
     using namespace dvae;
-    DVAE_TRY(scan_check("scan_fwd", rows, seqs, off, D, dtype));
+    DVAE_TRY(scan_check("scan_fwd", rows, seqs, off, ld_gate > ld_x ? ld_gate : ld_x, D, dtype));
     DVAE_REQUIRE((ld_gate == 0 || ld_gate >= D) && (ld_x == 0 || ld_x >= D), "scan_fwd: a row stride is below %d channels", D);
     DVAE_REQUIRE(rows == 0 || (gate && x && h && ws), "scan_fwd: null pointer");
     DVAE_REQUIRE(seqs == 0 || last, "scan_fwd: null pointer");
     DVAE_REQUIRE((uintptr_t)ws % 16 == 0, "scan_fwd: the workspace must be 16-byte aligned");
     hipStream_t s = (hipStream_t)stream;
     const ScanWs L = scan_ws(rows, D);
-    const int vec = widest(elem_size(dtype), 8, {(int64_t)D, ld_gate, ld_x}, {gate, x, (const void*)h});
+    const int vec = widest(elem_size(dtype), 4, {(int64_t)D, ld_gate, ld_x}, {gate, x, (const void*)h});
     ScanParams p = {};
     p.gate = gate; p.x = x; p.ld_gate = ld_gate; p.ld_x = ld_x; p.h = h; p.h0 = h0; p.last = last; p.states = states;
     p.q = {off, off_i64, seqs, seqs > 0 ? rows / seqs : 0, rows};
@@ -521,14 +632,15 @@ extern "C" int dvae_scan_bwd(const void* gate, int64_t ld_gate, const void* x, i
                              const float* h0, const float* states, const void* dh, int64_t ld_dh, const float* dlast, void* dgate,
                              void* dx, float* dh0, void* ws, int64_t rows, int64_t seqs, int32_t D, int32_t dtype, void* stream) {
     using namespace dvae;
-    DVAE_TRY(scan_check("scan_bwd", rows, seqs, off, D, dtype));
+    const int64_t ld_in = ld_gate > ld_x ? ld_gate : ld_x;
+    DVAE_TRY(scan_check("scan_bwd", rows, seqs, off, ld_in > ld_dh ? ld_in : ld_dh, D, dtype));
     DVAE_REQUIRE((ld_gate == 0 || ld_gate >= D) && (ld_x == 0 || ld_x >= D) && (ld_dh == 0 || ld_dh >= D),
                  "scan_bwd: a row stride is below %d channels", D);
     DVAE_REQUIRE(rows == 0 || (gate && x && states && dgate && dx && ws), "scan_bwd: null pointer");
     DVAE_REQUIRE((uintptr_t)ws % 16 == 0, "scan_bwd: the workspace must be 16-byte aligned");
     hipStream_t s = (hipStream_t)stream;
     const ScanWs L = scan_ws(rows, D);
-    const int vec = widest(elem_size(dtype), 8, {(int64_t)D, ld_gate, ld_x, dh ? ld_dh : 0},
+    const int vec = widest(elem_size(dtype), 4, {(int64_t)D, ld_gate, ld_x, dh ? ld_dh : 0},
                            {gate, x, dh, (const void*)dgate, (const void*)dx});
     ScanParams p = {};
     p.gate = gate; p.x = x; p.dh = dh; p.ld_gate = ld_gate; p.ld_x = ld_x; p.ld_dh = ld_dh;
@@ -557,15 +669,15 @@ extern "C" int dvae_scan_step(const void* gate, int64_t ld_gate, const void* x, 
     DVAE_REQUIRE(slots || rows <= pool, "scan_step: %d rows, but a pool of %lld states", rows, (long long)pool);
     if (rows == 0) return DVAE_OK;
     DVAE_REQUIRE(gate && x && h && (state || pool == 0), "scan_step: null pointer");
-    const int vec = widest(elem_size(dtype), 8, {(int64_t)D, ld_gate, ld_x}, {gate, x, (const void*)h});
+    const int vec = widest(elem_size(dtype), 16, {(int64_t)D, ld_gate, ld_x}, {gate, x, (const void*)h});
     const int slabs = cdiv(D, 64 * vec);
     const long units = (long)rows * slabs;
     DVAE_REQUIRE(units < (1LL << 31), "scan_step: %d rows of %d channels are too many", rows, D);
     const dim3 grid((unsigned)((units + 3) / 4));
-#define SCAN_STEP(T, V, RW, W)                                                                                              \
+#define SCAN_STEP(T, V)                                                                                              \
     hipLaunchKernelGGL((scan_step_kernel<T, V>), grid, dim3(256), 0, (hipStream_t)stream, (const T*)gate, (long)ld_gate, (const T*)x, \
                        (long)ld_x, state, (long)ld_state, (long)pool, slots, slots_i64, (T*)h, rows, D, slabs)
-    SCAN_BY_TYPE(dtype, vec, SCAN_STEP);
+    DVAE_BY_TYPE(dtype, vec, SCAN_STEP);
 #undef SCAN_STEP
     DVAE_LAUNCH_CHECK();
     return DVAE_OK;

@@ -22,6 +22,24 @@ template <typename T, int V> __device__ __forceinline__ void store_floats(T* p, 
     store_pack<T, V>(p, o);
 }
 
+// The value is in registers here, and nothing computed from it before is reused behind: keeps a load from being sunk behind
+// a branch, and what can be recomputed cheaply from being kept in registers across a long section.
+template <typename T, int V> __device__ __forceinline__ void hold(Pack<T, V>& v) {
+    if constexpr (sizeof(v) >= 4) {
+        unsigned w[sizeof(v) / 4];
+        __builtin_memcpy(w, &v, sizeof(v));
+#pragma unroll
+        for (unsigned i = 0; i < sizeof(v) / 4; ++i) asm volatile("" : "+v"(w[i]));
+        __builtin_memcpy(&v, w, sizeof(v));
+    } else {
+        unsigned short w;
+        __builtin_memcpy(&w, &v, 2);
+        asm volatile("" : "+v"(w));
+        __builtin_memcpy(&v, &w, 2);
+    }
+}
+__device__ __forceinline__ void hold(float& v) { asm volatile("" : "+v"(v)); }
+
 static inline int elem_size(int dtype) { return dtype == DVAE_F32 ? 4 : 2; }
 static inline bool known_dtype(int dtype) { return dtype == DVAE_F32 || dtype == DVAE_BF16 || dtype == DVAE_F16; }
 
