@@ -249,9 +249,19 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const T* __restrict__ do
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if ((int)blockIdx.x >= sum_blocks) {
         __shared__ unsigned long long named;
+        __shared__ int edge[2];
         const int r0 = ((int)blockIdx.x - sum_blocks) * ZERO_ROWS, rows = min(ZERO_ROWS, vocab - r0);
-        if (wave == 0) {  // lane r looks for row r0 + r among the tokens of the range
-            int lo = wave_lower_bound(key, n, r0), hi = wave_lower_bound(key, n, r0 + rows);
+        if (threadIdx.x == 0) named = 0;
+        if (wave < 2) {
+            const int at = wave_lower_bound(key, n, wave == 0 ? r0 : r0 + rows);
+            if (lane == 0) edge[wave] = at;
+        }
+        __syncthreads();
+        int lo = edge[0], hi = edge[1];
+        if (hi - lo <= 1024) {  // few tokens: all of them at once
+            for (int i = lo + (int)threadIdx.x; i < hi; i += 256)
+                if (i == lo || key[i] != key[i - 1]) atomicOr(&named, 1ull << (key[i] - r0));
+        } else if (wave == 0) {  // a hot row among them: lane r looks for row r0 + r
             const int end = hi;
             while (lo < hi) {
                 const int mid = lo + (hi - lo) / 2;

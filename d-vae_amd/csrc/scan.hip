@@ -496,6 +496,12 @@ __global__ __launch_bounds__(256) void scan_step_kernel(const T* __restrict__ ga
         if (live) store_floats<T, V>(h + (long)b * D + c, zero);
         return;
     }
+    // the row and the state are under way while the slots are searched; a row that is not the first of its slot drops them
+    const int cc = live ? c : D - V;
+    Pack<T, V> g = load_pack<T, V>(gate + (long)b * ld_gate + cc), y = load_pack<T, V>(x + (long)b * ld_x + cc);
+    float s[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) s[j] = state[k * ld_state + cc + j];
     bool again = false;  // a later row names the same slot
     if (slots)
         for (int r0 = 0; r0 < B; r0 += 64 * 8) {
@@ -509,27 +515,24 @@ __global__ __launch_bounds__(256) void scan_step_kernel(const T* __restrict__ ga
                 again = again || __ballot(same[u] && r > b && r < B);
             }
         }
-    float s[V];
-    if (live)
-#pragma unroll
-        for (int j = 0; j < V; ++j) s[j] = state[k * ld_state + c + j];
     auto advance = [&](int r) {
-        if (!live) return;
-        const Pack<T, V> g = load_pack<T, V>(gate + (long)r * ld_gate + c), y = load_pack<T, V>(x + (long)r * ld_x + c);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             float z, omz;
             gate_of_code(gate_code((float)g.e[j]), z, omz);
             s[j] = fmaf(z, s[j], omz * (float)y.e[j]);
         }
-        store_floats<T, V>(h + (long)r * D + c, s);
+        if (live) store_floats<T, V>(h + (long)r * D + c, s);
     };
     advance(b);
     if (again)
         for (int r0 = b + 1; r0 < B; r0 += 64) {
             unsigned long long more = __ballot(r0 + lane < B && slot(min(r0 + lane, B - 1)) == k);
             while (more) {
-                advance(r0 + __ffsll(more) - 1);
+                const int r = r0 + __ffsll(more) - 1;
+                g = load_pack<T, V>(gate + (long)r * ld_gate + cc);
+                y = load_pack<T, V>(x + (long)r * ld_x + cc);
+                advance(r);
                 more &= more - 1;
             }
         }

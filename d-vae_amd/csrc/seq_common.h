@@ -8,11 +8,19 @@ namespace dvae {
 // V consecutive elements of T as one access (V * sizeof(T) <= 16 bytes, aligned to that)
 template <typename T, int V> struct alignas(sizeof(T) * V) Pack { T e[V]; };
 
+// the access itself as one integer vector (hipcc otherwise splits a constant pack into stores of its elements)
+template <int BYTES> struct Word;
+template <> struct Word<2> { typedef unsigned short type; };
+template <> struct Word<4> { typedef unsigned type; };
+template <> struct Word<8> { typedef unsigned type __attribute__((ext_vector_type(2))); };
+template <> struct Word<16> { typedef unsigned type __attribute__((ext_vector_type(4))); };
 template <typename T, int V> __device__ __forceinline__ Pack<T, V> load_pack(const T* p) {
-    return *reinterpret_cast<const Pack<T, V>*>(p);
+    typedef typename Word<sizeof(T) * V>::type W;
+    return __builtin_bit_cast(Pack<T, V>, *reinterpret_cast<const W*>(p));
 }
 template <typename T, int V> __device__ __forceinline__ void store_pack(T* p, const Pack<T, V>& v) {
-    *reinterpret_cast<Pack<T, V>*>(p) = v;
+    typedef typename Word<sizeof(T) * V>::type W;
+    *reinterpret_cast<W*>(p) = __builtin_bit_cast(W, v);
 }
 // one rounding, to nearest even
 template <typename T, int V> __device__ __forceinline__ void store_floats(T* p, const float (&f)[V]) {
