@@ -53,6 +53,11 @@ class LevelDesc(C.Structure):
                                          "ld_dhprev", "ldw_bf16")] + [("w_bf16", C.c_void_p)]
 
 
+class MatrixDesc(C.Structure):
+    """dvae_matrix_desc (include/dvae_hip.h)"""
+    _fields_ = [("g", C.c_void_p), ("out", C.c_void_p), ("ld_g", C.c_int64), ("ld_out", C.c_int64), ("rows", C.c_int32), ("cols", C.c_int32)]
+
+
 _P = C.c_void_p
 _I = C.c_int32
 _L = C.c_int64
@@ -112,6 +117,8 @@ SIGNATURES = {
     "dvae_scan_fwd": (_I, [_P, _L, _P, _L, _P, _I, _P, _P, _P, _P, _P, _L, _L, _I, _I, _P]),
     "dvae_scan_bwd": (_I, [_P, _L, _P, _L, _P, _I, _P, _P, _P, _L, _P, _P, _P, _P, _P, _L, _L, _I, _I, _P]),
     "dvae_scan_step": (_I, [_P, _L, _P, _L, _P, _L, _L, _P, _I, _P, _I, _I, _I, _P]),
+    "dvae_orthogonalize_ws_bytes": (_L, [C.POINTER(MatrixDesc), _I]),
+    "dvae_orthogonalize": (_I, [C.POINTER(MatrixDesc), _I, _I, C.POINTER(_F), _P, _I, _P]),
     "dvae_encode_ws_floats": (C.c_int64, [_MD, _BC]),
     "dvae_loss_ws_floats": (C.c_int64, [_MD, _BC]),
     "dvae_debug_side_stream": (_I, [_P, C.POINTER(_P)]),

@@ -13,6 +13,63 @@ import torch
 
 from . import _lib
 from .dist import GradSumReducer
+from .sequence import _matrix, _On, _workspace
+
+
+QUINTIC = (3.4445, -4.7750, 2.0315)  # p(s) = a s + b s^3 + c s^5: five steps take singular values from 0.002 up to 0.7 .. 1.2
+
+
+def orthogonalize(updates, steps=5, coefficients=QUINTIC, out=None):
+    """The nearest (semi-)orthogonal matrix to each of `updates`, approximately: `steps` Newton-Schulz steps
+    X <- a X + (b A + c A A) X with A = X X^T (on the smaller side) from X = G / |G|_F.
+
+    updates: a matrix or a list of matrices (float32, bfloat16 or float16, one type, on one HIP device); a list goes through
+    every product in one launch.  coefficients: (a, b, c), or one such triple for each step; a set that lets a singular value
+    leave [-2, 2] is refused.  out: where to write (same shapes and type; a matrix may be its own output), default new tensors.
+    Accuracy of float32 throughout, rounded once to the matrices' type.  A zero matrix gives zeros, one with a NaN or an
+    infinity NaN.  Not differentiable (it acts on updates)."""
+    one = torch.is_tensor(updates)
+    mats = [updates] if one else list(updates)
+    if out is not None:
+        outs = [out] if one else list(out)
+        if len(outs) != len(mats):
+            raise ValueError("out has %d matrices, updates %d" % (len(outs), len(mats)))
+    steps = int(steps)
+    triples = [tuple(coefficients)] * steps if not hasattr(coefficients[0], "__len__") else [tuple(c) for c in coefficients]
+    if len(triples) != steps or any(len(c) != 3 for c in triples):
+        raise ValueError("coefficients must be (a, b, c) or one such triple for each of the %d steps" % steps)
+    if not mats:
+        return []
+    code = _matrix(mats[0], "updates", 2)
+    dtype, device = mats[0].dtype, mats[0].device
+    with torch.no_grad():
+        srcs = []
+        for g in mats:
+            _matrix(g, "updates", 2)
+            if g.dtype != dtype or g.device != device:
+                raise ValueError("the matrices of one call must have one type and one device")
+            if g.numel() == 0:
+                raise ValueError("updates: an empty matrix")
+            srcs.append(g if (g.shape[1] == 1 or g.stride(1) == 1) and (g.shape[0] == 1 or g.stride(0) >= g.shape[1]) else g.contiguous())
+        if out is None:
+            outs = [torch.empty(g.shape, dtype=dtype, device=device) for g in mats]
+        else:
+            for o, g in zip(outs, mats):
+                if o.shape != g.shape or o.dtype != dtype or o.device != device:
+                    raise ValueError("out must have the shapes, type and device of updates")
+                if (o.shape[1] > 1 and o.stride(1) != 1) or (o.shape[0] > 1 and o.stride(0) < o.shape[1]):
+                    raise ValueError("out: the elements of a row must lie side by side")
+        lib = _lib.load()
+        descs = (_lib.MatrixDesc * len(mats))(*[
+            _lib.MatrixDesc(g.data_ptr(), o.data_ptr(), g.stride(0) if g.shape[0] > 1 else g.shape[1],
+                            o.stride(0) if o.shape[0] > 1 else o.shape[1], g.shape[0], g.shape[1]) for g, o in zip(srcs, outs)])
+        abc = (C.c_float * (3 * steps))(*[v for c in triples for v in c])
+        ws = _workspace(lib.dvae_orthogonalize_ws_bytes(descs, len(mats)), device, "dvae_orthogonalize_ws_bytes")
+        with _On(device) as stream:
+            _lib.check(lib.dvae_orthogonalize(descs, len(mats), steps, abc, ws.data_ptr(), code, stream), "dvae_orthogonalize")
+        if out is not None:
+            torch.autograd.graph.increment_version(outs)
+    return outs[0] if one else outs
 
 
 class FlatAdam(torch.optim.Optimizer):

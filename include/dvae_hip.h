@@ -490,6 +490,24 @@ int dvae_scan_step(const void* gate, int64_t ld_gate, const void* x, int64_t ld_
                    int64_t pool, const void* slots, int32_t slots_i64, void* h, int32_t rows, int32_t D, int32_t dtype,
                    void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Orthogonalised updates (the matrix step of optim.FlatMuon, beside Adam above).
+ * out = the last X of `steps` Newton-Schulz steps X <- a X + (b A + c A A) X, A = X X^T (on the smaller side), from
+ * X = g / |g|_F, for `count` matrices of one element type (HOST array of descriptors; g, out device pointers, row strides in
+ * elements, out not overlapping any g).  coefficients (host): a, b, c of every step, 3 * steps floats; sets that let a singular
+ * value leave [-2, 2] are refused.  fp32 accuracy whatever the type (split fp16 planes, see csrc/orthogonalize.hip), rounded
+ * once at the end; a zero matrix gives zeros, one that holds a NaN or an infinity gives NaN.  Sides up to 32768.
+ * ws: dvae_orthogonalize_ws_bytes() bytes, 16-byte aligned, for this call alone. */
+typedef struct dvae_matrix_desc {
+    const void* g;
+    void* out;
+    int64_t ld_g, ld_out;
+    int32_t rows, cols;
+} dvae_matrix_desc;
+int64_t dvae_orthogonalize_ws_bytes(const dvae_matrix_desc* mats, int32_t count);
+int dvae_orthogonalize(const dvae_matrix_desc* mats, int32_t count, int32_t steps, const float* coefficients, void* ws,
+                       int32_t dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
