@@ -117,7 +117,7 @@ SIGNATURES = {
     "dvae_scan_fwd": (_I, [_P, _L, _P, _L, _P, _I, _P, _P, _P, _P, _P, _L, _L, _I, _I, _P]),
     "dvae_scan_bwd": (_I, [_P, _L, _P, _L, _P, _I, _P, _P, _P, _L, _P, _P, _P, _P, _P, _L, _L, _I, _I, _P]),
     "dvae_scan_step": (_I, [_P, _L, _P, _L, _P, _L, _L, _P, _I, _P, _I, _I, _I, _P]),
-    "dvae_orthogonalize_ws_bytes": (_L, [C.POINTER(MatrixDesc), _I]),
+    "dvae_orthogonalize_ws_bytes": (_L, [C.POINTER(MatrixDesc), _I, _I]),
     "dvae_orthogonalize": (_I, [C.POINTER(MatrixDesc), _I, _I, C.POINTER(_F), _P, _I, _P]),
     "dvae_encode_ws_floats": (C.c_int64, [_MD, _BC]),
     "dvae_loss_ws_floats": (C.c_int64, [_MD, _BC]),

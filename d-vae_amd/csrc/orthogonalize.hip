@@ -30,7 +30,7 @@ typedef float nsf32x16 __attribute__((ext_vector_type(16)));
 typedef unsigned nsu32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int NS_GROUP = 32;          // matrices per launch
-constexpr int NS_PARTS = 64;          // partial sums of a norm
+constexpr int NS_PARTS = 256;         // partial sums of a norm
 constexpr float NS_S = 8192.f;        // 2^13
 constexpr int NS_LDS_ROW = 128 + 16;  // bytes: a 16-lane group's fragments fall on all banks
 
@@ -46,7 +46,7 @@ struct NsMat {
 };
 struct NsGroup {
     NsMat mat[NS_GROUP];
-    int count, dtype;
+    int count, dtype, planes, pad;  // sides are padded to whole multiples of `pad` with zeros
     char* ws;
     double* parts;  // [count][NS_PARTS]
     float* r;       // [count]
@@ -54,14 +54,14 @@ struct NsGroup {
 };
 
 __host__ __device__ inline int ns_pad(int v, int tb) { return (v + tb - 1) / tb * tb; }
-__host__ __device__ inline long ns_bytes(int mp, int np) { return (long)mp * np * 4; }
+__host__ __device__ inline long ns_bytes(int mp, int np, int planes) { return (long)mp * np * 2 * planes; }
 // 0 / 1: X / X^T, 2 / 3: the other pair, 4: A, 5: B
-__host__ __device__ inline long ns_offset(int mp, int np, int which) {
-    const long x = ns_bytes(mp, np);
-    return which < 4 ? which * x : 4 * x + (which - 4) * ns_bytes(mp, mp);
+__host__ __device__ inline long ns_offset(int mp, int np, int planes, int which) {
+    const long x = ns_bytes(mp, np, planes);
+    return which < 4 ? which * x : 4 * x + (which - 4) * ns_bytes(mp, mp, planes);
 }
-// byte of column k in a row of blocks, plane 0 (hi); plane 1 is 64 bytes behind
-__device__ __forceinline__ int ns_col(int k) { return (k >> 5) * 128 + (k & 31) * 2; }
+// byte of column k in a row of blocks; the second plane is 64 bytes behind
+template <int PL> __device__ __forceinline__ int ns_col(int k) { return PL == 2 ? (k >> 5) * 128 + (k & 31) * 2 : k * 2; }
 
 // which matrix a unit of the grid belongs to
 __device__ __forceinline__ int ns_find(const NsGroup& p, int unit) {
@@ -71,12 +71,18 @@ __device__ __forceinline__ int ns_find(const NsGroup& p, int unit) {
 }
 
 template <typename T> __device__ __forceinline__ void ns_sum(const NsMat& m, double* out) {
-    const T* g = (const T*)m.g;
+    // NS_PARTS workgroups: as many rows each as there are, and where there are few, shares of the columns
+    const int across = m.rows >= NS_PARTS ? 1 : NS_PARTS / m.rows, down = NS_PARTS / across;
+    const int r0 = blockIdx.x / across, c0 = blockIdx.x % across;
     double s = 0;
-    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < (long)m.rows * m.cols; i += NS_PARTS * 256) {
-        const double v = (double)(float)g[(i / m.cols) * m.ld_g + i % m.cols];
-        s += v * v;
-    }
+    if (r0 < down)
+        for (int r = r0; r < m.rows; r += down) {
+            const T* row = (const T*)m.g + r * m.ld_g;
+            for (int c = c0 * 256 + threadIdx.x; c < m.cols; c += across * 256) {
+                const double v = (double)(float)row[c];
+                s += v * v;
+            }
+        }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
     __shared__ double w[4];
@@ -93,21 +99,39 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(NsGroup p) {
     else ns_sum<_Float16>(m, out);
 }
 
-__device__ __forceinline__ void ns_split(float v, _Float16& hi, _Float16& lo) {
-    hi = (_Float16)v;
-    lo = (_Float16)(v - (float)hi);
+// Eight scaled values to eight columns of a row of blocks
+template <int PL> __device__ __forceinline__ void ns_put8(char* at, const float (&v)[8]) {
+    h16x8 hi, lo;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        hi[e] = (_Float16)v[e];
+        lo[e] = (_Float16)(v[e] - (float)hi[e]);
+    }
+    *(h16x8*)at = hi;
+    if (PL == 2) *(h16x8*)(at + 64) = lo;
 }
 
 // G -> X and X^T in planes: 64 x 64 tiles of G (padding included) through LDS
-__global__ __launch_bounds__(256) void ns_split_kernel(NsGroup p, int tb) {
+template <int PL> __global__ __launch_bounds__(256) void ns_split_kernel(NsGroup p) {
     __shared__ float tile[64][65];
     __shared__ int expo;
     const int k = ns_find(p, blockIdx.x);
     const NsMat& m = p.mat[k];
-    const int rp = ns_pad(m.rows, tb), cp = ns_pad(m.cols, tb);
+    const int rp = ns_pad(m.rows, p.pad), cp = ns_pad(m.cols, p.pad);
     const int t = blockIdx.x - m.tile0, r0 = t / (cp / 64) * 64, c0 = t % (cp / 64) * 64;
+    const int j = threadIdx.x & 63, i0 = threadIdx.x >> 6;
+    float g[16];
+#pragma unroll
+    for (int u = 0; u < 16; ++u) {
+        const int r = r0 + i0 + 4 * u, c = c0 + j;
+        const long at = (long)min(r, m.rows - 1) * m.ld_g + min(c, m.cols - 1);
+        const float v = p.dtype == DVAE_F32 ? ((const float*)m.g)[at] : p.dtype == DVAE_BF16 ? (float)((const __bf16*)m.g)[at] : (float)((const _Float16*)m.g)[at];
+        g[u] = r < m.rows && c < m.cols ? v : 0.f;
+    }
     if (threadIdx.x < 64) {
-        double s = p.parts[k * NS_PARTS + threadIdx.x];
+        double s = 0;
+#pragma unroll
+        for (int u = 0; u < NS_PARTS / 64; ++u) s += p.parts[k * NS_PARTS + u * 64 + threadIdx.x];
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
         if (threadIdx.x == 0) {
@@ -119,44 +143,38 @@ __global__ __launch_bounds__(256) void ns_split_kernel(NsGroup p, int tb) {
     }
     __syncthreads();
     const double scale = ldexp((double)NS_S, -expo);
-    const int j = threadIdx.x & 63;
-    for (int i = threadIdx.x >> 6; i < 64; i += 4) {
-        float v = 0.f;
-        if (r0 + i < m.rows && c0 + j < m.cols) {
-            const long at = (long)(r0 + i) * m.ld_g + c0 + j;
-            v = p.dtype == DVAE_F32 ? ((const float*)m.g)[at] : p.dtype == DVAE_BF16 ? (float)((const __bf16*)m.g)[at] : (float)((const _Float16*)m.g)[at];
-            v = (float)((double)v * scale);
-        }
-        tile[i][j] = v;
-    }
+#pragma unroll
+    for (int u = 0; u < 16; ++u) tile[i0 + 4 * u][j] = (float)((double)g[u] * scale);
     __syncthreads();
     const bool wide = m.rows <= m.cols;
     const int mp = wide ? rp : cp, np = wide ? cp : rp;
-    char* straight = p.ws + m.base + ns_offset(mp, np, wide ? 0 : 1);  // rows as G's
-    char* turned = p.ws + m.base + ns_offset(mp, np, wide ? 1 : 0);
-    for (int i = threadIdx.x >> 6; i < 64; i += 4) {
-        _Float16 hi, lo;
-        ns_split(tile[i][j], hi, lo);
-        char* at = straight + (long)(r0 + i) * cp * 4 + ns_col(c0 + j);
-        *(_Float16*)at = hi;
-        *(_Float16*)(at + 64) = lo;
-        ns_split(tile[j][i], hi, lo);
-        at = turned + (long)(c0 + i) * rp * 4 + ns_col(r0 + j);
-        *(_Float16*)at = hi;
-        *(_Float16*)(at + 64) = lo;
+    char* straight = p.ws + m.base + ns_offset(mp, np, PL, wide ? 0 : 1);  // rows as G's
+    char* turned = p.ws + m.base + ns_offset(mp, np, PL, wide ? 1 : 0);
+#pragma unroll
+    for (int u = threadIdx.x; u < 512; u += 256) {
+        const int row = u >> 3, c8 = (u & 7) * 8;
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = tile[row][c8 + e];
+        ns_put8<PL>(straight + (long)(r0 + row) * cp * 2 * PL + ns_col<PL>(c0 + c8), v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = tile[c8 + e][row];
+        ns_put8<PL>(turned + (long)(c0 + row) * rp * 2 * PL + ns_col<PL>(r0 + c8), v);
     }
 }
 
 enum { NS_GRAM, NS_POLY, NS_STEP, NS_LAST };
 
 // One of the products, TB x TB output tiles, 4 waves as 2 x 2, each TB/2 x TB/2 of 32 x 32 MFMA blocks.  A stage of the K
-// loop is one block (32 columns, both planes) of TB rows of either operand; the next stage's loads are in flight during
-// the MFMAs and go to the other half of LDS behind them.
-template <int TB, int MODE>
+// loop is one block (32 columns in two planes, 64 in one) of TB rows of either operand.  The loads run PF stages ahead in
+// registers and go to the other half of LDS in the middle of the stage before theirs.
+template <int TB, int PL, int PF, int MODE>
 __global__ __launch_bounds__(256) void ns_product_kernel(NsGroup p, int from, int first) {
     constexpr int TM = TB / 64;
-    constexpr int PASSES = TB / 32;  // 16 bytes per thread and pass: 32 rows
+    constexpr int PASSES = TB / 32;  // 16 bytes per thread and pass: 32 rows of one block
     constexpr int OPERAND = TB * NS_LDS_ROW;
+    constexpr int TP = TB + 4;       // row pitch of the output tile in LDS, floats
+    static_assert(PF % 2 == 0 && TB * TP * 4 <= 4 * OPERAND, "");
     __shared__ __attribute__((aligned(16))) char lds[2][2 * OPERAND];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     // workgroups that share an XCD (equal id mod 8) take neighbouring tiles
@@ -164,7 +182,7 @@ __global__ __launch_bounds__(256) void ns_product_kernel(NsGroup p, int from, in
     const int unit = (xcd < rest ? xcd * (q + 1) : rest * (q + 1) + (xcd - rest) * q) + (blockIdx.x >> 3);
     const int k = ns_find(p, unit);
     const NsMat& m = p.mat[k];
-    const int mp = ns_pad(m.m(), TB), np = ns_pad(m.n(), TB), mt = mp / TB, nt = np / TB;
+    const int mp = ns_pad(m.m(), p.pad), np = ns_pad(m.n(), p.pad), mt = mp / TB, nt = np / TB;
     const int t = unit - m.tile0;
     int ti, tj;
     if (MODE == NS_GRAM || MODE == NS_POLY) {  // row by row of the upper triangle: row i begins at i mt - i (i - 1) / 2
@@ -178,10 +196,10 @@ __global__ __launch_bounds__(256) void ns_product_kernel(NsGroup p, int from, in
         tj = in / rows;
     }
     char* const base = p.ws + m.base;
-    const long pitch = (long)(MODE == NS_GRAM ? np : mp) * 4;  // of both operands
-    const char* a_rows = base + ns_offset(mp, np, MODE == NS_GRAM ? from : MODE == NS_POLY ? 4 : 5) + (long)ti * TB * pitch;
-    const char* b_rows = base + ns_offset(mp, np, MODE == NS_GRAM ? from : MODE == NS_POLY ? 4 : from + 1) + (long)tj * TB * pitch;
-    const int blocks = (int)(pitch / 128);
+    const long pitch = (long)(MODE == NS_GRAM ? np : mp) * 2 * PL;  // of both operands
+    const char* a_rows = base + ns_offset(mp, np, PL, MODE == NS_GRAM ? from : MODE == NS_POLY ? 4 : 5) + (long)ti * TB * pitch;
+    const char* b_rows = base + ns_offset(mp, np, PL, MODE == NS_GRAM ? from : MODE == NS_POLY ? 4 : from + 1) + (long)tj * TB * pitch;
+    const int stages = (int)(pitch / 128);
 
     nsf32x16 acc[TM][TM];
 #pragma unroll
@@ -193,121 +211,139 @@ __global__ __launch_bounds__(256) void ns_product_kernel(NsGroup p, int from, in
     const int wm = wave >> 1, wn = wave & 1;
     const long my = (long)(tid >> 3) * pitch + (tid & 7) * 16;
     const int my_lds = (tid >> 3) * NS_LDS_ROW + (tid & 7) * 16;
-    nsu32x4 ra[PASSES], rb[PASSES];
-    auto load = [&](int s) {
+    nsu32x4 ra[PF][PASSES], rb[PF][PASSES];
+    auto load = [&](int u, int s) {  // past the last stage the last one is loaded again and not used
+        const long at = my + (long)min(s, stages - 1) * 128;
 #pragma unroll
         for (int i = 0; i < PASSES; ++i) {
-            ra[i] = *(const nsu32x4*)(a_rows + my + i * 32 * pitch + (long)s * 128);
-            rb[i] = *(const nsu32x4*)(b_rows + my + i * 32 * pitch + (long)s * 128);
+            ra[u][i] = *(const nsu32x4*)(a_rows + at + i * 32 * pitch);
+            rb[u][i] = *(const nsu32x4*)(b_rows + at + i * 32 * pitch);
         }
     };
-    auto store = [&](char* l) {
+    auto store = [&](int u, char* l) {
 #pragma unroll
         for (int i = 0; i < PASSES; ++i) {
-            *(nsu32x4*)(l + my_lds + i * 32 * NS_LDS_ROW) = ra[i];
-            *(nsu32x4*)(l + OPERAND + my_lds + i * 32 * NS_LDS_ROW) = rb[i];
+            *(nsu32x4*)(l + my_lds + i * 32 * NS_LDS_ROW) = ra[u][i];
+            *(nsu32x4*)(l + OPERAND + my_lds + i * 32 * NS_LDS_ROW) = rb[u][i];
         }
     };
-    load(0);
-    store(lds[0]);
-    load(min(1, blocks - 1));
+#pragma unroll
+    for (int u = 0; u < PF; ++u) load(u, u);
+    store(0, lds[0]);
     __syncthreads();
     // lane l of a fragment: row l & 31, columns 8 (l >> 5) .. + 7 of 16
     const int frag = (lane & 31) * NS_LDS_ROW + (lane >> 5) * 16;
-    for (int s = 0; s < blocks; ++s) {
-        const char* la = lds[s & 1] + wm * (TB / 2) * NS_LDS_ROW + frag;
-        const char* lb = lds[s & 1] + OPERAND + wn * (TB / 2) * NS_LDS_ROW + frag;
+    constexpr int SUB = PL == 2 ? 2 : 4;  // 16-column steps of a stage
+    for (int s0 = 0; s0 < stages; s0 += PF) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            h16x8 ah[TM], al[TM], bh[TM], bl[TM];
+        for (int u = 0; u < PF; ++u) {
+            const int s = s0 + u;
+            if (s >= stages) break;
+            const char* la = lds[u & 1] + wm * (TB / 2) * NS_LDS_ROW + frag;
+            const char* lb = lds[u & 1] + OPERAND + wn * (TB / 2) * NS_LDS_ROW + frag;
 #pragma unroll
-            for (int i = 0; i < TM; ++i) {
-                ah[i] = *(const h16x8*)(la + i * 32 * NS_LDS_ROW + h * 32);
-                al[i] = *(const h16x8*)(la + i * 32 * NS_LDS_ROW + h * 32 + 64);
-                bh[i] = *(const h16x8*)(lb + i * 32 * NS_LDS_ROW + h * 32);
-                bl[i] = *(const h16x8*)(lb + i * 32 * NS_LDS_ROW + h * 32 + 64);
+            for (int h = 0; h < SUB; ++h) {
+                h16x8 ah[TM], al[TM], bh[TM], bl[TM];
+#pragma unroll
+                for (int i = 0; i < TM; ++i) {
+                    ah[i] = *(const h16x8*)(la + i * 32 * NS_LDS_ROW + h * 32);
+                    bh[i] = *(const h16x8*)(lb + i * 32 * NS_LDS_ROW + h * 32);
+                    if (PL == 2) {
+                        al[i] = *(const h16x8*)(la + i * 32 * NS_LDS_ROW + h * 32 + 64);
+                        bl[i] = *(const h16x8*)(lb + i * 32 * NS_LDS_ROW + h * 32 + 64);
+                    }
+                }
+                auto mma = [&](const h16x8 (&x)[TM], const h16x8 (&y)[TM]) {
+#pragma unroll
+                    for (int i = 0; i < TM; ++i)
+#pragma unroll
+                        for (int j = 0; j < TM; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[i], y[j], acc[i][j], 0, 0, 0);
+                };
+                if (PL == 2) {
+                    mma(al, bh);
+                    mma(ah, bl);
+                }
+                mma(ah, bh);
+                if (h == SUB / 2 - 1) {
+                    store((u + 1) % PF, lds[(u & 1) ^ 1]);
+                    __builtin_amdgcn_sched_barrier(0);
+                    load(u, s + PF);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
             }
-#pragma unroll
-            for (int i = 0; i < TM; ++i)
-#pragma unroll
-                for (int j = 0; j < TM; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al[i], bh[j], acc[i][j], 0, 0, 0);
-#pragma unroll
-            for (int i = 0; i < TM; ++i)
-#pragma unroll
-                for (int j = 0; j < TM; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[i], bl[j], acc[i][j], 0, 0, 0);
-#pragma unroll
-            for (int i = 0; i < TM; ++i)
-#pragma unroll
-                for (int j = 0; j < TM; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[i], bh[j], acc[i][j], 0, 0, 0);
-            if (h == 0) {
-                store(lds[(s & 1) ^ 1]);
-                __builtin_amdgcn_sched_barrier(0);
-                load(min(s + 2, blocks - 1));
-                __builtin_amdgcn_sched_barrier(0);
-            }
+            __syncthreads();
         }
-        __syncthreads();
     }
 
-    // Epilogue.  Lane l of a block holds column l & 31 and rows (r & 3) + 8 (r >> 2) + 4 (l >> 5): quads of rows of one
-    // column, which are contiguous in the turned copy.  The source of the added multiple is read from there.
+    // Epilogue: the tile goes through LDS, so that every access to memory is 16 bytes of a row in either orientation.
+    // Lane l of an MFMA block holds column l & 31 and rows (r & 3) + 8 (r >> 2) + 4 (l >> 5).
     const float r = first ? p.r[k] : 1.f;
-    const float unscale = 1.f / (NS_S * NS_S);
-    const float from_src = MODE == NS_GRAM ? 0.f : MODE == NS_POLY ? p.b * r * r * r : p.a * r;
-    const float from_acc = unscale * (MODE == NS_POLY ? p.c * r * r * r * r * r : 1.f);
-    const char* src = base + ns_offset(mp, np, MODE == NS_POLY ? 4 : from + 1);  // rows of mp columns
-    const int to = from ^ 2;
-    char* straight = base + ns_offset(mp, np, MODE == NS_GRAM ? 4 : MODE == NS_POLY ? 5 : to);
-    char* turned = MODE == NS_STEP ? base + ns_offset(mp, np, to + 1) : straight;
-    const long straight_pitch = (long)(MODE == NS_STEP ? np : mp) * 4, turned_pitch = (long)mp * 4;
-    const bool mirror = MODE == NS_STEP || ti != tj;  // a diagonal tile of a symmetric product has its mirror in itself
+    const float from_src = MODE == NS_GRAM ? 0.f : (MODE == NS_POLY ? p.b * r * r * r : p.a * r) / NS_S;
+    const float from_acc = (MODE == NS_POLY ? p.c * r * r * r * r * r : 1.f) / (NS_S * NS_S);
+    float* const tile = (float*)&lds[0][0];
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
-        for (int j = 0; j < TM; ++j) {
-            const int col = tj * TB + wn * (TB / 2) + j * 32 + (lane & 31);
+        for (int j = 0; j < TM; ++j)
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const int row = ti * TB + wm * (TB / 2) + i * 32 + u * 8 + 4 * (lane >> 5);
-                const long at = col * turned_pitch + ns_col(row);
-                float v[4];
+            for (int e = 0; e < 16; ++e)
+                tile[(wm * (TB / 2) + i * 32 + (e & 3) + 8 * (e >> 2) + 4 * (lane >> 5)) * TP + wn * (TB / 2) + j * 32 + (lane & 31)] =
+                    acc[i][j][e] * from_acc;
+    __syncthreads();
+    const int row0 = ti * TB, col0 = tj * TB;
+    const bool mirror = MODE == NS_STEP || ((MODE == NS_GRAM || MODE == NS_POLY) && ti != tj);  // a diagonal tile is its own mirror
+    {
+        const char* src = base + ns_offset(mp, np, PL, MODE == NS_POLY ? 4 : from);
+        char* dst = base + ns_offset(mp, np, PL, MODE == NS_GRAM ? 4 : MODE == NS_POLY ? 5 : from ^ 2);
+        const long row_bytes = (long)(MODE == NS_STEP || MODE == NS_LAST ? np : mp) * 2 * PL;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = acc[i][j][u * 4 + e] * from_acc;
-                if (MODE != NS_GRAM) {
-                    const h16x4 sh = *(const h16x4*)(src + at), sl = *(const h16x4*)(src + at + 64);
+        for (int u = tid; u < TB * TB / 8; u += 256) {
+            const int row = u / (TB / 8), c8 = u % (TB / 8) * 8;
+            const long at = (long)(row0 + row) * row_bytes + ns_col<PL>(col0 + c8);
+            float v[8];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] = fmaf(((float)sh[e] + (float)sl[e]) * (1.f / NS_S), from_src, v[e]);
-                }
-                if (MODE == NS_LAST) {
-                    const bool wide = m.rows <= m.cols;
-                    if (col >= m.n()) continue;
+            for (int e = 0; e < 8; ++e) v[e] = tile[row * TP + c8 + e];
+            if (MODE != NS_GRAM) {
+                const h16x8 hi = *(const h16x8*)(src + at);
+                h16x8 lo = {};
+                if (PL == 2) lo = *(const h16x8*)(src + at + 64);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        if (row + e >= m.m()) continue;
-                        const long o = wide ? (long)(row + e) * m.ld_out + col : (long)col * m.ld_out + row + e;
-                        if (p.dtype == DVAE_F32) ((float*)m.out)[o] = v[e];
-                        else if (p.dtype == DVAE_BF16) ((__bf16*)m.out)[o] = (__bf16)v[e];
-                        else ((_Float16*)m.out)[o] = (_Float16)v[e];
-                    }
-                } else {
-                    h16x4 hi, lo;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        _Float16 a, b;
-                        ns_split(v[e] * NS_S, a, b);
-                        hi[e] = a;
-                        lo[e] = b;
-                        char* o = straight + (row + e) * straight_pitch + ns_col(col);
-                        *(_Float16*)o = a;
-                        *(_Float16*)(o + 64) = b;
-                    }
-                    if (mirror) {
-                        *(h16x4*)(turned + at) = hi;
-                        *(h16x4*)(turned + at + 64) = lo;
-                    }
+                for (int e = 0; e < 8; ++e) {
+                    v[e] = fmaf((float)hi[e] + (float)lo[e], from_src, v[e]);
+                    if (MODE == NS_LAST || mirror) tile[row * TP + c8 + e] = v[e];
                 }
             }
+            if (MODE != NS_LAST) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] *= NS_S;
+                ns_put8<PL>(dst + at, v);
+            }
         }
+    }
+    if (MODE == NS_LAST) {
+        __syncthreads();
+        const bool wide = m.rows <= m.cols;  // else the rows of out are the columns of X
+        for (int u = tid; u < TB * TB; u += 256) {
+            const int row = wide ? u / TB : u % TB, col = wide ? u % TB : u / TB;
+            if (row0 + row >= m.m() || col0 + col >= m.n()) continue;
+            const float v = tile[row * TP + col];
+            const long o = wide ? (long)(row0 + row) * m.ld_out + col0 + col : (long)(col0 + col) * m.ld_out + row0 + row;
+            if (p.dtype == DVAE_F32) ((float*)m.out)[o] = v;
+            else if (p.dtype == DVAE_BF16) ((__bf16*)m.out)[o] = (__bf16)v;
+            else ((_Float16*)m.out)[o] = (_Float16)v;
+        }
+    } else if (mirror) {
+        if (MODE != NS_GRAM) __syncthreads();
+        char* dst = base + ns_offset(mp, np, PL, MODE == NS_GRAM ? 4 : MODE == NS_POLY ? 5 : (from ^ 2) + 1);
+#pragma unroll
+        for (int u = tid; u < TB * TB / 8; u += 256) {
+            const int col = u / (TB / 8), r8 = u % (TB / 8) * 8;
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = tile[(r8 + e) * TP + col] * NS_S;
+            ns_put8<PL>(dst + (long)(col0 + col) * mp * 2 * PL + ns_col<PL>(row0 + r8), v);
+        }
+    }
 }
 
 static int ns_cus() {
@@ -319,15 +355,24 @@ static int ns_cus() {
     return cus;
 }
 
-// tile of a call: 128 where the update products of a group fill the chip with them
-static int ns_tile(const dvae_matrix_desc* d, int32_t count) {
+// A product runs on 128 x 128 tiles where those fill the chip one and a quarter times, else on 64 x 64.
+static bool ns_big(long tiles128) { return 4 * tiles128 >= 5L * ns_cus(); }
+// what the sides are padded to: to 64 where not even the update products, the ones with most tiles, use the larger tile
+static int ns_pad_of(const dvae_matrix_desc* d, int32_t count) {
     long tiles = 0;
     for (int i = 0; i < count; ++i) tiles += (long)cdiv(d[i].rows, 128) * cdiv(d[i].cols, 128);
-    return tiles >= ns_cus() ? 128 : 64;
+    return ns_big(tiles) ? 128 : 64;
 }
-static long ns_matrix_bytes(const dvae_matrix_desc& d, int tb) {
-    const int mp = ns_pad(d.rows < d.cols ? d.rows : d.cols, tb), np = ns_pad(d.rows < d.cols ? d.cols : d.rows, tb);
-    return ns_offset(mp, np, 6);
+static long ns_matrix_bytes(const dvae_matrix_desc& d, int pad, int planes) {
+    const int mp = ns_pad(d.rows < d.cols ? d.rows : d.cols, pad), np = ns_pad(d.rows < d.cols ? d.cols : d.rows, pad);
+    return ns_offset(mp, np, planes, 6);
+}
+// One plane for a group of bf16 matrices whose smaller sides are all at least 512; see the head of the file.
+static int ns_planes(const dvae_matrix_desc* d, int32_t count, int dtype) {
+    if (dtype != DVAE_BF16) return 2;
+    for (int i = 0; i < count; ++i)
+        if (d[i].rows < 512 || d[i].cols < 512) return 2;
+    return 1;
 }
 constexpr long NS_HEAD = NS_GROUP * (NS_PARTS * 8 + 8);
 
@@ -341,14 +386,15 @@ static int ns_check(const char* who, const dvae_matrix_desc* d, int32_t count) {
 
 }  // namespace dvae
 
-extern "C" int64_t dvae_orthogonalize_ws_bytes(const dvae_matrix_desc* mats, int32_t count) {
+extern "C" int64_t dvae_orthogonalize_ws_bytes(const dvae_matrix_desc* mats, int32_t count, int32_t dtype) {
     using namespace dvae;
+    DVAE_REQUIRE(known_dtype(dtype), "orthogonalize_ws_bytes: unknown element type %d", dtype);
     DVAE_TRY(ns_check("orthogonalize_ws_bytes", mats, count));
     int64_t most = 0;
     for (int g0 = 0; g0 < count; g0 += NS_GROUP) {  // the groups follow each other on the stream and share the space
-        const int n = count - g0 < NS_GROUP ? count - g0 : NS_GROUP, tb = ns_tile(mats + g0, n);
+        const int n = count - g0 < NS_GROUP ? count - g0 : NS_GROUP, pad = ns_pad_of(mats + g0, n), planes = ns_planes(mats + g0, n, dtype);
         int64_t sum = NS_HEAD;
-        for (int i = 0; i < n; ++i) sum += ns_matrix_bytes(mats[g0 + i], tb);
+        for (int i = 0; i < n; ++i) sum += ns_matrix_bytes(mats[g0 + i], pad, planes);
         most = sum > most ? sum : most;
     }
     return most;
@@ -382,49 +428,74 @@ extern "C" int dvae_orthogonalize(const dvae_matrix_desc* mats, int32_t count, i
     DVAE_REQUIRE(ws && (uintptr_t)ws % 16 == 0, "orthogonalize: the workspace must be 16-byte aligned");
     hipStream_t s = (hipStream_t)stream;
     for (int g0 = 0; g0 < count; g0 += NS_GROUP) {
-        const int n = count - g0 < NS_GROUP ? count - g0 : NS_GROUP, tb = ns_tile(mats + g0, n);
+        const int n = count - g0 < NS_GROUP ? count - g0 : NS_GROUP;
         NsGroup p = {};
         p.count = n;
         p.dtype = dtype;
+        p.planes = ns_planes(mats + g0, n, dtype);
+        p.pad = ns_pad_of(mats + g0, n);
         p.parts = (double*)ws;
         p.r = (float*)((char*)ws + NS_GROUP * NS_PARTS * 8);
         p.ws = (char*)ws + NS_HEAD;
+        // the matrices with the longest sums first: their tiles are the last to end
+        int order[NS_GROUP];
+        for (int i = 0; i < n; ++i) order[i] = g0 + i;
+        for (int i = 1; i < n; ++i)
+            for (int j = i; j > 0; --j) {
+                auto longer = [&](int k) { return mats[k].rows > mats[k].cols ? mats[k].rows : mats[k].cols; };
+                if (longer(order[j]) <= longer(order[j - 1])) break;
+                const int swap = order[j]; order[j] = order[j - 1]; order[j - 1] = swap;
+            }
         long base = 0;
-        int split = 0, square = 0, update = 0;
-        int tri0[NS_GROUP], upd0[NS_GROUP], spl0[NS_GROUP];
+        int split = 0, square[2] = {0, 0}, update[2] = {0, 0};  // tiles of all matrices; [0]: 64 x 64, [1]: 128 x 128
+        int split0[NS_GROUP], square0[2][NS_GROUP], update0[2][NS_GROUP];
         for (int i = 0; i < n; ++i) {
-            const dvae_matrix_desc& d = mats[g0 + i];
+            const dvae_matrix_desc& d = mats[order[i]];
             NsMat& m = p.mat[i];
             m.g = d.g; m.out = d.out; m.ld_g = d.ld_g; m.ld_out = d.ld_out; m.rows = d.rows; m.cols = d.cols; m.base = base;
-            base += ns_matrix_bytes(d, tb);
-            const int mt = ns_pad(m.m(), tb) / tb, nt = ns_pad(m.n(), tb) / tb;
-            spl0[i] = split; tri0[i] = square; upd0[i] = update;
-            split += mt * nt * (tb / 64) * (tb / 64);
-            square += mt * (mt + 1) / 2;
-            update += mt * nt;
+            base += ns_matrix_bytes(d, p.pad, p.planes);
+            const int mp = ns_pad(m.m(), p.pad), np = ns_pad(m.n(), p.pad);
+            split0[i] = split;
+            split += (mp / 64) * (np / 64);
+            for (int b = 0; b < 2; ++b) {
+                const int mt = mp / (64 << b), nt = np / (64 << b);
+                square0[b][i] = square[b]; update0[b][i] = update[b];
+                square[b] += mt * (mt + 1) / 2;
+                update[b] += mt * nt;
+            }
         }
+        const int sq = p.pad == 128 && ns_big(square[1]), up = p.pad == 128 && ns_big(update[1]);
         auto place = [&](const int* at) { for (int i = 0; i < n; ++i) p.mat[i].tile0 = at[i]; };
         hipLaunchKernelGGL(ns_norm_kernel, dim3(NS_PARTS, n), dim3(256), 0, s, p);
         DVAE_LAUNCH_CHECK();
-        place(spl0);
-        hipLaunchKernelGGL(ns_split_kernel, dim3(split), dim3(256), 0, s, p, tb);
+        place(split0);
+        if (p.planes == 2) hipLaunchKernelGGL((ns_split_kernel<2>), dim3(split), dim3(256), 0, s, p);
+        else hipLaunchKernelGGL((ns_split_kernel<1>), dim3(split), dim3(256), 0, s, p);
         DVAE_LAUNCH_CHECK();
-#define NS_PRODUCT(MODE, grid)                                                                                                 \
-    do {                                                                                                                       \
-        if (tb == 128) hipLaunchKernelGGL((ns_product_kernel<128, MODE>), dim3(grid), dim3(256), 0, s, p, 2 * (t & 1), t == 0); \
-        else hipLaunchKernelGGL((ns_product_kernel<64, MODE>), dim3(grid), dim3(256), 0, s, p, 2 * (t & 1), t == 0);           \
-        DVAE_LAUNCH_CHECK();                                                                                                   \
+#define NS_LAUNCH(TB, PL, PF, MODE, grid) \
+    hipLaunchKernelGGL((ns_product_kernel<TB, PL, PF, MODE>), dim3(grid), dim3(256), 0, s, p, 2 * (t & 1), t == 0)
+#define NS_PRODUCT(MODE, big, grid)                                   \
+    do {                                                              \
+        if (p.planes == 2) {                                          \
+            if (big) NS_LAUNCH(128, 2, 2, MODE, grid);                \
+            else NS_LAUNCH(64, 2, 4, MODE, grid);                     \
+        } else {                                                      \
+            if (big) NS_LAUNCH(128, 1, 2, MODE, grid);                \
+            else NS_LAUNCH(64, 1, 4, MODE, grid);                     \
+        }                                                             \
+        DVAE_LAUNCH_CHECK();                                          \
     } while (0)
         for (int t = 0; t < steps; ++t) {
             p.a = coefficients[3 * t]; p.b = coefficients[3 * t + 1]; p.c = coefficients[3 * t + 2];
-            place(tri0);
-            NS_PRODUCT(NS_GRAM, square);
-            NS_PRODUCT(NS_POLY, square);
-            place(upd0);
-            if (t + 1 < steps) NS_PRODUCT(NS_STEP, update);
-            else NS_PRODUCT(NS_LAST, update);
+            place(square0[sq]);
+            NS_PRODUCT(NS_GRAM, sq, square[sq]);
+            NS_PRODUCT(NS_POLY, sq, square[sq]);
+            place(update0[up]);
+            if (t + 1 < steps) NS_PRODUCT(NS_STEP, up, update[up]);
+            else NS_PRODUCT(NS_LAST, up, update[up]);
         }
 #undef NS_PRODUCT
+#undef NS_LAUNCH
     }
     return DVAE_OK;
 }

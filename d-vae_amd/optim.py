@@ -64,7 +64,7 @@ def orthogonalize(updates, steps=5, coefficients=QUINTIC, out=None):
             _lib.MatrixDesc(g.data_ptr(), o.data_ptr(), g.stride(0) if g.shape[0] > 1 else g.shape[1],
                             o.stride(0) if o.shape[0] > 1 else o.shape[1], g.shape[0], g.shape[1]) for g, o in zip(srcs, outs)])
         abc = (C.c_float * (3 * steps))(*[v for c in triples for v in c])
-        ws = _workspace(lib.dvae_orthogonalize_ws_bytes(descs, len(mats)), device, "dvae_orthogonalize_ws_bytes")
+        ws = _workspace(lib.dvae_orthogonalize_ws_bytes(descs, len(mats), code), device, "dvae_orthogonalize_ws_bytes")
         with _On(device) as stream:
             _lib.check(lib.dvae_orthogonalize(descs, len(mats), steps, abc, ws.data_ptr(), code, stream), "dvae_orthogonalize")
         if out is not None:

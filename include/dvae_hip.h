@@ -504,7 +504,7 @@ typedef struct dvae_matrix_desc {
     int64_t ld_g, ld_out;
     int32_t rows, cols;
 } dvae_matrix_desc;
-int64_t dvae_orthogonalize_ws_bytes(const dvae_matrix_desc* mats, int32_t count);
+int64_t dvae_orthogonalize_ws_bytes(const dvae_matrix_desc* mats, int32_t count, int32_t dtype);
 int dvae_orthogonalize(const dvae_matrix_desc* mats, int32_t count, int32_t steps, const float* coefficients, void* ws,
                        int32_t dtype, void* stream);
 
