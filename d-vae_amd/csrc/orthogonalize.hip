@@ -165,25 +165,27 @@ template <int PL> __global__ __launch_bounds__(256) void ns_split_kernel(NsGroup
 
 enum { NS_GRAM, NS_POLY, NS_STEP, NS_LAST };
 
-// One of the products, TB x TB output tiles, 4 waves as 2 x 2, each TB/2 x TB/2 of 32 x 32 MFMA blocks.  A stage of the K
+// One of the products, TB x TB output tiles; KG groups of waves, each with every KG-th stage of the sum; a group is 2 x WN
+// waves of TB/2 x TB/WN outputs, TM x TN MFMA blocks of 32 x 32.  A stage of the K
 // loop is one block (32 columns in two planes, 64 in one) of TB rows of either operand.  The loads run PF stages ahead in
 // registers and go to the other half of LDS in the middle of the stage before theirs.
-template <int TB, int PL, int PF, int MODE>
-__global__ __launch_bounds__(256) void ns_product_kernel(NsGroup p, int from, int first) {
-    constexpr int TM = TB / 64;
-    constexpr int PASSES = TB / 32;  // 16 bytes per thread and pass: 32 rows of one block
+template <int TB, int WN, int KG, int PL, int PF, int MODE>
+__global__ __launch_bounds__(128 * WN * KG) void ns_product_kernel(NsGroup p, int from, int first) {
+    constexpr int TM = TB / 64, TN = TB / WN / 32, NT = 128 * WN;
+    constexpr int LR = NT / 8, PASSES = TB / LR;  // 16 bytes per thread and pass: LR rows of one block
     constexpr int OPERAND = TB * NS_LDS_ROW;
-    constexpr int TP = TB + 4;       // row pitch of the output tile in LDS, floats
-    static_assert(PF % 2 == 0 && TB * TP * 4 <= 4 * OPERAND, "");
-    __shared__ __attribute__((aligned(16))) char lds[2][2 * OPERAND];
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    // workgroups that share an XCD (equal id mod 8) take neighbouring tiles
-    const int q = gridDim.x >> 3, rest = gridDim.x & 7, xcd = blockIdx.x & 7;
-    const int unit = (xcd < rest ? xcd * (q + 1) : rest * (q + 1) + (xcd - rest) * q) + (blockIdx.x >> 3);
-    const int k = ns_find(p, unit);
+    constexpr int TP = TB + 4;                    // row pitch of the output in LDS, floats; 64 rows at a time
+    static_assert(PF % 2 == 0 && 64 * TP * 4 <= 4 * OPERAND, "");
+    __shared__ __attribute__((aligned(16))) char lds[KG][2][2 * OPERAND];
+    const int group = __builtin_amdgcn_readfirstlane(threadIdx.x / NT), tid = threadIdx.x % NT;
+    const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int k = ns_find(p, blockIdx.x);
     const NsMat& m = p.mat[k];
     const int mp = ns_pad(m.m(), p.pad), np = ns_pad(m.n(), p.pad), mt = mp / TB, nt = np / TB;
-    const int t = unit - m.tile0;
+    // workgroups that share an XCD (equal id mod 8) take neighbouring tiles of a matrix
+    const int tiles = MODE == NS_GRAM || MODE == NS_POLY ? mt * (mt + 1) / 2 : mt * nt;
+    const int local = blockIdx.x - m.tile0, q = tiles >> 3, rest = tiles & 7, xcd = local & 7;
+    const int t = (xcd < rest ? xcd * (q + 1) : rest * (q + 1) + (xcd - rest) * q) + (local >> 3);
     int ti, tj;
     if (MODE == NS_GRAM || MODE == NS_POLY) {  // row by row of the upper triangle: row i begins at i mt - i (i - 1) / 2
         ti = (int)((2 * mt + 1 - sqrtf((float)((2 * mt + 1) * (2 * mt + 1) - 8 * t))) * 0.5f);
@@ -199,37 +201,53 @@ __global__ __launch_bounds__(256) void ns_product_kernel(NsGroup p, int from, in
     const long pitch = (long)(MODE == NS_GRAM ? np : mp) * 2 * PL;  // of both operands
     const char* a_rows = base + ns_offset(mp, np, PL, MODE == NS_GRAM ? from : MODE == NS_POLY ? 4 : 5) + (long)ti * TB * pitch;
     const char* b_rows = base + ns_offset(mp, np, PL, MODE == NS_GRAM ? from : MODE == NS_POLY ? 4 : from + 1) + (long)tj * TB * pitch;
-    const int stages = (int)(pitch / 128);
+    const int blocks = (int)(pitch / 128), stages = (blocks + KG - 1) / KG;
 
-    nsf32x16 acc[TM][TM];
+    const int col0 = tj * TB;
+    const bool mirror = MODE == NS_STEP || ((MODE == NS_GRAM || MODE == NS_POLY) && ti != tj);  // a diagonal tile is its own mirror
+    const char* src = base + ns_offset(mp, np, PL, MODE == NS_POLY ? 4 : from);
+    char* dst = base + ns_offset(mp, np, PL, MODE == NS_GRAM ? 4 : MODE == NS_POLY ? 5 : from ^ 2);
+    char* turned = base + ns_offset(mp, np, PL, MODE == NS_GRAM ? 4 : MODE == NS_POLY ? 5 : (from ^ 2) + 1);
+    const long row_bytes = (long)(MODE == NS_STEP || MODE == NS_LAST ? np : mp) * 2 * PL;
+    auto row_of = [&](int i, int row) { return ti * TB + (row >> 5) * (TB / 2) + i * 32 + (row & 31); };
+    // with one output per thread (the small products, where latency counts) the source is under way from the start
+    constexpr bool EARLY = MODE != NS_GRAM && TM == 1 && 64 * TB / 8 <= NT * KG;
+    h16x8 early_hi = {}, early_lo = {};
+    if (EARLY && threadIdx.x < 64 * TB / 8) {
+        const char* at = src + (long)row_of(0, threadIdx.x / (TB / 8)) * row_bytes + ns_col<PL>(col0 + threadIdx.x % (TB / 8) * 8);
+        early_hi = *(const h16x8*)at;
+        if (PL == 2) early_lo = *(const h16x8*)(at + 64);
+    }
+
+    nsf32x16 acc[TM][TN];
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
-        for (int j = 0; j < TM; ++j)
+        for (int j = 0; j < TN; ++j)
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
-    const int wm = wave >> 1, wn = wave & 1;
+    const int wm = wave / WN, wn = wave % WN;
     const long my = (long)(tid >> 3) * pitch + (tid & 7) * 16;
     const int my_lds = (tid >> 3) * NS_LDS_ROW + (tid & 7) * 16;
     nsu32x4 ra[PF][PASSES], rb[PF][PASSES];
-    auto load = [&](int u, int s) {  // past the last stage the last one is loaded again and not used
-        const long at = my + (long)min(s, stages - 1) * 128;
+    auto load = [&](int u, int s) {  // past the last block the last one is loaded again and not used
+        const long at = my + (long)min(s * KG + group, blocks - 1) * 128;
 #pragma unroll
         for (int i = 0; i < PASSES; ++i) {
-            ra[u][i] = *(const nsu32x4*)(a_rows + at + i * 32 * pitch);
-            rb[u][i] = *(const nsu32x4*)(b_rows + at + i * 32 * pitch);
+            ra[u][i] = *(const nsu32x4*)(a_rows + at + i * LR * pitch);
+            rb[u][i] = *(const nsu32x4*)(b_rows + at + i * LR * pitch);
         }
     };
     auto store = [&](int u, char* l) {
 #pragma unroll
         for (int i = 0; i < PASSES; ++i) {
-            *(nsu32x4*)(l + my_lds + i * 32 * NS_LDS_ROW) = ra[u][i];
-            *(nsu32x4*)(l + OPERAND + my_lds + i * 32 * NS_LDS_ROW) = rb[u][i];
+            *(nsu32x4*)(l + my_lds + i * LR * NS_LDS_ROW) = ra[u][i];
+            *(nsu32x4*)(l + OPERAND + my_lds + i * LR * NS_LDS_ROW) = rb[u][i];
         }
     };
 #pragma unroll
     for (int u = 0; u < PF; ++u) load(u, u);
-    store(0, lds[0]);
+    store(0, lds[group][0]);
     __syncthreads();
     // lane l of a fragment: row l & 31, columns 8 (l >> 5) .. + 7 of 16
     const int frag = (lane & 31) * NS_LDS_ROW + (lane >> 5) * 16;
@@ -239,33 +257,37 @@ __global__ __launch_bounds__(256) void ns_product_kernel(NsGroup p, int from, in
         for (int u = 0; u < PF; ++u) {
             const int s = s0 + u;
             if (s >= stages) break;
-            const char* la = lds[u & 1] + wm * (TB / 2) * NS_LDS_ROW + frag;
-            const char* lb = lds[u & 1] + OPERAND + wn * (TB / 2) * NS_LDS_ROW + frag;
+            const char* la = lds[group][u & 1] + wm * (TB / 2) * NS_LDS_ROW + frag;
+            const char* lb = lds[group][u & 1] + OPERAND + wn * (TB / WN) * NS_LDS_ROW + frag;
+            const bool mine = KG == 1 || s * KG + group < blocks;
 #pragma unroll
             for (int h = 0; h < SUB; ++h) {
-                h16x8 ah[TM], al[TM], bh[TM], bl[TM];
+                h16x8 ah[TM], al[TM], bh[TN], bl[TN];
 #pragma unroll
                 for (int i = 0; i < TM; ++i) {
                     ah[i] = *(const h16x8*)(la + i * 32 * NS_LDS_ROW + h * 32);
-                    bh[i] = *(const h16x8*)(lb + i * 32 * NS_LDS_ROW + h * 32);
-                    if (PL == 2) {
-                        al[i] = *(const h16x8*)(la + i * 32 * NS_LDS_ROW + h * 32 + 64);
-                        bl[i] = *(const h16x8*)(lb + i * 32 * NS_LDS_ROW + h * 32 + 64);
-                    }
+                    if (PL == 2) al[i] = *(const h16x8*)(la + i * 32 * NS_LDS_ROW + h * 32 + 64);
                 }
-                auto mma = [&](const h16x8 (&x)[TM], const h16x8 (&y)[TM]) {
+#pragma unroll
+                for (int j = 0; j < TN; ++j) {
+                    bh[j] = *(const h16x8*)(lb + j * 32 * NS_LDS_ROW + h * 32);
+                    if (PL == 2) bl[j] = *(const h16x8*)(lb + j * 32 * NS_LDS_ROW + h * 32 + 64);
+                }
+                auto mma = [&](const h16x8 (&x)[TM], const h16x8 (&y)[TN]) {
 #pragma unroll
                     for (int i = 0; i < TM; ++i)
 #pragma unroll
-                        for (int j = 0; j < TM; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[i], y[j], acc[i][j], 0, 0, 0);
+                        for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[i], y[j], acc[i][j], 0, 0, 0);
                 };
-                if (PL == 2) {
-                    mma(al, bh);
-                    mma(ah, bl);
+                if (mine) {
+                    if (PL == 2) {
+                        mma(al, bh);
+                        mma(ah, bl);
+                    }
+                    mma(ah, bh);
                 }
-                mma(ah, bh);
                 if (h == SUB / 2 - 1) {
-                    store((u + 1) % PF, lds[(u & 1) ^ 1]);
+                    store((u + 1) % PF, lds[group][(u & 1) ^ 1]);
                     __builtin_amdgcn_sched_barrier(0);
                     load(u, s + PF);
                     __builtin_amdgcn_sched_barrier(0);
@@ -275,73 +297,74 @@ __global__ __launch_bounds__(256) void ns_product_kernel(NsGroup p, int from, in
         }
     }
 
-    // Epilogue: the tile goes through LDS, so that every access to memory is 16 bytes of a row in either orientation.
+    // Epilogue: the output goes through LDS, one 32-row block of either wave row at a time, so that every access to memory
+    // is 16 bytes of a row in either orientation; the groups' sums meet there, in their order.
     // Lane l of an MFMA block holds column l & 31 and rows (r & 3) + 8 (r >> 2) + 4 (l >> 5).
     const float r = first ? p.r[k] : 1.f;
     const float from_src = MODE == NS_GRAM ? 0.f : (MODE == NS_POLY ? p.b * r * r * r : p.a * r) / NS_S;
     const float from_acc = (MODE == NS_POLY ? p.c * r * r * r * r * r : 1.f) / (NS_S * NS_S);
-    float* const tile = (float*)&lds[0][0];
+    float* const tile = (float*)&lds[0][0][0];
+    constexpr int GROUP_FLOATS = 4 * OPERAND / 4;
 #pragma unroll
-    for (int i = 0; i < TM; ++i)
+    for (int i = 0; i < TM; ++i) {
+        if (i > 0) __syncthreads();
 #pragma unroll
-        for (int j = 0; j < TM; ++j)
+        for (int j = 0; j < TN; ++j)
 #pragma unroll
             for (int e = 0; e < 16; ++e)
-                tile[(wm * (TB / 2) + i * 32 + (e & 3) + 8 * (e >> 2) + 4 * (lane >> 5)) * TP + wn * (TB / 2) + j * 32 + (lane & 31)] =
+                tile[group * GROUP_FLOATS + (wm * 32 + (e & 3) + 8 * (e >> 2) + 4 * (lane >> 5)) * TP + wn * (TB / WN) + j * 32 + (lane & 31)] =
                     acc[i][j][e] * from_acc;
-    __syncthreads();
-    const int row0 = ti * TB, col0 = tj * TB;
-    const bool mirror = MODE == NS_STEP || ((MODE == NS_GRAM || MODE == NS_POLY) && ti != tj);  // a diagonal tile is its own mirror
-    {
-        const char* src = base + ns_offset(mp, np, PL, MODE == NS_POLY ? 4 : from);
-        char* dst = base + ns_offset(mp, np, PL, MODE == NS_GRAM ? 4 : MODE == NS_POLY ? 5 : from ^ 2);
-        const long row_bytes = (long)(MODE == NS_STEP || MODE == NS_LAST ? np : mp) * 2 * PL;
-#pragma unroll
-        for (int u = tid; u < TB * TB / 8; u += 256) {
+        __syncthreads();
+        for (int u = threadIdx.x; u < 64 * TB / 8; u += NT * KG) {
             const int row = u / (TB / 8), c8 = u % (TB / 8) * 8;
-            const long at = (long)(row0 + row) * row_bytes + ns_col<PL>(col0 + c8);
+            const long at = (long)row_of(i, row) * row_bytes + ns_col<PL>(col0 + c8);
             float v[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = tile[row * TP + c8 + e];
-            if (MODE != NS_GRAM) {
-                const h16x8 hi = *(const h16x8*)(src + at);
-                h16x8 lo = {};
-                if (PL == 2) lo = *(const h16x8*)(src + at + 64);
+            for (int e = 0; e < 8; ++e) {
+                v[e] = tile[row * TP + c8 + e];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    v[e] = fmaf((float)hi[e] + (float)lo[e], from_src, v[e]);
-                    if (MODE == NS_LAST || mirror) tile[row * TP + c8 + e] = v[e];
-                }
+                for (int g = 1; g < KG; ++g) v[e] += tile[g * GROUP_FLOATS + row * TP + c8 + e];
             }
+            if (MODE != NS_GRAM) {
+                h16x8 hi = early_hi, lo = early_lo;
+                if (!EARLY) {
+                    hi = *(const h16x8*)(src + at);
+                    if (PL == 2) lo = *(const h16x8*)(src + at + 64);
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = fmaf((float)hi[e] + (float)lo[e], from_src, v[e]);
+            }
+            if ((MODE != NS_GRAM || KG > 1) && (MODE == NS_LAST || mirror))
+#pragma unroll
+                for (int e = 0; e < 8; ++e) tile[row * TP + c8 + e] = v[e];
             if (MODE != NS_LAST) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[e] *= NS_S;
                 ns_put8<PL>(dst + at, v);
             }
         }
-    }
-    if (MODE == NS_LAST) {
-        __syncthreads();
-        const bool wide = m.rows <= m.cols;  // else the rows of out are the columns of X
-        for (int u = tid; u < TB * TB; u += 256) {
-            const int row = wide ? u / TB : u % TB, col = wide ? u % TB : u / TB;
-            if (row0 + row >= m.m() || col0 + col >= m.n()) continue;
-            const float v = tile[row * TP + col];
-            const long o = wide ? (long)(row0 + row) * m.ld_out + col0 + col : (long)(col0 + col) * m.ld_out + row0 + row;
-            if (p.dtype == DVAE_F32) ((float*)m.out)[o] = v;
-            else if (p.dtype == DVAE_BF16) ((__bf16*)m.out)[o] = (__bf16)v;
-            else ((_Float16*)m.out)[o] = (_Float16)v;
-        }
-    } else if (mirror) {
-        if (MODE != NS_GRAM) __syncthreads();
-        char* dst = base + ns_offset(mp, np, PL, MODE == NS_GRAM ? 4 : MODE == NS_POLY ? 5 : (from ^ 2) + 1);
+        if (MODE == NS_LAST) {
+            __syncthreads();
+            const bool wide = m.rows <= m.cols;  // else the rows of out are the columns of X
+            for (int u = threadIdx.x; u < 64 * TB; u += NT * KG) {
+                const int row = wide ? u / TB : u % 64, c = wide ? u % TB : u / 64;
+                const int gr = row_of(i, row), gc = col0 + c;
+                if (gr >= m.m() || gc >= m.n()) continue;
+                const float v = tile[row * TP + c];
+                const long o = wide ? gr * m.ld_out + gc : gc * m.ld_out + gr;
+                if (p.dtype == DVAE_F32) ((float*)m.out)[o] = v;
+                else if (p.dtype == DVAE_BF16) ((__bf16*)m.out)[o] = (__bf16)v;
+                else ((_Float16*)m.out)[o] = (_Float16)v;
+            }
+        } else if (mirror) {
+            if (MODE != NS_GRAM || KG > 1) __syncthreads();
+            for (int u = threadIdx.x; u < 64 * TB / 8; u += NT * KG) {
+                const int c = u / 8, r8 = u % 8 * 8;
+                float v[8];
 #pragma unroll
-        for (int u = tid; u < TB * TB / 8; u += 256) {
-            const int col = u / (TB / 8), r8 = u % (TB / 8) * 8;
-            float v[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = tile[(r8 + e) * TP + col] * NS_S;
-            ns_put8<PL>(dst + (long)(col0 + col) * mp * 2 * PL + ns_col<PL>(row0 + r8), v);
+                for (int e = 0; e < 8; ++e) v[e] = tile[(r8 + e) * TP + c] * NS_S;
+                ns_put8<PL>(turned + (long)(col0 + c) * mp * 2 * PL + ns_col<PL>(row_of(i, r8)), v);
+            }
         }
     }
 }
@@ -357,11 +380,20 @@ static int ns_cus() {
 
 // A product runs on 128 x 128 tiles where those fill the chip one and a quarter times, else on 64 x 64.
 static bool ns_big(long tiles128) { return 4 * tiles128 >= 5L * ns_cus(); }
-// what the sides are padded to: to 64 where not even the update products, the ones with most tiles, use the larger tile
+// 256 x 256 tiles, one workgroup per CU, where the last round of them is nearly full.
+static bool ns_huge(long tiles256) {
+    const long rounds = (tiles256 + ns_cus() - 1) / ns_cus();
+    return 8 * tiles256 >= 7 * rounds * ns_cus();
+}
+// what the sides are padded to: the largest tile that any product takes; 256 only where that adds little to the work
 static int ns_pad_of(const dvae_matrix_desc* d, int32_t count) {
-    long tiles = 0;
-    for (int i = 0; i < count; ++i) tiles += (long)cdiv(d[i].rows, 128) * cdiv(d[i].cols, 128);
-    return ns_big(tiles) ? 128 : 64;
+    long big = 0, huge = 0;
+    for (int i = 0; i < count; ++i) {
+        big += (long)cdiv(d[i].rows, 128) * cdiv(d[i].cols, 128);
+        huge += (long)cdiv(d[i].rows, 256) * cdiv(d[i].cols, 256);
+    }
+    if (ns_huge(huge) && 32 * huge <= 9 * big) return 256;
+    return ns_big(big) ? 128 : 64;
 }
 static long ns_matrix_bytes(const dvae_matrix_desc& d, int pad, int planes) {
     const int mp = ns_pad(d.rows < d.cols ? d.rows : d.cols, pad), np = ns_pad(d.rows < d.cols ? d.cols : d.rows, pad);
@@ -392,7 +424,7 @@ extern "C" int64_t dvae_orthogonalize_ws_bytes(const dvae_matrix_desc* mats, int
     DVAE_TRY(ns_check("orthogonalize_ws_bytes", mats, count));
     int64_t most = 0;
     for (int g0 = 0; g0 < count; g0 += NS_GROUP) {  // the groups follow each other on the stream and share the space
-        const int n = count - g0 < NS_GROUP ? count - g0 : NS_GROUP, pad = ns_pad_of(mats + g0, n), planes = ns_planes(mats + g0, n, dtype);
+        const int n = count - g0 < NS_GROUP ? count - g0 : NS_GROUP, planes = ns_planes(mats + g0, n, dtype), pad = ns_pad_of(mats + g0, n);
         int64_t sum = NS_HEAD;
         for (int i = 0; i < n; ++i) sum += ns_matrix_bytes(mats[g0 + i], pad, planes);
         most = sum > most ? sum : most;
@@ -447,8 +479,8 @@ extern "C" int dvae_orthogonalize(const dvae_matrix_desc* mats, int32_t count, i
                 const int swap = order[j]; order[j] = order[j - 1]; order[j - 1] = swap;
             }
         long base = 0;
-        int split = 0, square[2] = {0, 0}, update[2] = {0, 0};  // tiles of all matrices; [0]: 64 x 64, [1]: 128 x 128
-        int split0[NS_GROUP], square0[2][NS_GROUP], update0[2][NS_GROUP];
+        int split = 0, square[3] = {}, update[3] = {};  // tiles of all matrices; [b]: of 64 << b
+        int split0[NS_GROUP], square0[3][NS_GROUP], update0[3][NS_GROUP];
         for (int i = 0; i < n; ++i) {
             const dvae_matrix_desc& d = mats[order[i]];
             NsMat& m = p.mat[i];
@@ -457,14 +489,15 @@ extern "C" int dvae_orthogonalize(const dvae_matrix_desc* mats, int32_t count, i
             const int mp = ns_pad(m.m(), p.pad), np = ns_pad(m.n(), p.pad);
             split0[i] = split;
             split += (mp / 64) * (np / 64);
-            for (int b = 0; b < 2; ++b) {
+            for (int b = 0; b < 3; ++b) {
                 const int mt = mp / (64 << b), nt = np / (64 << b);
                 square0[b][i] = square[b]; update0[b][i] = update[b];
                 square[b] += mt * (mt + 1) / 2;
                 update[b] += mt * nt;
             }
         }
-        const int sq = p.pad == 128 && ns_big(square[1]), up = p.pad == 128 && ns_big(update[1]);
+        auto size = [&](const int* tiles) { return p.pad == 256 && ns_huge(tiles[2]) ? 2 : p.pad >= 128 && ns_big(tiles[1]) ? 1 : 0; };
+        const int sq = size(square), up = size(update);
         auto place = [&](const int* at) { for (int i = 0; i < n; ++i) p.mat[i].tile0 = at[i]; };
         hipLaunchKernelGGL(ns_norm_kernel, dim3(NS_PARTS, n), dim3(256), 0, s, p);
         DVAE_LAUNCH_CHECK();
@@ -472,18 +505,22 @@ extern "C" int dvae_orthogonalize(const dvae_matrix_desc* mats, int32_t count, i
         if (p.planes == 2) hipLaunchKernelGGL((ns_split_kernel<2>), dim3(split), dim3(256), 0, s, p);
         else hipLaunchKernelGGL((ns_split_kernel<1>), dim3(split), dim3(256), 0, s, p);
         DVAE_LAUNCH_CHECK();
-#define NS_LAUNCH(TB, PL, PF, MODE, grid) \
-    hipLaunchKernelGGL((ns_product_kernel<TB, PL, PF, MODE>), dim3(grid), dim3(256), 0, s, p, 2 * (t & 1), t == 0)
-#define NS_PRODUCT(MODE, big, grid)                                   \
-    do {                                                              \
-        if (p.planes == 2) {                                          \
-            if (big) NS_LAUNCH(128, 2, 2, MODE, grid);                \
-            else NS_LAUNCH(64, 2, 4, MODE, grid);                     \
-        } else {                                                      \
-            if (big) NS_LAUNCH(128, 1, 2, MODE, grid);                \
-            else NS_LAUNCH(64, 1, 4, MODE, grid);                     \
-        }                                                             \
-        DVAE_LAUNCH_CHECK();                                          \
+#define NS_LAUNCH(TB, WN, KG, PL, PF, MODE, grid) \
+    hipLaunchKernelGGL((ns_product_kernel<TB, WN, KG, PL, PF, MODE>), dim3(grid), dim3(128 * WN * KG), 0, s, p, 2 * (t & 1), t == 0)
+#define NS_PRODUCT(MODE, size, grid)                                                      \
+    do {                                                                                  \
+        if (p.planes == 2) {                                                              \
+            if (size == 2) NS_LAUNCH(256, 4, 1, 2, 2, MODE, grid);                        \
+            else if (size == 1) NS_LAUNCH(128, 2, 1, 2, 2, MODE, grid);                   \
+            else if (grid <= ns_cus()) NS_LAUNCH(64, 2, 4, 2, 2, MODE, grid);             \
+            else NS_LAUNCH(64, 2, 1, 2, 4, MODE, grid);                                   \
+        } else {                                                                          \
+            if (size == 2) NS_LAUNCH(256, 4, 1, 1, 2, MODE, grid);                        \
+            else if (size == 1) NS_LAUNCH(128, 2, 1, 1, 2, MODE, grid);                   \
+            else if (grid <= ns_cus()) NS_LAUNCH(64, 2, 4, 1, 2, MODE, grid);             \
+            else NS_LAUNCH(64, 2, 1, 1, 4, MODE, grid);                                   \
+        }                                                                                 \
+        DVAE_LAUNCH_CHECK();                                                              \
     } while (0)
         for (int t = 0; t < steps; ++t) {
             p.a = coefficients[3 * t]; p.b = coefficients[3 * t + 1]; p.c = coefficients[3 * t + 2];
