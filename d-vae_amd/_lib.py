@@ -119,6 +119,8 @@ SIGNATURES = {
     "dvae_scan_step": (_I, [_P, _L, _P, _L, _P, _L, _L, _P, _I, _P, _I, _I, _I, _P]),
     "dvae_orthogonalize_ws_bytes": (_L, [C.POINTER(MatrixDesc), _I, _I]),
     "dvae_orthogonalize": (_I, [C.POINTER(MatrixDesc), _I, _I, C.POINTER(_F), _P, _I, _P]),
+    "dvae_muon_begin_f32": (_I, [_P] * 6 + [_L, _F, _I, _F, _F, _F, _F, _I, _I, _P]),
+    "dvae_muon_apply_f32": (_I, [_P, _P, _P, _L, _F, _F, _P]),
     "dvae_encode_ws_floats": (C.c_int64, [_MD, _BC]),
     "dvae_loss_ws_floats": (C.c_int64, [_MD, _BC]),
     "dvae_debug_side_stream": (_I, [_P, C.POINTER(_P)]),

@@ -61,7 +61,6 @@ __global__ __launch_bounds__(256) void adam_dev_kernel(float* __restrict__ p, fl
         P.f -= step_size * (M.f / denom);                     \
     }
         ADAM1(x) ADAM1(y) ADAM1(z) ADAM1(w)
-#undef ADAM1
         reinterpret_cast<float4*>(p)[i] = P;
         reinterpret_cast<float4*>(m)[i] = M;
         reinterpret_cast<float4*>(v)[i] = V;
@@ -69,6 +68,54 @@ __global__ __launch_bounds__(256) void adam_dev_kernel(float* __restrict__ p, fl
     }
 }
 __global__ void adam_advance_kernel(int* step_dev) { step_dev[0] += 1; }
+
+// The two elementwise passes of a Muon step over the same flat buffers, around dvae_orthogonalize.  `factor` holds one
+// float per 64 elements (parameters begin on multiples of 64): > 0 where they belong to a matrix, its learning-rate factor.
+//   begin:  matrices   m += (1 - mu) (g - m);  u = nesterov ? g + mu (m - g) : m      (u goes through dvae_orthogonalize)
+//           the rest   Adam, as above
+//   apply:  matrices   p = (1 - lr wd) p - lr factor u
+// HBM-bound: begin reads 2 and writes 2 floats per matrix element (Adam: 4 and 3), apply reads 2 and writes 1.
+__global__ __launch_bounds__(256) void muon_begin_kernel(float* __restrict__ p, float* __restrict__ g, float* __restrict__ m,
+                                                         float* __restrict__ v, float* __restrict__ u,
+                                                         const float* __restrict__ factor, long n4, float mu, int nesterov, float b1,
+                                                         float b2, float eps, float step_size, float inv_sqrt_bc2, int zero_grad) {
+    for (long i = blockIdx.x * (long)blockDim.x + threadIdx.x; i < n4; i += (long)gridDim.x * blockDim.x) {
+        const float4 G = reinterpret_cast<const float4*>(g)[i];
+        float4 M = reinterpret_cast<float4*>(m)[i];
+        if (factor[i >> 4] > 0.f) {
+            float4 U;
+#define MUON1(f)                                          \
+    M.f = M.f + (1.f - mu) * (G.f - M.f);                 \
+    U.f = nesterov ? G.f + mu * (M.f - G.f) : M.f;
+            MUON1(x) MUON1(y) MUON1(z) MUON1(w)
+#undef MUON1
+            reinterpret_cast<float4*>(u)[i] = U;
+        } else {
+            float4 P = reinterpret_cast<float4*>(p)[i], V = reinterpret_cast<float4*>(v)[i];
+            ADAM1(x) ADAM1(y) ADAM1(z) ADAM1(w)
+            reinterpret_cast<float4*>(p)[i] = P;
+            reinterpret_cast<float4*>(v)[i] = V;
+        }
+        reinterpret_cast<float4*>(m)[i] = M;
+        if (zero_grad) reinterpret_cast<float4*>(g)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+}
+#undef ADAM1
+__global__ __launch_bounds__(256) void muon_apply_kernel(float* __restrict__ p, const float* __restrict__ u,
+                                                         const float* __restrict__ factor, long n4, float lr, float keep) {
+    for (long i = blockIdx.x * (long)blockDim.x + threadIdx.x; i < n4; i += (long)gridDim.x * blockDim.x) {
+        const float f = factor[i >> 4];
+        if (f > 0.f) {
+            float4 P = reinterpret_cast<float4*>(p)[i];
+            const float4 U = reinterpret_cast<const float4*>(u)[i];
+            P.x = keep * P.x - lr * f * U.x;
+            P.y = keep * P.y - lr * f * U.y;
+            P.z = keep * P.z - lr * f * U.z;
+            P.w = keep * P.w - lr * f * U.w;
+            reinterpret_cast<float4*>(p)[i] = P;
+        }
+    }
+}
 
 }  // namespace dvae
 
@@ -108,6 +155,41 @@ extern "C" int dvae_adam_step_f32(float* p, float* g, float* m, float* v, int64_
     if (blocks > 2048) blocks = 2048;
     hipLaunchKernelGGL(adam_kernel, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, p, g, m, v, n4, beta1,
                        beta2, eps, step_size, inv_sqrt_bc2, zero_grad != 0);
+    DVAE_LAUNCH_CHECK();
+    return DVAE_OK;
+}
+
+static unsigned flat_blocks(long n4) {
+    const long blocks = (n4 + 255) / 256;
+    return (unsigned)(blocks > 2048 ? 2048 : blocks);
+}
+
+extern "C" int dvae_muon_begin_f32(float* p, float* g, float* m, float* v, float* u, const float* factor, int64_t n, float momentum,
+                                   int32_t nesterov, float adam_lr, float beta1, float beta2, float eps, int32_t step,
+                                   int32_t zero_grad, void* stream) {
+    using namespace dvae;
+    if (n == 0) return DVAE_OK;
+    DVAE_REQUIRE(p && g && m && v && u && factor, "muon_begin: null pointer");
+    DVAE_REQUIRE(n > 0 && n % 64 == 0, "muon_begin: the flat length must be a multiple of 64 floats");
+    DVAE_REQUIRE(((uintptr_t)p | (uintptr_t)g | (uintptr_t)m | (uintptr_t)v | (uintptr_t)u) % 16 == 0, "muon_begin: buffers must be 16-byte aligned");
+    DVAE_REQUIRE(step >= 1, "muon_begin: step counts from 1");
+    const double bc1 = 1.0 - pow((double)beta1, (double)step);
+    const double bc2 = 1.0 - pow((double)beta2, (double)step);
+    hipLaunchKernelGGL(muon_begin_kernel, dim3(flat_blocks(n / 4)), dim3(256), 0, (hipStream_t)stream, p, g, m, v, u, factor, (long)(n / 4),
+                       momentum, nesterov != 0, beta1, beta2, eps, (float)((double)adam_lr / bc1), (float)(1.0 / sqrt(bc2)),
+                       zero_grad != 0);
+    DVAE_LAUNCH_CHECK();
+    return DVAE_OK;
+}
+
+extern "C" int dvae_muon_apply_f32(float* p, const float* u, const float* factor, int64_t n, float lr, float weight_decay, void* stream) {
+    using namespace dvae;
+    if (n == 0) return DVAE_OK;
+    DVAE_REQUIRE(p && u && factor, "muon_apply: null pointer");
+    DVAE_REQUIRE(n > 0 && n % 64 == 0, "muon_apply: the flat length must be a multiple of 64 floats");
+    DVAE_REQUIRE(((uintptr_t)p | (uintptr_t)u) % 16 == 0, "muon_apply: buffers must be 16-byte aligned");
+    hipLaunchKernelGGL(muon_apply_kernel, dim3(flat_blocks(n / 4)), dim3(256), 0, (hipStream_t)stream, p, u, factor, (long)(n / 4), lr,
+                       1.f - lr * weight_decay);
     DVAE_LAUNCH_CHECK();
     return DVAE_OK;
 }

@@ -107,10 +107,7 @@ class FlatAdam(torch.optim.Optimizer):
         if self.extra is not None:
             self.extra.zero_grad()
 
-    @torch.no_grad()
-    def step(self, closure=None):
-        loss = closure() if closure is not None else None
-        g = self.param_groups[0]
+    def _check_views(self):
         r = self.reducer
         base_p, base_g = self.flat_p.data_ptr(), r.flat.data_ptr()
         for p, o in zip(r.params, r.offsets):
@@ -120,6 +117,13 @@ class FlatAdam(torch.optim.Optimizer):
                 raise _lib.DvaeHipError("FlatAdam: a parameter (or its .grad) no longer lives in the flat buffers "
                                         "(was the model moved or its gradients set to None after the optimizer "
                                         "was built?); build the optimizer after the last .to()")
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = closure() if closure is not None else None
+        g = self.param_groups[0]
+        r = self.reducer
+        self._check_views()
         lib = _lib.load()
         # zero_grad: with the gradient sink attached every write to the flat gradient buffer goes through the model
         # (which clears `reducer.clean`), so the kernel can leave the buffer zeroed and the next zero_grad() is free
@@ -260,3 +264,129 @@ class FlatAdam(torch.optim.Optimizer):
             g.update(saved)
         if self.extra is not None and sd.get("extra") is not None:
             self.extra.load_state_dict(sd["extra"])
+
+
+class FlatMuon(FlatAdam):
+    """Muon for the weight matrices, Adam for everything else, on FlatAdam's flat buffers: the momentum of a matrix is
+    orthogonalised (`orthogonalize`, all matrices of the model together) before it is applied.  The arguments are those of
+    torch.optim.Muon, whose counterpart this is:
+
+      m += (1 - momentum) (g - m);  u = g + momentum (m - g) if nesterov else m
+      p  = (1 - lr weight_decay) p - lr f orthogonalize(u),   f = sqrt(max(1, rows / columns))   ("original")
+                                                               or 0.2 sqrt(max(rows, columns))    ("match_rms_adamw")
+
+    matrices: names of the parameters that take this update; by default every weight matrix the train step touches except
+    those that act on one-hot inputs (*.weight_ih, and the gates and mappers of DVAE_BN: rows of a table) and the last layers
+    of the two predictors.  The rest, and `extra_params`, take Adam's with adam_lr, betas, eps.  param_groups[0] holds the
+    matrices (lr, momentum, nesterov, weight_decay), param_groups[1] the rest; schedulers see both."""
+
+    def __init__(self, model, lr=2e-2, momentum=0.95, nesterov=True, weight_decay=0.0, adam_lr=1e-4, betas=(0.9, 0.999),
+                 eps=1e-8, ns_steps=5, ns_coefficients=QUINTIC, adjust_lr_fn="original", matrices=None, reducer=None,
+                 extra_params=None):
+        if adjust_lr_fn not in ("original", "match_rms_adamw"):
+            raise ValueError("adjust_lr_fn must be 'original' or 'match_rms_adamw'")
+        if not 0.0 <= momentum < 1.0 or lr < 0.0 or weight_decay < 0.0:
+            raise ValueError("FlatMuon: momentum must lie in [0, 1), lr and weight_decay must not be negative")
+        super(FlatMuon, self).__init__(model, lr=adam_lr, betas=betas, eps=eps, reducer=reducer, extra_params=extra_params)
+        r = self.reducer
+        if matrices is None:
+            heads = ("add_vertex.2.weight", "add_edge.2.weight")
+            tables = ("gate_forward.0.weight", "gate_backward.0.weight", "mapper_forward.0.weight", "mapper_backward.0.weight")
+            matrices = [k for k, p in zip(r.names, r.params) if p.dim() == 2 and not k.endswith("weight_ih") and k not in heads
+                        and not (model._is_bn and k in tables)]
+        matrices = list(matrices)
+        at = dict(zip(r.names, range(len(r.names))))
+        for k in matrices:
+            if k not in at or r.params[at[k]].dim() != 2:
+                raise ValueError("FlatMuon: %s is not a weight matrix of the train step" % k)
+        self.matrices = [k for k in r.names if k in set(matrices)]
+        self.is_matrix = [k in set(matrices) for k in r.names]
+        self.ns_steps, self.ns_coefficients = int(ns_steps), ns_coefficients
+        rest = self.param_groups[0]
+        first = dict(rest, params=[p for p, mat in zip(r.params, self.is_matrix) if mat], lr=lr, momentum=momentum,
+                     nesterov=bool(nesterov), weight_decay=weight_decay)
+        del first["betas"], first["eps"]
+        rest["params"] = [p for p, mat in zip(r.params, self.is_matrix) if not mat]
+        self.param_groups[:] = [first, rest]
+        factor = torch.zeros(r.numel // 64, dtype=torch.float32)
+        for p, o, mat in zip(r.params, r.offsets, self.is_matrix):
+            if mat:
+                rows, cols = p.shape
+                f = max(1.0, rows / cols) ** 0.5 if adjust_lr_fn == "original" else 0.2 * max(rows, cols) ** 0.5
+                factor[o // 64:(o + p.numel() + 63) // 64] = f
+        self.factor = factor.to(self.flat_p.device)
+        self.flat_u = torch.zeros_like(self.flat_p)
+        self.updates = [self.flat_u[o:o + p.numel()].view_as(p) for p, o, mat in zip(r.params, r.offsets, self.is_matrix) if mat]
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = closure() if closure is not None else None
+        mats, rest = self.param_groups
+        r = self.reducer
+        self._check_views()
+        lib = _lib.load()
+        zero = int(bool(getattr(self.model, "_grad_sink", False)) and getattr(self.model, "_reducer", None) is r)
+        n = self.flat_p.numel()
+        self.steps += 1
+        with _On(self.flat_p.device) as stream:
+            _lib.check(lib.dvae_muon_begin_f32(self.flat_p.data_ptr(), r.flat.data_ptr(), self.exp_avg.data_ptr(),
+                                               self.exp_avg_sq.data_ptr(), self.flat_u.data_ptr(), self.factor.data_ptr(), n,
+                                               float(mats["momentum"]), int(mats["nesterov"]), float(rest["lr"]),
+                                               float(rest["betas"][0]), float(rest["betas"][1]), float(rest["eps"]), self.steps,
+                                               zero, stream), "dvae_muon_begin_f32")
+            if self.updates:
+                orthogonalize(self.updates, self.ns_steps, self.ns_coefficients, out=self.updates)
+                _lib.check(lib.dvae_muon_apply_f32(self.flat_p.data_ptr(), self.flat_u.data_ptr(), self.factor.data_ptr(), n,
+                                                   float(mats["lr"]), float(mats["weight_decay"]), stream), "dvae_muon_apply_f32")
+        r.clean = bool(zero)
+        self.model._pw_dirty = True  # written through raw pointers, as by FlatAdam
+        if self.extra is not None:
+            for eg in self.extra.param_groups:
+                eg["lr"] = rest["lr"]
+            self.extra.step()
+        return loss
+
+    # Checkpoints: {"state": {i: {"momentum_buffer"} or {"step", "exp_avg", "exp_avg_sq"}}, "param_groups": [matrices, rest]},
+    # i numbering model.parameters() as in FlatAdam's; the rest as torch.optim.Adam writes it, the matrices as torch.optim.Muon.
+    def _adam_part(self, call, *args):
+        """a FlatAdam method with the group of Adam's parameters as the only one"""
+        mats, rest = self.param_groups
+        self.param_groups[:] = [rest]
+        try:
+            return call(*args)
+        finally:
+            self.param_groups[:] = [mats, rest]
+
+    def _matrix_numbers(self):
+        number = {id(p): i for i, p in enumerate(self._ordered_params())}
+        return sorted(number[id(p)] for p in self.param_groups[0]["params"])
+
+    def state_dict(self):
+        sd = self._adam_part(super(FlatMuon, self).state_dict)
+        mats = self._matrix_numbers()
+        for i in mats:
+            if i in sd["state"]:
+                sd["state"][i] = {"momentum_buffer": sd["state"][i]["exp_avg"]}
+        adam = sd["param_groups"][0]
+        adam["params"] = [i for i in adam["params"] if i not in mats]
+        mine = {k: v for k, v in self.param_groups[0].items() if k != "params"}
+        sd["param_groups"] = [dict(mine, params=mats), adam]
+        sd["steps"] = self.steps
+        return sd
+
+    def load_state_dict(self, sd):
+        if len(sd.get("param_groups", ())) != 2 or "steps" not in sd:
+            raise ValueError("not a FlatMuon state dict (expected two parameter groups and the key 'steps')")
+        params, mats = self._ordered_params(), self._matrix_numbers()
+        if list(sd["param_groups"][0]["params"]) != mats:
+            raise ValueError("the state belongs to another choice of matrices")
+        state = {}
+        for i, st in sd["state"].items():
+            if int(i) in mats:
+                m = st["momentum_buffer"]
+                st = {"step": torch.tensor(float(sd["steps"])), "exp_avg": m, "exp_avg_sq": torch.zeros_like(m)}
+            state[int(i)] = st
+        adam = dict(sd["param_groups"][1], params=list(range(len(params))))
+        self._adam_part(super(FlatMuon, self).load_state_dict, {"state": state, "param_groups": [adam]})
+        self.param_groups[0].update({k: v for k, v in sd["param_groups"][0].items() if k != "params"})
+        self.steps = int(sd["steps"])

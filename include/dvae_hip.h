@@ -508,6 +508,17 @@ int64_t dvae_orthogonalize_ws_bytes(const dvae_matrix_desc* mats, int32_t count,
 int dvae_orthogonalize(const dvae_matrix_desc* mats, int32_t count, int32_t steps, const float* coefficients, void* ws,
                        int32_t dtype, void* stream);
 
+/* The elementwise passes of a Muon step around the call above, over flat fp32 buffers laid out alike (n % 64 == 0, parameters
+ * on multiples of 64 floats).  factor: n / 64 floats (device), for every 64 elements the learning-rate factor of the matrix
+ * they belong to, or 0 for parameters that take Adam's update.
+ *   dvae_muon_begin_f32   matrices: m += (1 - momentum) (g - m), u = nesterov ? g + momentum (m - g) : m;
+ *                         the rest: dvae_adam_step_f32's update (step counts from 1); zero_grad as there
+ *   dvae_muon_apply_f32   matrices: p = (1 - lr weight_decay) p - lr factor u */
+int dvae_muon_begin_f32(float* p, float* g, float* m, float* v, float* u, const float* factor, int64_t n, float momentum,
+                        int32_t nesterov, float adam_lr, float beta1, float beta2, float eps, int32_t step,
+                        int32_t zero_grad, void* stream);
+int dvae_muon_apply_f32(float* p, const float* u, const float* factor, int64_t n, float lr, float weight_decay, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -138,3 +138,129 @@ def test_orthogonalize_on_two_streams_at_once():
     torch.cuda.synchronize()
     for a, b in zip(want, got):
         assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+# --------------------------------------------------------------------------------------------------------------- FlatMuon
+
+def model_and_batch(bn=False, seed=0):
+    import numpy as np
+    torch.manual_seed(seed)
+    cls = dvae_amd.DVAE_BN if bn else dvae_amd.DVAE
+    model = cls(8, 8, 0, 1, hs=70, nz=16, bidirectional=True).cuda().train()
+    rng = np.random.default_rng(seed)
+    types = rng.integers(2, 8, (24, 8))
+    types[:, 0], types[:, -1] = 0, 1
+    adj = np.triu(rng.random((24, 8, 8)) < 0.4, 1)
+    adj[:, np.arange(7), np.arange(1, 8)] = True
+    ga = dvae_amd.GraphArrays.from_dense(types, adj, np.full(24, 8))
+    return model, ga
+
+
+def grads_of(model, ga, eps):
+    batch = model._collate_fn(ga)
+    mu, logvar = model.encode(batch)
+    loss = model.loss(mu, logvar, batch, eps=eps)[0]
+    loss.backward()
+    return loss
+
+
+@pytest.mark.parametrize("bn,nesterov,wd,fn", [(False, True, 0.0, "original"), (True, False, 0.1, "match_rms_adamw")])
+def test_flat_muon_steps_against_the_formulas(bn, nesterov, wd, fn):
+    model, ga = model_and_batch(bn)
+    opt = O.FlatMuon(model, lr=0.02, momentum=0.9, nesterov=nesterov, weight_decay=wd, adam_lr=1e-3, adjust_lr_fn=fn)
+    r = opt.reducer
+    assert opt.matrices and "grue_forward.weight_ih" not in opt.matrices and "add_edge.2.weight" not in opt.matrices
+    assert ("gate_forward.0.weight" in opt.matrices) == (not bn)
+    want = [p.detach().double().cpu().clone() for p in r.params]
+    mom = [torch.zeros_like(w) for w in want]
+    sq = [torch.zeros_like(w) for w in want]
+    slack = [0.0] * len(want)  # what the orthogonalisation may be off by, times the step
+    rounding = [0.0] * len(want)
+    g = gen(9)
+    for step in range(1, 4):
+        opt.zero_grad()
+        grads_of(model, ga, torch.randn(24, 16, generator=g))
+        grads = [p.grad.double().cpu().clone() for p in r.params]
+        opt.step()
+        for i, (name, d) in enumerate(zip(r.names, grads)):
+            if name in opt.matrices:
+                mom[i] += (1 - 0.9) * (d - mom[i])
+                u = d + 0.9 * (mom[i] - d) if nesterov else mom[i]
+                rows, cols = d.shape
+                f = max(1.0, rows / cols) ** 0.5 if fn == "original" else 0.2 * max(rows, cols) ** 0.5
+                o = plain(u)
+                want[i] = (1 - 0.02 * wd) * want[i] - 0.02 * f * o
+                # + 8 u for the momentum in fp32, amplified like the iteration's own errors
+                slack[i] += 0.02 * f * float(o.norm()) * 341 * (16 * 2.0 ** -22 + 8 * 2.0 ** -24)
+            else:
+                mom[i] += 0.1 * (d - mom[i])
+                sq[i] = 0.999 * sq[i] + 0.001 * d * d
+                want[i] = want[i] - 1e-3 / (1 - 0.9 ** step) * mom[i] / (sq[i].sqrt() / math.sqrt(1 - 0.999 ** step) + 1e-8)
+                slack[i] += 1e-3 * math.sqrt(d.numel()) * 64 * 2.0 ** -24  # a dozen roundings of an update of at most ~1
+            rounding[i] += 3 * 2.0 ** -24 * float(want[i].norm())
+        for i, p in enumerate(r.params):
+            assert float((p.detach().double().cpu() - want[i]).norm()) <= slack[i] + rounding[i], (step, r.names[i])
+    assert not r.flat.any()  # the gradients were left zeroed for the next step
+
+
+def test_flat_muon_checkpoint_continues_identically(tmp_path):
+    model, ga = model_and_batch()
+    opt = O.FlatMuon(model, lr=0.01, weight_decay=0.01)
+    g = gen(10)
+    eps = [torch.randn(24, 16, generator=g) for _ in range(4)]
+    for e in eps[:2]:
+        opt.zero_grad()
+        grads_of(model, ga, e)
+        opt.step()
+    dvae_amd.harness.save_checkpoint(str(tmp_path), 2, model, opt)
+    other, _ = model_and_batch(seed=5)
+    opt2 = O.FlatMuon(other, lr=0.5)
+    dvae_amd.harness.load_module_state(other, str(tmp_path / "model_checkpoint2.pth"))
+    dvae_amd.harness.load_module_state(opt2, str(tmp_path / "optimizer_checkpoint2.pth"))
+    assert opt2.steps == 2 and opt2.param_groups[0]["lr"] == 0.01 and opt2.param_groups[0]["weight_decay"] == 0.01
+    assert torch.equal(opt.exp_avg, opt2.exp_avg)
+    mats = torch.cat([torch.arange(o, o + p.numel()) for p, o, m in zip(opt.reducer.params, opt.reducer.offsets, opt.is_matrix) if not m])
+    assert torch.equal(opt.exp_avg_sq.cpu()[mats], opt2.exp_avg_sq.cpu()[mats])
+    for e in eps[2:]:
+        for m, o in ((model, opt), (other, opt2)):
+            o.zero_grad()
+            grads_of(m, ga, e)
+        opt2.reducer.flat.copy_(opt.reducer.flat)  # (the step's own gradients vary in the last bits: atomics)
+        opt.step(), opt2.step()
+    assert torch.equal(opt.flat_p, opt2.flat_p)
+    with pytest.raises(ValueError, match="FlatMuon state"):
+        opt.load_state_dict(O.FlatAdam(model_and_batch()[0]).state_dict())
+    with pytest.raises(ValueError, match="choice of matrices"):
+        opt.load_state_dict(O.FlatMuon(model_and_batch()[0], matrices=["fc3.weight"]).state_dict())
+
+
+def test_flat_muon_trains_an_epoch_with_a_scheduler():
+    import random
+    model, ga = model_and_batch()
+    opt = O.FlatMuon(model)
+    sched = torch.optim.lr_scheduler.ReduceLROnPlateau(opt, "min", factor=0.1, patience=10)
+    before = {k: p.detach().clone() for k, p in model.named_parameters()}
+    import numpy as np
+    for _ in range(2):
+        sums = dvae_amd.harness.train_epoch(model, opt, (ga, np.zeros(24)), batch_size=8, rng=random.Random(0))
+        assert all(math.isfinite(v) for v in sums)
+        sched.step(sums[0])
+    moved = {k for k, p in model.named_parameters() if not torch.equal(p, before[k])}
+    assert set(opt.reducer.names) == moved
+
+
+def test_flat_muon_refusals():
+    model, _ = model_and_batch()
+    for bad in (dict(adjust_lr_fn="none"), dict(momentum=1.0), dict(lr=-1.0), dict(matrices=["fc1.bias"]), dict(matrices=["nothing"])):
+        with pytest.raises(ValueError):
+            O.FlatMuon(model, **bad)
+    with pytest.raises(ValueError, match="capturable"):
+        dvae_amd.harness.GraphedTrainStep(model, O.FlatMuon(model))
+    m = torch.randn(8, 8).cuda()
+    for bad in ((m[0], {}), (m.double(), {}), ([m, m.half()], {}), (m[:0], {}), (m, dict(out=m[:4])), (m, dict(steps=0)), (m, dict(coefficients=(1.0, 2.0))),
+                ([m], dict(out=[])), (m, dict(out=m.t()[:, :4]))):
+        with pytest.raises((ValueError, dvae_amd._lib.DvaeHipError)):
+            O.orthogonalize(bad[0], **bad[1])
+    with pytest.raises(dvae_amd._lib.DvaeHipError, match="singular values leave"):
+        O.orthogonalize(m, coefficients=(4.0, 0.0, 0.0))
+    assert O.orthogonalize([]) == []

@@ -64,3 +64,35 @@ def test_workspace_sizes_grow_with_the_work():
     assert lib.dvae_scan_state_floats(0, 8) == 0 and lib.dvae_scan_state_floats(1, 8) == 8
     assert lib.dvae_scan_state_floats(1 << 39, 8) > 1 << 32  # 64 bits all the way
     assert lib.dvae_embed_bwd_ws_bytes(1 << 20, 1 << 20, 1 << 12) > 1 << 30
+
+
+def test_matrix_descriptions_are_checked_before_any_launch():
+    def desc(g=4096, out=4096, ld_g=8, ld_out=8, rows=8, cols=8):
+        return (L.MatrixDesc * 1)(L.MatrixDesc(g, out, ld_g, ld_out, rows, cols))
+    abc = (C.c_float * 15)(*[3.4445, -4.7750, 2.0315] * 5)
+    p = C.c_void_p(4096)
+    assert "null" in rc("dvae_orthogonalize", None, 1, 5, abc, p, 0, None)
+    assert "element type" in rc("dvae_orthogonalize", desc(), 1, 5, abc, p, 5, None)
+    assert "steps" in rc("dvae_orthogonalize", desc(), 1, 0, abc, p, 0, None)
+    assert "sides" in rc("dvae_orthogonalize", desc(rows=0), 1, 5, abc, p, 0, None)
+    assert "sides" in rc("dvae_orthogonalize_ws_bytes", desc(cols=40000), 1, 0)
+    assert "row stride" in rc("dvae_orthogonalize", desc(ld_g=7), 1, 5, abc, p, 0, None)
+    assert "null" in rc("dvae_orthogonalize", desc(out=None), 1, 5, abc, p, 0, None)
+    assert "aligned" in rc("dvae_orthogonalize", desc(), 1, 5, abc, C.c_void_p(4097), 0, None)
+    assert "singular" in rc("dvae_orthogonalize", desc(), 1, 5, (C.c_float * 15)(*[4.0, 0.0, 0.0] * 5), p, 0, None)
+    assert "64" in rc("dvae_muon_begin_f32", p, p, p, p, p, p, 100, 0.9, 1, 1e-3, 0.9, 0.999, 1e-8, 1, 0, None)
+    assert "step" in rc("dvae_muon_begin_f32", p, p, p, p, p, p, 128, 0.9, 1, 1e-3, 0.9, 0.999, 1e-8, 0, 0, None)
+    assert "null" in rc("dvae_muon_apply_f32", p, None, p, 128, 0.1, 0.0, None)
+
+
+def test_the_matrix_description_has_the_header_layout(tmp_path):
+    import os
+    import subprocess
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    src = tmp_path / "layout.c"
+    names = [f for f, _ in L.MatrixDesc._fields_]
+    src.write_text("#include <stdio.h>\n#include <stddef.h>\n#include \"dvae_hip.h\"\nint main(void) { printf(\"%zu\", sizeof(dvae_matrix_desc));\n"
+                   + "".join('printf(" %%zu", offsetof(dvae_matrix_desc, %s));\n' % f for f in names) + "return 0; }\n")
+    subprocess.run(["gcc", "-std=c99", "-Wall", "-Werror", "-I", os.path.join(root, "include"), str(src), "-o", str(tmp_path / "layout")], check=True)
+    out = subprocess.run([str(tmp_path / "layout")], check=True, capture_output=True, text=True).stdout.split()
+    assert [int(v) for v in out] == [C.sizeof(L.MatrixDesc)] + [getattr(L.MatrixDesc, f).offset for f in names]
