@@ -165,6 +165,21 @@ template <int PL> __global__ __launch_bounds__(256) void ns_split_kernel(NsGroup
 
 enum { NS_GRAM, NS_POLY, NS_STEP, NS_LAST };
 
+// Tile t of mt x nt: the two symmetric products have those on and above the diagonal, row by row (row i begins at
+// i mt - i (i - 1) / 2); the others go through bands of 8 tile rows column by column.
+template <int MODE> __device__ __forceinline__ void ns_tile_at(int t, int mt, int nt, int& ti, int& tj) {
+    if (MODE == NS_GRAM || MODE == NS_POLY) {
+        ti = (int)((2 * mt + 1 - sqrtf((float)((2 * mt + 1) * (2 * mt + 1) - 8 * t))) * 0.5f);
+        while (ti > 0 && ti * mt - ti * (ti - 1) / 2 > t) --ti;
+        while ((ti + 1) * mt - (ti + 1) * ti / 2 <= t) ++ti;
+        tj = ti + t - (ti * mt - ti * (ti - 1) / 2);
+    } else {
+        const int band = t / (8 * nt), in = t % (8 * nt), rows = min(8, mt - band * 8);
+        ti = band * 8 + in % rows;
+        tj = in / rows;
+    }
+}
+
 // One of the products, TB x TB output tiles; KG groups of waves, each with every KG-th stage of the sum; a group is 2 x WN
 // waves of TB/2 x TB/WN outputs, TM x TN MFMA blocks of 32 x 32.  A stage of the K
 // loop is one block (32 columns in two planes, 64 in one) of TB rows of either operand.  The loads run PF stages ahead in
@@ -187,16 +202,7 @@ __global__ __launch_bounds__(128 * WN * KG) void ns_product_kernel(NsGroup p, in
     const int local = blockIdx.x - m.tile0, q = tiles >> 3, rest = tiles & 7, xcd = local & 7;
     const int t = (xcd < rest ? xcd * (q + 1) : rest * (q + 1) + (xcd - rest) * q) + (local >> 3);
     int ti, tj;
-    if (MODE == NS_GRAM || MODE == NS_POLY) {  // row by row of the upper triangle: row i begins at i mt - i (i - 1) / 2
-        ti = (int)((2 * mt + 1 - sqrtf((float)((2 * mt + 1) * (2 * mt + 1) - 8 * t))) * 0.5f);
-        while (ti > 0 && ti * mt - ti * (ti - 1) / 2 > t) --ti;
-        while ((ti + 1) * mt - (ti + 1) * ti / 2 <= t) ++ti;
-        tj = ti + t - (ti * mt - ti * (ti - 1) / 2);
-    } else {  // bands of 8 tile rows, column by column
-        const int band = t / (8 * nt), in = t % (8 * nt), rows = min(8, mt - band * 8);
-        ti = band * 8 + in % rows;
-        tj = in / rows;
-    }
+    ns_tile_at<MODE>(t, mt, nt, ti, tj);
     char* const base = p.ws + m.base;
     const long pitch = (long)(MODE == NS_GRAM ? np : mp) * 2 * PL;  // of both operands
     const char* a_rows = base + ns_offset(mp, np, PL, MODE == NS_GRAM ? from : MODE == NS_POLY ? 4 : 5) + (long)ti * TB * pitch;
@@ -369,6 +375,109 @@ __global__ __launch_bounds__(128 * WN * KG) void ns_product_kernel(NsGroup p, in
     }
 }
 
+// The same products where they are small and their latency counts: 32 x 32 output tiles, one MFMA block each, the eight waves
+// of a workgroup take every eighth block of the sum.  Fragments come straight from memory (a lane's 16 bytes are 16 bytes of a
+// row), two blocks in flight per wave; no LDS and no barrier until the waves' sums meet.
+template <int PL, int MODE>
+__global__ __launch_bounds__(512) void ns_small_kernel(NsGroup p, int from, int first) {
+    constexpr int W = 8, TP = 36;
+    __shared__ __attribute__((aligned(16))) float part[W][32 * TP];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int k = ns_find(p, blockIdx.x);
+    const NsMat& m = p.mat[k];
+    const int mp = ns_pad(m.m(), p.pad), np = ns_pad(m.n(), p.pad);
+    int ti, tj;
+    ns_tile_at<MODE>(blockIdx.x - m.tile0, mp / 32, np / 32, ti, tj);
+    char* const base = p.ws + m.base;
+    const long pitch = (long)(MODE == NS_GRAM ? np : mp) * 2 * PL;
+    const char* a_rows = base + ns_offset(mp, np, PL, MODE == NS_GRAM ? from : MODE == NS_POLY ? 4 : 5);
+    const char* b_rows = base + ns_offset(mp, np, PL, MODE == NS_GRAM ? from : MODE == NS_POLY ? 4 : from + 1);
+    a_rows += (long)(ti * 32 + (lane & 31)) * pitch + (lane >> 5) * 16;
+    b_rows += (long)(tj * 32 + (lane & 31)) * pitch + (lane >> 5) * 16;
+    const int blocks = (int)(pitch / 128);
+    // the source of the added multiple is under way from the start: thread u < 128 has row u / 4, columns 8 (u % 4) ..
+    const int row = (threadIdx.x >> 2) & 31, c8 = (threadIdx.x & 3) * 8;
+    const long row_bytes = (long)(MODE == NS_STEP || MODE == NS_LAST ? np : mp) * 2 * PL;
+    const long at = (long)(ti * 32 + row) * row_bytes + ns_col<PL>(tj * 32 + c8);
+    h16x8 src_hi = {}, src_lo = {};
+    if (MODE != NS_GRAM && threadIdx.x < 128) {
+        const char* src = base + ns_offset(mp, np, PL, MODE == NS_POLY ? 4 : from) + at;
+        src_hi = *(const h16x8*)src;
+        if (PL == 2) src_lo = *(const h16x8*)(src + 64);
+    }
+    nsf32x16 acc, cross;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[e] = cross[e] = 0.f;
+    for (int s0 = wave; s0 < blocks; s0 += 2 * W) {
+        h16x8 a[2][4], b[2][4];
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {  // two planes: hi hi lo lo; one plane: four 16-column steps
+                const long o = (long)min(s0 + n * W, blocks - 1) * 128 + h * 32;
+                a[n][h] = *(const h16x8*)(a_rows + o);
+                b[n][h] = *(const h16x8*)(b_rows + o);
+            }
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            if (s0 + n * W >= blocks) break;
+            if (PL == 2) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    cross = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[n][h + 2], b[n][h], cross, 0, 0, 0);
+                    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[n][h], b[n][h], acc, 0, 0, 0);
+                    cross = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[n][h], b[n][h + 2], cross, 0, 0, 0);
+                }
+            } else {
+#pragma unroll
+                for (int h = 0; h < 4; ++h) acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[n][h], b[n][h], acc, 0, 0, 0);
+            }
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 16; ++e) part[wave][((e & 3) + 8 * (e >> 2) + 4 * (lane >> 5)) * TP + (lane & 31)] = acc[e] + cross[e];
+    __syncthreads();
+    const float r = first ? p.r[k] : 1.f;
+    const float from_src = MODE == NS_GRAM ? 0.f : (MODE == NS_POLY ? p.b * r * r * r : p.a * r) / NS_S;
+    const float from_acc = (MODE == NS_POLY ? p.c * r * r * r * r * r : 1.f) / (NS_S * NS_S);
+    const bool mirror = MODE == NS_STEP || ((MODE == NS_GRAM || MODE == NS_POLY) && ti != tj);
+    if (threadIdx.x < 128) {
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            float t = 0.f;
+#pragma unroll
+            for (int w = 0; w < W; ++w) t += part[w][row * TP + c8 + e];
+            v[e] = fmaf((float)src_hi[e] + (float)src_lo[e], from_src, t * from_acc);
+            part[0][row * TP + c8 + e] = v[e];
+        }
+        if (MODE != NS_LAST) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] *= NS_S;
+            ns_put8<PL>(base + ns_offset(mp, np, PL, MODE == NS_GRAM ? 4 : MODE == NS_POLY ? 5 : from ^ 2) + at, v);
+        }
+    }
+    __syncthreads();
+    if (MODE == NS_LAST) {
+        const bool wide = m.rows <= m.cols;
+        for (int u = threadIdx.x; u < 1024; u += 512) {
+            const int i = wide ? u >> 5 : u & 31, j = wide ? u & 31 : u >> 5, gr = ti * 32 + i, gc = tj * 32 + j;
+            if (gr >= m.m() || gc >= m.n()) continue;
+            const float v = part[0][i * TP + j];
+            const long o = wide ? gr * m.ld_out + gc : gc * m.ld_out + gr;
+            if (p.dtype == DVAE_F32) ((float*)m.out)[o] = v;
+            else if (p.dtype == DVAE_BF16) ((__bf16*)m.out)[o] = (__bf16)v;
+            else ((_Float16*)m.out)[o] = (_Float16)v;
+        }
+    } else if (mirror && threadIdx.x < 128) {
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = part[0][(c8 + e) * TP + row] * NS_S;  // here `row` is a column of the tile, c8 its rows
+        ns_put8<PL>(base + ns_offset(mp, np, PL, MODE == NS_GRAM ? 4 : MODE == NS_POLY ? 5 : (from ^ 2) + 1) +
+                        (long)(tj * 32 + row) * mp * 2 * PL + ns_col<PL>(ti * 32 + c8), v);
+    }
+}
+
 static int ns_cus() {
     static const int cus = [] {
         int dev = 0, n = 0;
@@ -479,8 +588,8 @@ extern "C" int dvae_orthogonalize(const dvae_matrix_desc* mats, int32_t count, i
                 const int swap = order[j]; order[j] = order[j - 1]; order[j - 1] = swap;
             }
         long base = 0;
-        int split = 0, square[3] = {}, update[3] = {};  // tiles of all matrices; [b]: of 64 << b
-        int split0[NS_GROUP], square0[3][NS_GROUP], update0[3][NS_GROUP];
+        int split = 0, square[4] = {}, update[4] = {};  // tiles of all matrices; [b]: of 32 << b
+        int split0[NS_GROUP], square0[4][NS_GROUP], update0[4][NS_GROUP];
         for (int i = 0; i < n; ++i) {
             const dvae_matrix_desc& d = mats[order[i]];
             NsMat& m = p.mat[i];
@@ -489,14 +598,16 @@ extern "C" int dvae_orthogonalize(const dvae_matrix_desc* mats, int32_t count, i
             const int mp = ns_pad(m.m(), p.pad), np = ns_pad(m.n(), p.pad);
             split0[i] = split;
             split += (mp / 64) * (np / 64);
-            for (int b = 0; b < 3; ++b) {
-                const int mt = mp / (64 << b), nt = np / (64 << b);
+            for (int b = 0; b < 4; ++b) {
+                const int mt = mp / (32 << b), nt = np / (32 << b);
                 square0[b][i] = square[b]; update0[b][i] = update[b];
                 square[b] += mt * (mt + 1) / 2;
                 update[b] += mt * nt;
             }
         }
-        auto size = [&](const int* tiles) { return p.pad == 256 && ns_huge(tiles[2]) ? 2 : p.pad >= 128 && ns_big(tiles[1]) ? 1 : 0; };
+        auto size = [&](const int* tiles) {
+            return p.pad == 256 && ns_huge(tiles[3]) ? 3 : p.pad >= 128 && ns_big(tiles[2]) ? 2 : tiles[0] <= ns_cus() ? 0 : 1;
+        };
         const int sq = size(square), up = size(update);
         auto place = [&](const int* at) { for (int i = 0; i < n; ++i) p.mat[i].tile0 = at[i]; };
         hipLaunchKernelGGL(ns_norm_kernel, dim3(NS_PARTS, n), dim3(256), 0, s, p);
@@ -507,16 +618,19 @@ extern "C" int dvae_orthogonalize(const dvae_matrix_desc* mats, int32_t count, i
         DVAE_LAUNCH_CHECK();
 #define NS_LAUNCH(TB, WN, KG, PL, PF, MODE, grid) \
     hipLaunchKernelGGL((ns_product_kernel<TB, WN, KG, PL, PF, MODE>), dim3(grid), dim3(128 * WN * KG), 0, s, p, 2 * (t & 1), t == 0)
+#define NS_SMALL(PL, MODE, grid) hipLaunchKernelGGL((ns_small_kernel<PL, MODE>), dim3(grid), dim3(512), 0, s, p, 2 * (t & 1), t == 0)
 #define NS_PRODUCT(MODE, size, grid)                                                      \
     do {                                                                                  \
         if (p.planes == 2) {                                                              \
-            if (size == 2) NS_LAUNCH(256, 4, 1, 2, 2, MODE, grid);                        \
-            else if (size == 1) NS_LAUNCH(128, 2, 1, 2, 2, MODE, grid);                   \
+            if (size == 3) NS_LAUNCH(256, 4, 1, 2, 2, MODE, grid);                        \
+            else if (size == 2) NS_LAUNCH(128, 2, 1, 2, 2, MODE, grid);                   \
+            else if (size == 0) NS_SMALL(2, MODE, grid);                                  \
             else if (grid <= ns_cus()) NS_LAUNCH(64, 2, 4, 2, 2, MODE, grid);             \
             else NS_LAUNCH(64, 2, 1, 2, 4, MODE, grid);                                   \
         } else {                                                                          \
-            if (size == 2) NS_LAUNCH(256, 4, 1, 1, 2, MODE, grid);                        \
-            else if (size == 1) NS_LAUNCH(128, 2, 1, 1, 2, MODE, grid);                   \
+            if (size == 3) NS_LAUNCH(256, 4, 1, 1, 2, MODE, grid);                        \
+            else if (size == 2) NS_LAUNCH(128, 2, 1, 1, 2, MODE, grid);                   \
+            else if (size == 0) NS_SMALL(1, MODE, grid);                                  \
             else if (grid <= ns_cus()) NS_LAUNCH(64, 2, 4, 1, 2, MODE, grid);             \
             else NS_LAUNCH(64, 2, 1, 1, 4, MODE, grid);                                   \
         }                                                                                 \
@@ -533,6 +647,7 @@ extern "C" int dvae_orthogonalize(const dvae_matrix_desc* mats, int32_t count, i
         }
 #undef NS_PRODUCT
 #undef NS_LAUNCH
+#undef NS_SMALL
     }
     return DVAE_OK;
 }

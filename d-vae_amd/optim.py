@@ -13,7 +13,7 @@ import torch
 
 from . import _lib
 from .dist import GradSumReducer
-from .sequence import _matrix, _On, _workspace
+from .sequence import _enqueue, _matrix, _workspace
 
 
 QUINTIC = (3.4445, -4.7750, 2.0315)  # p(s) = a s + b s^3 + c s^5: five steps take singular values from 0.002 up to 0.7 .. 1.2
@@ -65,8 +65,7 @@ def orthogonalize(updates, steps=5, coefficients=QUINTIC, out=None):
                             o.stride(0) if o.shape[0] > 1 else o.shape[1], g.shape[0], g.shape[1]) for g, o in zip(srcs, outs)])
         abc = (C.c_float * (3 * steps))(*[v for c in triples for v in c])
         ws = _workspace(lib.dvae_orthogonalize_ws_bytes(descs, len(mats), code), device, "dvae_orthogonalize_ws_bytes")
-        with _On(device) as stream:
-            _lib.check(lib.dvae_orthogonalize(descs, len(mats), steps, abc, ws.data_ptr(), code, stream), "dvae_orthogonalize")
+        _enqueue(device, "dvae_orthogonalize", descs, len(mats), steps, abc, ws.data_ptr(), code)
         if out is not None:
             torch.autograd.graph.increment_version(outs)
     return outs[0] if one else outs
@@ -324,20 +323,18 @@ class FlatMuon(FlatAdam):
         mats, rest = self.param_groups
         r = self.reducer
         self._check_views()
-        lib = _lib.load()
         zero = int(bool(getattr(self.model, "_grad_sink", False)) and getattr(self.model, "_reducer", None) is r)
         n = self.flat_p.numel()
         self.steps += 1
-        with _On(self.flat_p.device) as stream:
-            _lib.check(lib.dvae_muon_begin_f32(self.flat_p.data_ptr(), r.flat.data_ptr(), self.exp_avg.data_ptr(),
-                                               self.exp_avg_sq.data_ptr(), self.flat_u.data_ptr(), self.factor.data_ptr(), n,
-                                               float(mats["momentum"]), int(mats["nesterov"]), float(rest["lr"]),
-                                               float(rest["betas"][0]), float(rest["betas"][1]), float(rest["eps"]), self.steps,
-                                               zero, stream), "dvae_muon_begin_f32")
-            if self.updates:
-                orthogonalize(self.updates, self.ns_steps, self.ns_coefficients, out=self.updates)
-                _lib.check(lib.dvae_muon_apply_f32(self.flat_p.data_ptr(), self.flat_u.data_ptr(), self.factor.data_ptr(), n,
-                                                   float(mats["lr"]), float(mats["weight_decay"]), stream), "dvae_muon_apply_f32")
+        dev = self.flat_p.device
+        _enqueue(dev, "dvae_muon_begin_f32", self.flat_p.data_ptr(), r.flat.data_ptr(), self.exp_avg.data_ptr(),
+                 self.exp_avg_sq.data_ptr(), self.flat_u.data_ptr(), self.factor.data_ptr(), n, float(mats["momentum"]),
+                 int(mats["nesterov"]), float(rest["lr"]), float(rest["betas"][0]), float(rest["betas"][1]), float(rest["eps"]),
+                 self.steps, zero)
+        if self.updates:
+            orthogonalize(self.updates, self.ns_steps, self.ns_coefficients, out=self.updates)
+            _enqueue(dev, "dvae_muon_apply_f32", self.flat_p.data_ptr(), self.flat_u.data_ptr(), self.factor.data_ptr(), n,
+                     float(mats["lr"]), float(mats["weight_decay"]))
         r.clean = bool(zero)
         self.model._pw_dirty = True  # written through raw pointers, as by FlatAdam
         if self.extra is not None:

@@ -16,31 +16,38 @@ from . import _lib
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # DVAE_F32, DVAE_BF16, DVAE_F16
 
 
-def _need(cond, text):
-    if not cond:
-        raise ValueError(text)
-
-
 def _matrix(t, name, dims):
     """a floating-point matrix (or batch of them) on a HIP device; returns the element type code of the C-ABI"""
-    _need(torch.is_tensor(t) and t.dim() == dims, "%s must be a tensor with %d dimensions" % (name, dims))
-    _need(t.dtype in DTYPES, "%s must be float32, bfloat16 or float16, not %s" % (name, t.dtype))
+    if not torch.is_tensor(t) or t.dim() != dims:
+        raise ValueError("%s must be a tensor with %d dimensions" % (name, dims))
+    code = DTYPES.get(t.dtype)
+    if code is None:
+        raise ValueError("%s must be float32, bfloat16 or float16, not %s" % (name, t.dtype))
     if not t.is_cuda:
         raise _lib.DvaeHipError("%s is on %s; the operator only runs on a HIP device. There is no CPU fallback." % (name, t.device))
-    return DTYPES[t.dtype]
+    return code
 
 
 def _index(t, name, device):
-    _need(torch.is_tensor(t) and t.dtype in (torch.int32, torch.int64), "%s must be an int32 or int64 tensor" % name)
-    _need(t.device == device, "%s is on %s, the matrices on %s" % (name, t.device, device))
+    """an index tensor beside the matrices; (contiguous, is it int64)"""
+    if not torch.is_tensor(t) or t.dtype not in (torch.int32, torch.int64):
+        raise ValueError("%s must be an int32 or int64 tensor" % name)
+    if t.device != device:
+        raise ValueError("%s is on %s, the matrices on %s" % (name, t.device, device))
     return t.contiguous()
+
+
+def _wide(t):
+    return 1 if t is not None and t.dtype == torch.int64 else 0
 
 
 def _rows(t):
     """(t, row stride) of a [N, D] matrix whose elements lie side by side in a row; other layouts are copied"""
-    if t.shape[1] > 1 and t.stride(1) != 1 or t.shape[0] > 1 and 0 < t.stride(0) < t.shape[1]:
-        t = t.contiguous()
-    return t, t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    n, d = t.shape
+    s0, s1 = t.stride()
+    if d > 1 and s1 != 1 or n > 1 and 0 < s0 < d:
+        return t.contiguous(), d
+    return t, s0 if n > 1 else d
 
 
 def _flat_rows(t):
@@ -55,23 +62,17 @@ def _flat_rows(t):
     return _rows(t.reshape(B * T, D))
 
 
-class _On(object):
-    """the device of the operands as the current one while the library enqueues on its current stream"""
-
-    def __init__(self, device):
-        self.index = device.index
-        self.guard = None
-
-    def __enter__(self):
-        if self.index != torch.cuda.current_device():
-            self.guard = torch.cuda.device(self.index)
-            self.guard.__enter__()
-        return torch._C._cuda_getCurrentRawStream(self.index)
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
-        return False
+def _enqueue(device, name, *args):
+    """calls the library's function `name` with the current stream of `device`, that device being the current one"""
+    fn = getattr(_lib.load(), name)
+    index = device.index
+    if index == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc != 0:
+        _lib.check(rc, name)
 
 
 def _workspace(n_bytes, device, what):
@@ -80,35 +81,39 @@ def _workspace(n_bytes, device, what):
     return torch.empty(n_bytes, dtype=torch.uint8, device=device)
 
 
+def _once(name):
+    if torch.is_grad_enabled():  # create_graph=True: the backward pass itself is not recorded
+        raise RuntimeError("%s: the gradient is not differentiable again" % name)
+
+
 # ------------------------------------------------------------------------------------------------------------------ embed
+
+def _embed_forward(weight, ids, scale):
+    V, D = weight.shape
+    out = torch.empty(ids.shape + (D,), dtype=weight.dtype, device=weight.device)
+    _enqueue(weight.device, "dvae_embed_fwd", weight.data_ptr(), weight.stride(0) if V > 1 else D, ids.data_ptr(), _wide(ids),
+             out.data_ptr(), ids.numel(), V, D, scale, DTYPES[weight.dtype])
+    return out
+
 
 class _EmbedFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, weight, ids, scale):
-        lib = _lib.load()
-        V, D = weight.shape
-        out = torch.empty(tuple(ids.shape) + (D,), dtype=weight.dtype, device=weight.device)
-        with _On(weight.device) as stream:
-            _lib.check(lib.dvae_embed_fwd(weight.data_ptr(), weight.stride(0) if V > 1 else D, ids.data_ptr(),
-                                          int(ids.dtype == torch.int64), out.data_ptr(), ids.numel(), V, D, scale,
-                                          DTYPES[weight.dtype], stream), "dvae_embed_fwd")
         ctx.save_for_backward(ids)
-        ctx.table, ctx.scale = (V, D), scale
-        return out
+        ctx.table, ctx.scale = tuple(weight.shape), scale
+        return _embed_forward(weight, ids, scale)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        lib = _lib.load()
+        _once("embed")
         ids, = ctx.saved_tensors
         V, D = ctx.table
         n = ids.numel()
         dout, ld = _rows(dout.reshape(n, D))
         dw = torch.empty(V, D, dtype=dout.dtype, device=dout.device)
-        ws = _workspace(lib.dvae_embed_bwd_ws_bytes(n, V, D), dout.device, "dvae_embed_bwd_ws_bytes")
-        with _On(dout.device) as stream:
-            _lib.check(lib.dvae_embed_bwd(dout.data_ptr(), ld, ids.data_ptr(), int(ids.dtype == torch.int64), dw.data_ptr(),
-                                          ws.data_ptr(), n, V, D, ctx.scale, DTYPES[dout.dtype], stream), "dvae_embed_bwd")
+        ws = _workspace(_lib.load().dvae_embed_bwd_ws_bytes(n, V, D), dout.device, "dvae_embed_bwd_ws_bytes")
+        _enqueue(dout.device, "dvae_embed_bwd", dout.data_ptr(), ld, ids.data_ptr(), _wide(ids), dw.data_ptr(), ws.data_ptr(),
+                 n, V, D, ctx.scale, DTYPES[dout.dtype])
         return dw, None, None
 
 
@@ -119,59 +124,63 @@ def embed(weight, ids, scale=1.0):
     not vary from run to run."""
     _matrix(weight, "weight", 2)
     V, D = weight.shape
-    _need(V > 0 and D > 0, "weight is empty")
-    _need((D == 1 or weight.stride(1) == 1) and (V == 1 or weight.stride(0) >= D), "the elements of a row of weight must lie side by side")
-    return _EmbedFn.apply(weight, _index(ids, "ids", weight.device), float(scale))
+    if V == 0 or D == 0:
+        raise ValueError("weight is empty")
+    if D > 1 and weight.stride(1) != 1 or V > 1 and weight.stride(0) < D:
+        raise ValueError("the elements of a row of weight must lie side by side")
+    ids = _index(ids, "ids", weight.device)
+    if weight.requires_grad and torch.is_grad_enabled():
+        return _EmbedFn.apply(weight, ids, float(scale))
+    return _embed_forward(weight, ids, float(scale))
 
 
 # ------------------------------------------------------------------------------------------------------------- recurrence
 
+def _scan_forward(gate, x, offsets, h0, seqs, keep):
+    """(h, last, the states that the backward pass reads if `keep`)"""
+    lib = _lib.load()
+    g, ld_g = _flat_rows(gate)
+    y, ld_y = _flat_rows(x)
+    n, D = g.shape
+    dev = x.device
+    h = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    last = torch.empty(seqs, D, dtype=torch.float32, device=dev)
+    states = torch.empty(lib.dvae_scan_state_floats(n, D), dtype=torch.float32, device=dev) if keep else None
+    ws = _workspace(lib.dvae_scan_ws_bytes(n, D), dev, "dvae_scan_ws_bytes")
+    _enqueue(dev, "dvae_scan_fwd", g.data_ptr(), ld_g, y.data_ptr(), ld_y, _lib.ptr(offsets), _wide(offsets), _lib.ptr(h0),
+             h.data_ptr(), last.data_ptr(), _lib.ptr(states), ws.data_ptr(), n, seqs, D, DTYPES[x.dtype])
+    return h, last, states
+
+
 class _ScanFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, gate, x, offsets, h0, seqs):
-        lib = _lib.load()
-        g, ld_g = _flat_rows(gate)
-        y, ld_y = _flat_rows(x)
-        n, D = g.shape
-        h = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        last = torch.empty(seqs, D, dtype=torch.float32, device=x.device)
-        states = None
-        if any(ctx.needs_input_grad[i] for i in (0, 1, 3)):
-            states = torch.empty(lib.dvae_scan_state_floats(n, D), dtype=torch.float32, device=x.device)
-        ws = _workspace(lib.dvae_scan_ws_bytes(n, D), x.device, "dvae_scan_ws_bytes")
-        with _On(x.device) as stream:
-            _lib.check(lib.dvae_scan_fwd(g.data_ptr(), ld_g, y.data_ptr(), ld_y, _lib.ptr(offsets),
-                                         int(offsets is not None and offsets.dtype == torch.int64), _lib.ptr(h0), h.data_ptr(),
-                                         last.data_ptr(), _lib.ptr(states), ws.data_ptr(), n, seqs, D, DTYPES[x.dtype], stream),
-                       "dvae_scan_fwd")
+        h, last, ctx.states = _scan_forward(gate, x, offsets, h0, seqs, True)
         ctx.save_for_backward(gate, x, offsets, h0)
-        ctx.states, ctx.seqs = states, seqs
+        ctx.seqs = seqs
         ctx.set_materialize_grads(False)
         return h, last
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dh, dlast):
-        lib = _lib.load()
+        _once("gated_scan")
         gate, x, offsets, h0 = ctx.saved_tensors
         g, ld_g = _flat_rows(gate)
         y, ld_y = _flat_rows(x)
         n, D = g.shape
+        dev = x.device
         ld_dh = 0
         if dh is not None:
             dh, ld_dh = _flat_rows(dh)
         if dlast is not None:
             dlast = dlast.contiguous()
-        dgate = torch.empty(gate.shape, dtype=x.dtype, device=x.device)
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        dh0 = torch.empty(ctx.seqs, D, dtype=torch.float32, device=x.device) if ctx.needs_input_grad[3] else None
-        ws = _workspace(lib.dvae_scan_ws_bytes(n, D), x.device, "dvae_scan_ws_bytes")
-        with _On(x.device) as stream:
-            _lib.check(lib.dvae_scan_bwd(g.data_ptr(), ld_g, y.data_ptr(), ld_y, _lib.ptr(offsets),
-                                         int(offsets is not None and offsets.dtype == torch.int64), _lib.ptr(h0),
-                                         ctx.states.data_ptr(), _lib.ptr(dh), ld_dh, _lib.ptr(dlast), dgate.data_ptr(),
-                                         dx.data_ptr(), _lib.ptr(dh0), ws.data_ptr(), n, ctx.seqs, D, DTYPES[x.dtype], stream),
-                       "dvae_scan_bwd")
+        dgate = torch.empty(gate.shape, dtype=x.dtype, device=dev)
+        dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        dh0 = torch.empty(ctx.seqs, D, dtype=torch.float32, device=dev) if ctx.needs_input_grad[3] else None
+        ws = _workspace(_lib.load().dvae_scan_ws_bytes(n, D), dev, "dvae_scan_ws_bytes")
+        _enqueue(dev, "dvae_scan_bwd", g.data_ptr(), ld_g, y.data_ptr(), ld_y, _lib.ptr(offsets), _wide(offsets), _lib.ptr(h0),
+                 ctx.states.data_ptr(), _lib.ptr(dh), ld_dh, _lib.ptr(dlast), dgate.data_ptr(), dx.data_ptr(), _lib.ptr(dh0),
+                 ws.data_ptr(), n, ctx.seqs, D, DTYPES[x.dtype])
         return dgate, dx, None, dh0, None
 
 
@@ -188,21 +197,27 @@ def gated_scan(gate, x, offsets=None, h0=None):
     dims = 2 if offsets is not None else 3
     _matrix(gate, "gate", dims)
     _matrix(x, "x", dims)
-    _need(gate.dtype == x.dtype and gate.device == x.device, "gate and x differ in type or device")
-    _need(gate.shape == x.shape, "gate has the shape %s, x %s" % (tuple(gate.shape), tuple(x.shape)))
+    if gate.dtype != x.dtype or gate.device != x.device:
+        raise ValueError("gate and x differ in type or device")
+    if gate.shape != x.shape:
+        raise ValueError("gate has the shape %s, x %s" % (tuple(gate.shape), tuple(x.shape)))
     D = x.shape[-1]
-    _need(D > 0, "gate and x have no channels")
+    if D == 0:
+        raise ValueError("gate and x have no channels")
     if offsets is not None:
         offsets = _index(offsets, "offsets", x.device)
-        _need(offsets.dim() == 1 and offsets.numel() >= 1, "offsets must have one dimension and at least one value")
+        if offsets.dim() != 1 or offsets.numel() < 1:
+            raise ValueError("offsets must have one dimension and at least one value")
         seqs = offsets.numel() - 1
     else:
         seqs = x.shape[0]
     if h0 is not None:
-        _need(torch.is_tensor(h0) and h0.dtype == torch.float32 and h0.device == x.device and tuple(h0.shape) == (seqs, D),
-              "h0 must be a float32 tensor of shape (%d, %d) on %s" % (seqs, D, x.device))
+        if not torch.is_tensor(h0) or h0.dtype != torch.float32 or h0.device != x.device or tuple(h0.shape) != (seqs, D):
+            raise ValueError("h0 must be a float32 tensor of shape (%d, %d) on %s" % (seqs, D, x.device))
         h0 = h0.contiguous()
-    return _ScanFn.apply(gate, x, offsets, h0, seqs)
+    if torch.is_grad_enabled() and (gate.requires_grad or x.requires_grad or (h0 is not None and h0.requires_grad)):
+        return _ScanFn.apply(gate, x, offsets, h0, seqs)
+    return _scan_forward(gate, x, offsets, h0, seqs, False)[:2]
 
 
 def gated_step(gate, x, state, slots=None):
@@ -212,27 +227,29 @@ def gated_step(gate, x, state, slots=None):
     For serving: not differentiable, inputs that need gradients are refused outside torch.no_grad()."""
     code = _matrix(gate, "gate", 2)
     _matrix(x, "x", 2)
-    _need(gate.dtype == x.dtype and gate.device == x.device and gate.shape == x.shape, "gate and x differ in type, device or shape")
+    dev = x.device
+    if gate.dtype != x.dtype or gate.device != dev or gate.shape != x.shape:
+        raise ValueError("gate and x differ in type, device or shape")
     B, D = x.shape
-    _need(D > 0, "gate and x have no channels")
-    _need(torch.is_tensor(state) and state.dtype == torch.float32 and state.device == x.device and state.dim() == 2 and
-          state.shape[1] == D, "state must be a float32 tensor of shape (P, %d) on %s" % (D, x.device))
+    if D == 0:
+        raise ValueError("gate and x have no channels")
+    if not torch.is_tensor(state) or state.dtype != torch.float32 or state.device != dev or state.dim() != 2 or state.shape[1] != D:
+        raise ValueError("state must be a float32 tensor of shape (P, %d) on %s" % (D, dev))
     P = state.shape[0]
-    _need((D == 1 or state.stride(1) == 1) and (P <= 1 or state.stride(0) >= D), "the elements of a row of state must lie side by side")
-    if torch.is_grad_enabled() and (gate.requires_grad or x.requires_grad or state.requires_grad):
+    if D > 1 and state.stride(1) != 1 or P > 1 and state.stride(0) < D:
+        raise ValueError("the elements of a row of state must lie side by side")
+    if (gate.requires_grad or x.requires_grad or state.requires_grad) and torch.is_grad_enabled():
         raise ValueError("gated_step is not differentiable: call it under torch.no_grad(), or use gated_scan")
     if slots is not None:
-        slots = _index(slots, "slots", x.device)
-        _need(tuple(slots.shape) == (B,), "slots must have the shape (%d,)" % B)
-    else:
-        _need(B <= P, "%d rows, but %d states" % (B, P))
+        slots = _index(slots, "slots", dev)
+        if slots.dim() != 1 or slots.shape[0] != B:
+            raise ValueError("slots must have the shape (%d,)" % B)
+    elif B > P:
+        raise ValueError("%d rows, but %d states" % (B, P))
     g, ld_g = _rows(gate)
     y, ld_y = _rows(x)
-    h = torch.empty(B, D, dtype=x.dtype, device=x.device)
-    with _On(x.device) as stream:
-        _lib.check(_lib.load().dvae_scan_step(g.data_ptr(), ld_g, y.data_ptr(), ld_y, state.data_ptr(),
-                                              state.stride(0) if P > 1 else D, P, _lib.ptr(slots),
-                                              int(slots is not None and slots.dtype == torch.int64), h.data_ptr(), B, D, code,
-                                              stream), "dvae_scan_step")
+    h = torch.empty(B, D, dtype=x.dtype, device=dev)
+    _enqueue(dev, "dvae_scan_step", g.data_ptr(), ld_g, y.data_ptr(), ld_y, state.data_ptr(), state.stride(0) if P > 1 else D, P,
+             _lib.ptr(slots), _wide(slots), h.data_ptr(), B, D, code)
     torch.autograd.graph.increment_version(state)
     return h
