@@ -669,6 +669,8 @@ extern "C" int dvae_scan_step(const void* gate, int64_t ld_gate, const void* x, 
     DVAE_REQUIRE(rows >= 0 && rows <= (1 << 24) && pool >= 0, "scan_step: %d rows are not supported", rows);
     DVAE_REQUIRE(D >= 1 && D <= (1 << 20), "scan_step: %d channels are not in 1 .. 2^20", D);
     DVAE_REQUIRE((ld_gate == 0 || ld_gate >= D) && (ld_x == 0 || ld_x >= D) && ld_state >= D, "scan_step: a row stride is below %d channels", D);
+    // (every row reads all slots, to find the rows that share its own)
+    DVAE_REQUIRE(!slots || rows <= 65536, "scan_step: %d rows with slots; at most 65536 are supported", rows);
     DVAE_REQUIRE(slots || rows <= pool, "scan_step: %d rows, but a pool of %lld states", rows, (long long)pool);
     if (rows == 0) return DVAE_OK;
     DVAE_REQUIRE(gate && x && h && (state || pool == 0), "scan_step: null pointer");

@@ -27,19 +27,23 @@ def orthogonalize(updates, steps=5, coefficients=QUINTIC, out=None):
     every product in one launch.  coefficients: (a, b, c), or one such triple for each step; a set that lets a singular value
     leave [-2, 2] is refused.  out: where to write (same shapes and type; a matrix may be its own output), default new tensors.
     Accuracy of float32 throughout, rounded once to the matrices' type.  A zero matrix gives zeros, one with a NaN or an
-    infinity NaN.  Not differentiable (it acts on updates)."""
+    infinity NaN.  Not differentiable (it acts on updates): inputs that need gradients are refused outside torch.no_grad()."""
     one = torch.is_tensor(updates)
     mats = [updates] if one else list(updates)
     if out is not None:
         outs = [out] if one else list(out)
         if len(outs) != len(mats):
             raise ValueError("out has %d matrices, updates %d" % (len(outs), len(mats)))
-    steps = int(steps)
-    triples = [tuple(coefficients)] * steps if not hasattr(coefficients[0], "__len__") else [tuple(c) for c in coefficients]
+    steps, coefficients = int(steps), list(coefficients)
+    if coefficients and not hasattr(coefficients[0], "__len__"):
+        coefficients = [coefficients] * steps
+    triples = [tuple(c) for c in coefficients]
     if len(triples) != steps or any(len(c) != 3 for c in triples):
         raise ValueError("coefficients must be (a, b, c) or one such triple for each of the %d steps" % steps)
     if not mats:
         return []
+    if torch.is_grad_enabled() and any(torch.is_tensor(g) and g.requires_grad for g in mats):
+        raise ValueError("orthogonalize is not differentiable: call it under torch.no_grad()")
     code = _matrix(mats[0], "updates", 2)
     dtype, device = mats[0].dtype, mats[0].device
     with torch.no_grad():

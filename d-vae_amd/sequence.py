@@ -41,11 +41,12 @@ def _wide(t):
     return 1 if t is not None and t.dtype == torch.int64 else 0
 
 
-def _rows(t):
-    """(t, row stride) of a [N, D] matrix whose elements lie side by side in a row; other layouts are copied"""
+def _rows(t, most=1 << 23):
+    """(t, row stride) of a [N, D] matrix whose elements lie side by side in a row; other layouts, and rows more than `most`
+    elements apart (the recurrence addresses a few rows with 32-bit offsets), are copied"""
     n, d = t.shape
     s0, s1 = t.stride()
-    if d > 1 and s1 != 1 or n > 1 and 0 < s0 < d:
+    if d > 1 and s1 != 1 or n > 1 and (0 < s0 < d or s0 > most):
         return t.contiguous(), d
     return t, s0 if n > 1 else d
 
@@ -222,8 +223,9 @@ def gated_scan(gate, x, offsets=None, h0=None):
 
 def gated_step(gate, x, state, slots=None):
     """One token of each of B sequences: gate, x [B, D]; returns h [B, D] in x's type and updates `state` [P, D] (float32)
-    in place at the rows `slots` [B] (int32 / int64; default: row b has state b).  A slot outside [0, P) marks a padding
-    row: its h is zero and no state changes.  Rows that name the same slot advance it one after the other, in their order.
+    in place at the rows `slots` [B] (int32 / int64, B at most 65536; default: row b has state b).  A slot outside [0, P)
+    marks a padding row: its h is zero and no state changes.  Rows that name the same slot advance it one after the other,
+    in their order.
     For serving: not differentiable, inputs that need gradients are refused outside torch.no_grad()."""
     code = _matrix(gate, "gate", 2)
     _matrix(x, "x", 2)

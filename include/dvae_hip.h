@@ -470,7 +470,7 @@ int dvae_embed_bwd(const void* dout, int64_t ld_dout, const void* ids, int32_t i
  * sequence s is the rows [off[s], off[s+1]) (off: seqs + 1 values that do not decrease, int32 or int64; NULL: sequences of
  * rows / seqs rows each); values outside [0, rows] count as the nearer end.  The state before a sequence is h0[s] (fp32
  * [seqs][D]; NULL: zeros).  gate, x: row strides ld_* in elements (halves of one projection's output are allowed; 0 = one
- * row for all); h [rows][D] contiguous, rounded once; last [seqs][D] fp32: the state after each sequence (h0 where it is
+ * row for all; at most 2^23); h [rows][D] contiguous, rounded once; last [seqs][D] fp32: the state after each sequence (h0 where it is
  * empty).  Rows of no sequence give zeros.  states: dvae_scan_state_floats() floats that the backward pass reads (NULL if
  * there is none); ws: dvae_scan_ws_bytes() bytes, 16-byte aligned, for this call alone. */
 int64_t dvae_scan_state_floats(int64_t rows, int32_t D);
@@ -484,7 +484,7 @@ int dvae_scan_bwd(const void* gate, int64_t ld_gate, const void* x, int64_t ld_x
                   const float* h0, const float* states, const void* dh, int64_t ld_dh, const float* dlast, void* dgate, void* dx,
                   float* dh0, void* ws, int64_t rows, int64_t seqs, int32_t D, int32_t dtype, void* stream);
 /* One token of each of `rows` sequences: state[slots[b]] = h[b] = z[b] state[slots[b]] + (1 - z[b]) x[b], in place in a
- * pool of fp32 states (row stride ld_state).  slots: int32 / int64, NULL: row b has state b.  A slot outside [0, pool)
+ * pool of fp32 states (row stride ld_state).  slots: int32 / int64 (rows <= 65536), NULL: row b has state b.  A slot outside [0, pool)
  * marks a padding row: h[b] = 0, no state changes.  Rows with the same slot advance it one after the other in their order. */
 int dvae_scan_step(const void* gate, int64_t ld_gate, const void* x, int64_t ld_x, float* state, int64_t ld_state,
                    int64_t pool, const void* slots, int32_t slots_i64, void* h, int32_t rows, int32_t D, int32_t dtype,

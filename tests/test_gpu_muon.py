@@ -258,7 +258,7 @@ def test_flat_muon_refusals():
         dvae_amd.harness.GraphedTrainStep(model, O.FlatMuon(model))
     m = torch.randn(8, 8).cuda()
     for bad in ((m[0], {}), (m.double(), {}), ([m, m.half()], {}), (m[:0], {}), (m, dict(out=m[:4])), (m, dict(steps=0)), (m, dict(coefficients=(1.0, 2.0))),
-                ([m], dict(out=[])), (m, dict(out=m.t()[:, :4]))):
+                (m, dict(coefficients=())), (m.clone().requires_grad_(True), {}), ([m], dict(out=[])), (m, dict(out=m.t()[:, :4]))):
         with pytest.raises((ValueError, dvae_amd._lib.DvaeHipError)):
             O.orthogonalize(bad[0], **bad[1])
     with pytest.raises(dvae_amd._lib.DvaeHipError, match="singular values leave"):

@@ -69,6 +69,47 @@ def test_embed_and_its_gradient(dtype, n, vocab, dim):
     assert torch.equal(dw, again)
 
 
+def test_embed_many_tokens():
+    """more tokens than one round of the sorting workgroups"""
+    g = gen(30)
+    n, V = 600_001, 300
+    ids = torch.randint(-1, V, (n,), generator=g)
+    w = torch.randn(V, 3, generator=g).cuda().requires_grad_(True)
+    dout = torch.randn(n, 3, generator=g)
+    dw, = torch.autograd.grad(S.embed(w, ids.cuda()), [w], dout.cuda())
+    ok = ids >= 0
+    want = torch.zeros(V, 3, dtype=torch.float64).index_add_(0, ids[ok], dout.double()[ok])
+    size = torch.zeros(V, 3, dtype=torch.float64).index_add_(0, ids[ok], dout.double()[ok].abs())
+    close(dw, want, size * (32 + 70 + 8 + 2) * U, "dw")  # 63 chunks or so per row
+
+
+def test_offsets_past_32_bits():
+    n, D = 2_200_000, 1024  # 2.25e9 elements
+    ids = torch.zeros(n, dtype=torch.int32, device="cuda")
+    ids[-40:] = torch.arange(40, device="cuda", dtype=torch.int32) % 3
+    w = torch.randn(3, D, device="cuda").bfloat16().requires_grad_(True)
+    out = S.embed(w, ids)
+    assert torch.equal(out[-40:], w[ids[-40:].long()]) and torch.equal(out[:3], w[:1].expand(3, D))
+    dout = torch.zeros(n, D, device="cuda", dtype=torch.bfloat16)
+    dout[-40:] = 1
+    dw, = torch.autograd.grad(out, [w], dout)
+    count = torch.bincount(ids[-40:].long(), minlength=3).bfloat16()
+    assert torch.equal(dw, count[:, None].expand(3, D))
+    del out, dout
+    gate = torch.empty(n, D, device="cuda", dtype=torch.bfloat16).normal_()
+    x = torch.empty(n, D, device="cuda", dtype=torch.bfloat16).normal_()
+    off = torch.tensor([0, 1_100_000, n - 300, n], device="cuda")
+    a, b = gate.requires_grad_(True), x.requires_grad_(True)
+    h, last = S.gated_scan(a, b, off)
+    dg, dx = torch.autograd.grad([h, last], [a, b], [torch.ones(1, 1, device="cuda", dtype=torch.bfloat16).expand(n, D), torch.ones_like(last)])
+    h2, last2 = S.gated_scan(gate.detach()[-300:], x.detach()[-300:], torch.tensor([0, 300], device="cuda"))
+    # other tiles, so the last sequence's sums are composed in another order: both are within their bound of the exact one
+    tol = 2 * (8 * 300 + 32) * U * 6
+    close(h[-300:], h2.double().cpu(), tol + 2.0 ** -8 * 6, "h")
+    close(last[2], last2[0].double().cpu(), tol, "last")
+    assert torch.isfinite(dg[-300:]).all() and dx[-300:].abs().sum() > 0 and torch.isfinite(dx[:300]).all()
+
+
 def test_embed_shapes_strides_and_no_tokens():
     g = gen(1)
     big = torch.randn(9, 40, generator=g).cuda()
@@ -226,6 +267,10 @@ def test_gated_scan_equal_lengths_and_layouts():
         assert torch.equal(h, h3) and torch.equal(last, last3)
     one, last4 = S.gated_scan(gate[:, :1], x[:, :1])  # length one, rows of stride T 2 D
     assert torch.equal(one, h[:, :1]) and torch.equal(last4, h[:, 0])
+    wide = torch.zeros(2, 1 << 18, D, device="cuda")  # rows 2^18 D elements apart
+    wide[:, :1] = gate[:2, :1]
+    far, _ = S.gated_scan(wide[:, :1], x[:2, :1])
+    assert torch.equal(far, h[:2, :1])
     none, last5 = S.gated_scan(gate[:, :0], x[:, :0], h0=torch.ones(B, D, device="cuda"))
     assert none.shape == (B, 0, D) and torch.equal(last5, torch.ones(B, D, device="cuda"))
     gl, xl = gate.detach().requires_grad_(True), x.detach().requires_grad_(True)

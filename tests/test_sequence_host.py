@@ -55,6 +55,8 @@ def test_the_c_entries_refuse_bad_sizes_before_any_launch():
     assert "element type" in rc("dvae_scan_bwd", p, 8, p, 8, None, 0, None, p, p, 8, p, p, p, p, p, 8, 2, 8, 3, None)
     assert "rows" in rc("dvae_scan_ws_bytes", -1, 8)
     assert "pool" in rc("dvae_scan_step", p, 8, p, 8, p, 8, 3, None, 0, p, 4, 8, 0, None)
+    assert "65536" in rc("dvae_scan_step", p, 8, p, 8, p, 8, 1 << 20, p, 0, p, 65537, 8, 0, None)
+    assert "row stride" in rc("dvae_scan_fwd", p, (1 << 23) + 1, p, 8, None, 0, None, p, p, None, p, 8, 2, 8, 0, None)
     assert "row stride" in rc("dvae_scan_step", p, 8, p, 8, p, 7, 4, None, 0, p, 4, 8, 0, None)
     assert "null" in rc("dvae_scan_step", p, 8, p, 8, None, 8, 4, None, 0, p, 4, 8, 0, None)
 
