@@ -58,6 +58,27 @@ def test_orthogonalize(dtype, k):
     assert all(torch.equal(a, b) for a, b in zip(outs, again))
 
 
+BIG = [[(600, 640)], [(1400, 1500)], [(2300, 2500)], [(3200, 3205)], [(4000, 4096)], [(5600, 5630)], [(2305, 1000), (1000, 2305), (700, 3000)]]
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("k", range(len(BIG)))
+def test_orthogonalize_large(dtype, k):
+    """every tile size and both numbers of planes.  bf16 matrices of these sizes are held in one plane: A, B and X are rounded by
+    2^-12 / sqrt(3) (r.m.s., independent entries), of which A's counts |b + 2 c A| <= 5 times and B's twice: 8 a step relative
+    to X, and relative errors do not grow where p is concave from 0 (s p'(s) <= p(s)): five steps, and the result's rounding."""
+    dt, g = DT[dtype], torch.Generator(device="cuda")
+    g.manual_seed(k)
+    mats = [torch.randn(s, generator=g, device="cuda").to(dt) for s in BIG[k]]
+    for m, o in zip(mats, O.orthogonalize(mats)):
+        want = plain(m)  # in float64 on the device
+        rel = float((o.double() - want).norm() / want.norm())
+        assert rel < (341 * 16 * 2.0 ** -22 if dtype == "fp32" else 40 * 2.0 ** -12 / 3 ** 0.5 + 2.0 ** -9), (m.shape, rel)
+        if dtype == "fp32":
+            plain32 = plain(m, dtype=torch.float32).double()
+            assert rel < 4 * max(float((plain32 - want).norm() / want.norm()), 2.0 ** -22), (m.shape, rel)
+
+
 def test_orthogonalize_makes_singular_values_near_one():
     m = torch.randn(200, 333, generator=gen(1)).cuda()
     s = torch.linalg.svdvals(O.orthogonalize(m).double().cpu())
