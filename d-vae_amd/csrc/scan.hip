@@ -480,17 +480,18 @@ __global__ __launch_bounds__(256) void scan_begin_kernel(ulonglong2* __restrict_
 // ------------------------------------------------------------------------------------------------------- single tokens
 // One wave per row and slab.  Rows that name the same slot are advanced in their order by the first of them, so a
 // repeated slot is neither a race nor dependent on timing; the search for them reads the slots alone.
-template <typename T, int V>
+template <typename I> struct Slots4 { I s[4]; };  // (aligned to one slot only)
+
+template <typename T, int V, typename I>
 __global__ __launch_bounds__(256) void scan_step_kernel(const T* __restrict__ gate, long ld_gate, const T* __restrict__ x, long ld_x,
-                                                        float* __restrict__ state, long ld_state, long pool, const void* __restrict__ slots,
-                                                        int i64, T* __restrict__ h, int B, int D, int slabs) {
+                                                        float* __restrict__ state, long ld_state, long pool, const I* __restrict__ slots,
+                                                        T* __restrict__ h, int B, int D, int slabs) {
     const int lane = threadIdx.x & 63;
     const long unit = (long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int b = (int)(unit / slabs), c = (int)(unit % slabs) * 64 * V + lane * V;
     if (b >= B) return;
     const bool live = c < D;
-    auto slot = [&](int r) { return i64 ? reinterpret_cast<const int64_t*>(slots)[r] : (int64_t)reinterpret_cast<const int32_t*>(slots)[r]; };
-    const long k = slots ? slot(b) : b;
+    const long k = slots ? (long)slots[b] : b;
     if (k < 0 || k >= pool) {  // padding
         const float zero[V] = {};
         if (live) store_floats<T, V>(h + (long)b * D + c, zero);
@@ -503,18 +504,33 @@ __global__ __launch_bounds__(256) void scan_step_kernel(const T* __restrict__ ga
 #pragma unroll
     for (int j = 0; j < V; ++j) s[j] = state[k * ld_state + cc + j];
     bool again = false;  // a later row names the same slot
-    if (slots)
-        for (int r0 = 0; r0 < B; r0 += 64 * 8) {
-            bool same[8];
+    if (slots) {
+        const I mine = (I)k;
+        bool before = false, after = false;
+        // four slots a lane and load, four loads under way; the last loads end at B, rows seen twice do no harm
+        for (int r0 = 0; B >= 256 && r0 < B; r0 += 1024) {
+            Slots4<I> q[4];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) same[u] = slot(min(r0 + 64 * u + lane, B - 1)) == k;
+            for (int u = 0; u < 4; ++u) q[u] = *reinterpret_cast<const Slots4<I>*>(slots + min(r0 + 256 * u, B - 256) + lane * 4);
 #pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                const int r = r0 + 64 * u + lane;
-                if (__ballot(same[u] && r < b)) return;  // an earlier row advances this slot
-                again = again || __ballot(same[u] && r > b && r < B);
-            }
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int r = min(r0 + 256 * u, B - 256) + lane * 4 + e;
+                    before = before || (q[u].s[e] == mine && r < b);
+                    after = after || (q[u].s[e] == mine && r > b);
+                }
         }
+        if (B < 256)
+            for (int r0 = 0; r0 < B; r0 += 64) {
+                const int r = r0 + lane;
+                const bool same = r < B && slots[min(r, B - 1)] == mine;
+                before = before || (same && r < b);
+                after = after || (same && r > b);
+            }
+        if (__any(before)) return;  // an earlier row advances this slot
+        again = __any(after);
+    }
     auto advance = [&](int r) {
 #pragma unroll
         for (int j = 0; j < V; ++j) {
@@ -527,7 +543,7 @@ __global__ __launch_bounds__(256) void scan_step_kernel(const T* __restrict__ ga
     advance(b);
     if (again)
         for (int r0 = b + 1; r0 < B; r0 += 64) {
-            unsigned long long more = __ballot(r0 + lane < B && slot(min(r0 + lane, B - 1)) == k);
+            unsigned long long more = __ballot(r0 + lane < B && (long)slots[min(r0 + lane, B - 1)] == k);
             while (more) {
                 const int r = r0 + __ffsll(more) - 1;
                 g = load_pack<T, V>(gate + (long)r * ld_gate + cc);
@@ -679,11 +695,14 @@ extern "C" int dvae_scan_step(const void* gate, int64_t ld_gate, const void* x, 
     const long units = (long)rows * slabs;
     DVAE_REQUIRE(units < (1LL << 31), "scan_step: %d rows of %d channels are too many", rows, D);
     const dim3 grid((unsigned)((units + 3) / 4));
-#define SCAN_STEP(T, V)                                                                                              \
-    hipLaunchKernelGGL((scan_step_kernel<T, V>), grid, dim3(256), 0, (hipStream_t)stream, (const T*)gate, (long)ld_gate, (const T*)x, \
-                       (long)ld_x, state, (long)ld_state, (long)pool, slots, slots_i64, (T*)h, rows, D, slabs)
+#define SCAN_STEP_BY(T, V, I)                                                                                                   \
+    hipLaunchKernelGGL((scan_step_kernel<T, V, I>), grid, dim3(256), 0, (hipStream_t)stream, (const T*)gate, (long)ld_gate,       \
+                       (const T*)x, (long)ld_x, state, (long)ld_state, (long)pool, (const I*)slots, (T*)h, rows, D, slabs)
+#define SCAN_STEP(T, V) \
+    if (slots_i64) SCAN_STEP_BY(T, V, int64_t); else SCAN_STEP_BY(T, V, int32_t)
     DVAE_BY_TYPE(dtype, vec, SCAN_STEP);
 #undef SCAN_STEP
+#undef SCAN_STEP_BY
     DVAE_LAUNCH_CHECK();
     return DVAE_OK;
 }

@@ -26,7 +26,7 @@ def orthogonalize(updates, steps=5, coefficients=QUINTIC, out=None):
     updates: a matrix or a list of matrices (float32, bfloat16 or float16, one type, on one HIP device); a list goes through
     every product in one launch.  coefficients: (a, b, c), or one such triple for each step; a set that lets a singular value
     leave [-2, 2] is refused.  out: where to write (same shapes and type; a matrix may be its own output), default new tensors.
-    Accuracy of float32 throughout, rounded once to the matrices' type.  A zero matrix gives zeros, one with a NaN or an
+    Accuracy of float32 (for bfloat16 of its own rounding), rounded once to the matrices' type.  A zero matrix gives zeros, one with a NaN or an
     infinity NaN.  Not differentiable (it acts on updates): inputs that need gradients are refused outside torch.no_grad()."""
     one = torch.is_tensor(updates)
     mats = [updates] if one else list(updates)

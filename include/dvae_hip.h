@@ -495,8 +495,8 @@ int dvae_scan_step(const void* gate, int64_t ld_gate, const void* x, int64_t ld_
  * out = the last X of `steps` Newton-Schulz steps X <- a X + (b A + c A A) X, A = X X^T (on the smaller side), from
  * X = g / |g|_F, for `count` matrices of one element type (HOST array of descriptors; g, out device pointers, row strides in
  * elements, out not overlapping any g).  coefficients (host): a, b, c of every step, 3 * steps floats; sets that let a singular
- * value leave [-2, 2] are refused.  fp32 accuracy whatever the type (split fp16 planes, see csrc/orthogonalize.hip), rounded
- * once at the end; a zero matrix gives zeros, one that holds a NaN or an infinity gives NaN.  Sides up to 32768.
+ * value leave [-2, 2] are refused.  fp32 accuracy (split fp16 planes, see csrc/orthogonalize.hip) for fp32 and fp16, for
+ * bf16 an error of the order of the result's own rounding, rounded once at the end; a zero matrix gives zeros, one that holds a NaN or an infinity gives NaN.  Sides up to 32768.
  * ws: dvae_orthogonalize_ws_bytes() bytes, 16-byte aligned, for this call alone. */
 typedef struct dvae_matrix_desc {
     const void* g;

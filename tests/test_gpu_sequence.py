@@ -337,7 +337,7 @@ def test_gated_scan_offsets_outside_the_rows_count_as_the_nearer_end():
 # ------------------------------------------------------------------------------------------------------------------- step
 
 @pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
-@pytest.mark.parametrize("rows,pool,dim", [(1, 1, 1), (5, 9, 7), (64, 64, 501), (65, 300, 256), (300, 200, 68)])
+@pytest.mark.parametrize("rows,pool,dim", [(1, 1, 1), (5, 9, 7), (64, 64, 501), (65, 300, 256), (300, 200, 68), (255, 50, 20), (256, 50, 20), (2500, 700, 40)])
 def test_gated_step(dtype, rows, pool, dim):
     dt, g = DT[dtype], gen(rows + dim)
     gate, x = (torch.randn(rows, dim, generator=g) * 2).to(dt), torch.randn(rows, dim, generator=g).clamp(-3, 3).to(dt)
