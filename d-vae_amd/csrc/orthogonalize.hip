@@ -24,6 +24,13 @@
 // symmetric), B X against the rows of X^T, which is kept beside X: an output tile is written in both orientations.  The
 // two symmetric products compute the tiles on and above the diagonal alone and write each also mirrored.
 //
+// Tiles.  A stage of a 128 x 128 tile in two planes has 24 MFMAs (768 cycles) a wave for 96 KB through LDS (750 cycles): both
+// ends meet.  In one plane LDS would lead (750 to 512), which 256 x 256 tiles even out (2000 to 2048) where they fill whole
+// rounds of the chip: the update product at 4096 x 4096 190 -> 155 us (0.89 PFLOP/s); in two planes a whole call 5.03 -> 4.82 ms
+// (0.86 PFLOP/s of MFMA work).  Fewer tiles than 1.25 per CU take 64 x 64 (the products X X^T of the ENAS model: 60 -> 33 us); at most one
+// 64 x 64 tile per CU, four groups of waves share the sum (1024 x 1024: 217 us a call); at most one 32 x 32 tile per CU, the
+// direct kernel (501 x 501: 155 -> 131 us a call, 256 x 256: 118 -> 96; 768 x 768 would lose: 189 -> 232).
+//
 // Launches.  The matrices of a call go through each product together, one grid over all their tiles: an optimiser step on a
 // model's many small matrices is 17 launches, whatever their number (up to 32 per group).
 #include "common.h"

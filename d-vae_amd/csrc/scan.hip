@@ -15,6 +15,12 @@
 // each wave holds its RW rows in registers, the waves compose their (A, B) through LDS.  The tiles do not follow the
 // sequences: a sequence's first row just makes A = 0, so that many short sequences and one long one cost the same.  All
 // states, products and sums are fp32; outputs are rounded once.
+//
+// One pass over the data in either direction (forward 3, backward 5 matrices of memory traffic), tiles chained through
+// look_back.  Measured on 131072 x 1024 bf16: forward 225 us (3.6 TB/s), backward 392 us (3.4 TB/s), where a large copy
+// reaches 4.9; without the look-back the forward pass takes 166 us, so the chain and not the arithmetic is what is left there,
+// and the backward pass 363, with trivial gates 320: it is near the vector units' rate as well.
+// Tiles of 64 rows: 315 and 443 us; a look-back of 16 tiles: 277 and 407 us (more words read per tile than it saves waits).
 #include "seq_common.h"
 
 namespace dvae {
@@ -478,6 +484,7 @@ __global__ __launch_bounds__(256) void scan_begin_kernel(ulonglong2* __restrict_
 }
 
 // ------------------------------------------------------------------------------------------------------- single tokens
+// Bound by memory for large batches (2048 rows of 1024 bf16: 9.3 us; without slots 6.1 us, 4.8 TB/s), by the launch for small.
 // One wave per row and slab.  Rows that name the same slot are advanced in their order by the first of them, so a
 // repeated slot is neither a race nor dependent on timing; the search for them reads the slots alone.
 template <typename I> struct Slots4 { I s[4]; };  // (aligned to one slot only)
