@@ -17,15 +17,17 @@
 // states, products and sums are fp32; outputs are rounded once.
 //
 // One pass over the data in either direction (forward 3, backward 5 matrices of memory traffic), tiles chained through
-// look_back.  Measured on 131072 x 1024 bf16: forward 225 us (3.6 TB/s), backward 392 us (3.4 TB/s), where a large copy
-// reaches 4.9; without the look-back the forward pass takes 166 us, so the chain and not the arithmetic is what is left there,
-// and the backward pass 363, with trivial gates 320: it is near the vector units' rate as well.
-// Tiles of 64 rows: 315 and 443 us; a look-back of 16 tiles: 277 and 407 us (more words read per tile than it saves waits).
+// look_back.  Measured on 131072 x 1024 bf16: forward 225 us (3.6 TB/s), backward 372 us (3.6 TB/s), where a large copy
+// reaches 4.9.  Without the look-back the forward pass takes 166 us, so the chain and not the arithmetic is what is left there;
+// the backward pass with trivial gates and no look-back 320: reads and writes of five matrices, at the vector units' rate nearly.
+// Forward tiles of 64 rows: 318 us (a longer chain), of 256: 239; backward of 128: 392 (fewer workgroups a CU).  A look-back of
+// 16 tiles: 277 us forward (more words read per tile than it saves waits).
 #include "seq_common.h"
 
 namespace dvae {
 
-constexpr int TR = 128;  // rows of a tile: the state before every tile is kept for the backward pass
+constexpr int RW = 16;        // rows of a wave
+constexpr int TRF = 128, TRB = 64;  // rows of a tile, forward and backward; the state before every TRB rows is kept for the latter
 
 struct Rows {  // where the sequences lie
     const void* off;  // [S + 1] int32 / int64, or nullptr: S sequences of `len` rows each
@@ -43,7 +45,7 @@ struct Marks {
     long seq;                    // this lane's row's sequence
 };
 
-template <int RW> __device__ __forceinline__ Marks mark_rows(const Rows& q, long t0) {
+__device__ __forceinline__ Marks mark_rows(const Rows& q, long t0) {
     const int lane = threadIdx.x & 63;
     const long t = t0 + lane;
     bool start = false, end = false, cover = false;
@@ -156,7 +158,7 @@ struct ScanParams {
     void *h, *dgate, *dx;           // contiguous [N][D]
     const float *h0, *dlast;        // [S][D] or nullptr
     float *last, *dh0;              // [S][D]
-    float *states;                  // [tiles][D]: the state before each tile
+    float *states;                  // [N / TRB rounded up][D]: the state before every TRB rows
     unsigned long long* words;      // [tiles][D]: a tile's map, as published
     unsigned* ticket;
     Rows q;
@@ -203,7 +205,7 @@ template <typename T, int V> struct RowBuffer {
         else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, o), rsrc, col, i * pitch, 0);
     }
 };
-template <typename T, int V, int RW>
+template <typename T, int V>
 __device__ __forceinline__ void load_rows(Pack<T, V> (&r)[RW], const void* base, long ld, long t0, long N, int D, int c) {
     const RowBuffer<T, V> b(base, ld, t0, N, min(c, D - V));
 #pragma unroll
@@ -215,19 +217,20 @@ struct No { static constexpr bool value = false; };
 
 // Where a wave's rows all lie inside one sequence (PLAIN below) the row loops have no branches, so that the loads, the
 // exponentials and the chains of multiply-adds of several channels overlap.
-template <typename T, int V, int RW, int W>
-__global__ __launch_bounds__(W * 64) void scan_fwd_kernel(ScanParams p) {
-    static_assert(RW * W == TR && W >= V, "");
+template <typename T, int V>
+__global__ __launch_bounds__(TRF / RW * 64) void scan_fwd_kernel(ScanParams p) {
+    constexpr int W = TRF / RW;
+    static_assert(W >= V, "");
     __shared__ float As[W][64 * V], Bs[W][64 * V], Cs[64 * V];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const unsigned unit = __builtin_amdgcn_readfirstlane(take_ticket(p.ticket));
     const int c0 = (int)(unit % (unsigned)p.slabs) * 64 * V, c = c0 + lane * V;
-    const long tile = unit / (unsigned)p.slabs, t0 = tile * TR + wave * RW;
+    const long tile = unit / (unsigned)p.slabs, t0 = tile * TRF + wave * RW;
     const bool live = c < p.D;
     Pack<T, V> g[RW], x[RW];
-    load_rows<T, V, RW>(g, p.gate, p.ld_gate, t0, p.q.N, p.D, c);
-    load_rows<T, V, RW>(x, p.x, p.ld_x, t0, p.q.N, p.D, c);
-    const Marks m = mark_rows<RW>(p.q, t0);
+    load_rows<T, V>(g, p.gate, p.ld_gate, t0, p.q.N, p.D, c);
+    load_rows<T, V>(x, p.x, p.ld_x, t0, p.q.N, p.D, c);
+    const Marks m = mark_rows(p.q, t0);
     const bool plain = m.start == 0 && m.end == 0 && m.cover == (unsigned)((1ull << RW) - 1);
     float A[V], h[V], code[RW][V];
 #pragma unroll
@@ -271,7 +274,6 @@ __global__ __launch_bounds__(W * 64) void scan_fwd_kernel(ScanParams p) {
         publish(word, a, y);
         const float s = tile == 0 ? 0.f : look_back(word - p.D, -(long)p.D, tile);
         if (a != 0.f) publish(word, 0.f, through(a, y, s));
-        if (p.states) p.states[tile * p.D + c0 + k] = s;
         Cs[k] = s;
     }
     __syncthreads();
@@ -288,6 +290,9 @@ __global__ __launch_bounds__(W * 64) void scan_fwd_kernel(ScanParams p) {
         for (int w = 0; w < wave; ++w) s = through(As[w][lane * V + j], Bs[w][lane * V + j], s);
         h[j] = s;
     }
+    if (p.states && wave % (TRB / RW) == 0 && t0 < p.q.N)
+#pragma unroll
+        for (int j = 0; j < V; ++j) p.states[t0 / TRB * p.D + c + j] = h[j];
     const RowBuffer<T, V> out(p.h, p.D, t0, p.q.N, c);
     auto apply = [&](auto mixed) {
 #pragma unroll
@@ -318,25 +323,26 @@ __global__ __launch_bounds__(W * 64) void scan_fwd_kernel(ScanParams p) {
 }
 
 // Backward: the tiles are walked from the last; what flows from a tile to the one before it is z_t G_t of its first row.
-template <typename T, int V, int RW, int W>
-__global__ __launch_bounds__(W * 64) void scan_bwd_kernel(ScanParams p) {
-    static_assert(RW * W == TR && W >= V, "");
+template <typename T, int V>
+__global__ __launch_bounds__(TRB / RW * 64) void scan_bwd_kernel(ScanParams p) {
+    constexpr int W = TRB / RW;
+    static_assert(W >= V, "");
     __shared__ float As[W][64 * V], Bs[W][64 * V], Fs[W][64 * V], Cs[64 * V];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const unsigned unit = __builtin_amdgcn_readfirstlane(take_ticket(p.ticket));
     const int c0 = (int)(unit % (unsigned)p.slabs) * 64 * V, c = c0 + lane * V;
-    const long tiles = (p.q.N + TR - 1) / TR, tile = tiles - 1 - unit / (unsigned)p.slabs, t0 = tile * TR + wave * RW;
+    const long tiles = (p.q.N + TRB - 1) / TRB, tile = tiles - 1 - unit / (unsigned)p.slabs, t0 = tile * TRB + wave * RW;
     const bool live = c < p.D;
     Pack<T, V> g[RW], x[RW], d[RW];
-    load_rows<T, V, RW>(g, p.gate, p.ld_gate, t0, p.q.N, p.D, c);
-    load_rows<T, V, RW>(x, p.x, p.ld_x, t0, p.q.N, p.D, c);
-    if (p.dh) load_rows<T, V, RW>(d, p.dh, p.ld_dh, t0, p.q.N, p.D, c);
+    load_rows<T, V>(g, p.gate, p.ld_gate, t0, p.q.N, p.D, c);
+    load_rows<T, V>(x, p.x, p.ld_x, t0, p.q.N, p.D, c);
+    if (p.dh) load_rows<T, V>(d, p.dh, p.ld_dh, t0, p.q.N, p.D, c);
     else
 #pragma unroll
         for (int i = 0; i < RW; ++i)
 #pragma unroll
             for (int j = 0; j < V; ++j) d[i].e[j] = (T)0.f;
-    const Marks m = mark_rows<RW>(p.q, t0);
+    const Marks m = mark_rows(p.q, t0);
     const bool plain = m.start == 0 && m.end == 0 && m.cover == (unsigned)((1ull << RW) - 1);
     auto row_grad = [&](auto mixed, int i, float (&e)[V]) {  // dh of row i, and dlast where the sequence ends
 #pragma unroll
@@ -478,9 +484,11 @@ __global__ __launch_bounds__(256) void scan_begin_kernel(ulonglong2* __restrict_
         for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < pairs; i += (long)fill_blocks * 256) words[i] = make_ulonglong2(UNSET, UNSET);
         return;
     }
-    const long s = ((long)blockIdx.x - fill_blocks) * 4 + (threadIdx.x >> 6);
-    if (s >= q.S || (q.off ? q.at(s) < q.at(s + 1) : q.len > 0)) return;
-    for (int c = threadIdx.x & 63; c < D; c += 64) to[s * D + c] = from ? from[s * D + c] : 0.f;
+    for (int u = 0; u < 4; ++u) {
+        const long s = ((long)blockIdx.x - fill_blocks) * 4 + u;
+        if (s >= q.S || (q.off ? q.at(s) < q.at(s + 1) : q.len > 0)) continue;
+        for (int c = threadIdx.x; c < D; c += 256) to[s * D + c] = from ? from[s * D + c] : 0.f;
+    }
 }
 
 // ------------------------------------------------------------------------------------------------------- single tokens
@@ -577,27 +585,28 @@ static int scan_check(const char* who, int64_t rows, int64_t seqs, const void* o
 }
 
 struct ScanWs {
-    int64_t words, bytes;  // [16 bytes: the ticket][words, to a whole number of 16 bytes]
-    int64_t tiles;
+    int64_t words, bytes;  // [16 bytes: the ticket][words, to a whole number of 16 bytes]; enough for either direction
+    int64_t tiles, states;
 };
-static ScanWs scan_ws(int64_t rows, int64_t D) {
+static ScanWs scan_ws(int64_t rows, int64_t D, int tile_rows) {
     ScanWs w;
-    w.tiles = (rows + TR - 1) / TR;
+    w.tiles = (rows + tile_rows - 1) / tile_rows;
+    w.states = (rows + TRB - 1) / TRB * D;
     w.words = 16;
-    w.bytes = w.words + (w.tiles * D + 1) / 2 * 16;
+    w.bytes = w.words + (w.states + 1) / 2 * 16;
     return w;
 }
 
-// CALL(T, V, RW, W): V channels per lane, RW rows per wave, W waves.  Two channels a lane for 16-bit types, so that a wave
-// reads 256 bytes of a row as with one fp32 channel; odd row lengths and strides fall back to one.
-#define SCAN_BY_TYPE(dtype, vec, CALL)                                                       \
-    do {                                                                                     \
-        if ((dtype) == DVAE_F32) { CALL(float, 1, 16, 8); }                                  \
-        else if ((dtype) == DVAE_BF16) {                                                     \
-            if ((vec) == 2) { CALL(__bf16, 2, 16, 8); } else { CALL(__bf16, 1, 16, 8); }     \
-        } else {                                                                             \
-            if ((vec) == 2) { CALL(_Float16, 2, 16, 8); } else { CALL(_Float16, 1, 16, 8); } \
-        }                                                                                    \
+// CALL(T, V): V channels per lane.  Two for 16-bit types, so that a wave reads 256 bytes of a row as with one fp32 channel
+// (four: 300 us forward instead of 225 on 131072 x 1024 bf16); odd row lengths and strides fall back to one.
+#define SCAN_BY_TYPE(dtype, vec, CALL)                                        \
+    do {                                                                      \
+        if ((dtype) == DVAE_F32) { CALL(float, 1); }                          \
+        else if ((dtype) == DVAE_BF16) {                                      \
+            if ((vec) == 2) { CALL(__bf16, 2); } else { CALL(__bf16, 1); }    \
+        } else {                                                              \
+            if ((vec) == 2) { CALL(_Float16, 2); } else { CALL(_Float16, 1); } \
+        }                                                                     \
     } while (0)
 
 static int scan_begin(ScanParams& p, void* ws, const ScanWs& L, const float* from, float* to, hipStream_t s) {
@@ -619,12 +628,12 @@ static int scan_begin(ScanParams& p, void* ws, const ScanWs& L, const float* fro
 extern "C" int64_t dvae_scan_state_floats(int64_t rows, int32_t D) {
     using namespace dvae;
     DVAE_TRY(scan_check("scan_state_floats", rows, 1, nullptr, 0, D, DVAE_F32));
-    return scan_ws(rows, D).tiles * D;
+    return scan_ws(rows, D, TRB).states;
 }
 extern "C" int64_t dvae_scan_ws_bytes(int64_t rows, int32_t D) {
     using namespace dvae;
     DVAE_TRY(scan_check("scan_ws_bytes", rows, 1, nullptr, 0, D, DVAE_F32));
-    return scan_ws(rows, D).bytes;
+    return scan_ws(rows, D, TRB).bytes;
 }
 
 extern "C" int dvae_scan_fwd(const void* gate, int64_t ld_gate, const void* x, int64_t ld_x, const void* off, int32_t off_i64,
@@ -637,7 +646,7 @@ extern "C" int dvae_scan_fwd(const void* gate, int64_t ld_gate, const void* x, i
     DVAE_REQUIRE(seqs == 0 || last, "scan_fwd: null pointer");
     DVAE_REQUIRE((uintptr_t)ws % 16 == 0, "scan_fwd: the workspace must be 16-byte aligned");
     hipStream_t s = (hipStream_t)stream;
-    const ScanWs L = scan_ws(rows, D);
+    const ScanWs L = scan_ws(rows, D, TRF);
     const int vec = widest(elem_size(dtype), 4, {(int64_t)D, ld_gate, ld_x}, {gate, x, (const void*)h});
     ScanParams p = {};
     p.gate = gate; p.x = x; p.ld_gate = ld_gate; p.ld_x = ld_x; p.h = h; p.h0 = h0; p.last = last; p.states = states;
@@ -647,7 +656,7 @@ extern "C" int dvae_scan_fwd(const void* gate, int64_t ld_gate, const void* x, i
     DVAE_TRY(scan_begin(p, ws, L, h0, last, s));
     if (rows == 0) return DVAE_OK;
     const dim3 grid((unsigned)(L.tiles * p.slabs));
-#define SCAN_FWD(T, V, RW, W) hipLaunchKernelGGL((scan_fwd_kernel<T, V, RW, W>), grid, dim3(W * 64), 0, s, p)
+#define SCAN_FWD(T, V) hipLaunchKernelGGL((scan_fwd_kernel<T, V>), grid, dim3(TRF / RW * 64), 0, s, p)
     SCAN_BY_TYPE(dtype, vec, SCAN_FWD);
 #undef SCAN_FWD
     DVAE_LAUNCH_CHECK();
@@ -665,7 +674,7 @@ extern "C" int dvae_scan_bwd(const void* gate, int64_t ld_gate, const void* x, i
     DVAE_REQUIRE(rows == 0 || (gate && x && states && dgate && dx && ws), "scan_bwd: null pointer");
     DVAE_REQUIRE((uintptr_t)ws % 16 == 0, "scan_bwd: the workspace must be 16-byte aligned");
     hipStream_t s = (hipStream_t)stream;
-    const ScanWs L = scan_ws(rows, D);
+    const ScanWs L = scan_ws(rows, D, TRB);
     const int vec = widest(elem_size(dtype), 4, {(int64_t)D, ld_gate, ld_x, dh ? ld_dh : 0},
                            {gate, x, dh, (const void*)dgate, (const void*)dx});
     ScanParams p = {};
@@ -677,7 +686,7 @@ extern "C" int dvae_scan_bwd(const void* gate, int64_t ld_gate, const void* x, i
     DVAE_TRY(scan_begin(p, ws, L, dlast, dh0, s));
     if (rows == 0) return DVAE_OK;
     const dim3 grid((unsigned)(L.tiles * p.slabs));
-#define SCAN_BWD(T, V, RW, W) hipLaunchKernelGGL((scan_bwd_kernel<T, V, RW, W>), grid, dim3(W * 64), 0, s, p)
+#define SCAN_BWD(T, V) hipLaunchKernelGGL((scan_bwd_kernel<T, V>), grid, dim3(TRB / RW * 64), 0, s, p)
     SCAN_BY_TYPE(dtype, vec, SCAN_BWD);
 #undef SCAN_BWD
     DVAE_LAUNCH_CHECK();
