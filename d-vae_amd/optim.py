@@ -13,7 +13,7 @@ import torch
 
 from . import _lib
 from .dist import GradSumReducer
-from .sequence import _enqueue, _matrix, _workspace
+from .sequence import _enqueue, _matrix, _workspace, _written
 
 
 QUINTIC = (3.4445, -4.7750, 2.0315)  # p(s) = a s + b s^3 + c s^5: five steps take singular values from 0.002 up to 0.7 .. 1.2
@@ -71,7 +71,7 @@ def orthogonalize(updates, steps=5, coefficients=QUINTIC, out=None):
         ws = _workspace(lib.dvae_orthogonalize_ws_bytes(descs, len(mats), code), device, "dvae_orthogonalize_ws_bytes")
         _enqueue(device, "dvae_orthogonalize", descs, len(mats), steps, abc, ws.data_ptr(), code)
         if out is not None:
-            torch.autograd.graph.increment_version(outs)
+            _written(*outs)
     return outs[0] if one else outs
 
 

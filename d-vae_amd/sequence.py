@@ -82,6 +82,13 @@ def _workspace(n_bytes, device, what):
     return torch.empty(n_bytes, dtype=torch.uint8, device=device)
 
 
+def _written(*tensors):
+    """the library wrote into these: their autograd versions move as by an in-place operation"""
+    for t in tensors:
+        if not t.is_inference():
+            torch.autograd.graph.increment_version(t)
+
+
 def _once(name):
     if torch.is_grad_enabled():  # create_graph=True: the backward pass itself is not recorded
         raise RuntimeError("%s: the gradient is not differentiable again" % name)
@@ -253,5 +260,5 @@ def gated_step(gate, x, state, slots=None):
     h = torch.empty(B, D, dtype=x.dtype, device=dev)
     _enqueue(dev, "dvae_scan_step", g.data_ptr(), ld_g, y.data_ptr(), ld_y, state.data_ptr(), state.stride(0) if P > 1 else D, P,
              _lib.ptr(slots), _wide(slots), h.data_ptr(), B, D, code)
-    torch.autograd.graph.increment_version(state)
+    _written(state)
     return h

@@ -461,6 +461,24 @@ def test_gradients_are_not_differentiable_again():
         torch.autograd.grad(S.gated_scan(gate, gate.detach())[0].sum(), [gate], create_graph=True)
 
 
+def test_operators_in_inference_mode():
+    g = gen(40)
+    w, ids = torch.randn(5, 8, generator=g).cuda(), torch.tensor([4, 0, 9], device="cuda")
+    gate, x = torch.randn(3, 8, generator=g).cuda().requires_grad_(True), torch.randn(3, 8, generator=g).cuda()
+    off = torch.tensor([0, 1, 3], device="cuda")
+    with torch.no_grad():
+        state = torch.zeros(3, 8, device="cuda")
+        want = [S.embed(w, ids), S.gated_scan(gate, x, off)[0], S.gated_step(gate, x, state), dvae_amd.optim.orthogonalize(w, out=torch.empty_like(w))]
+    with torch.inference_mode():
+        mine = torch.zeros(3, 8, device="cuda")
+        got = [S.embed(w, ids), S.gated_scan(gate, x, off)[0], S.gated_step(gate, x, mine), dvae_amd.optim.orthogonalize(w, out=torch.empty_like(w))]
+        assert all(torch.equal(a, b) for a, b in zip(want, got)) and torch.equal(state, mine)
+    version = state._version
+    with torch.no_grad():
+        S.gated_step(gate, x, state)
+    assert state._version > version  # autograd sees that the state was written
+
+
 def test_refusals_on_the_device():
     w, ids = torch.randn(4, 8).cuda(), torch.tensor([1, 2], device="cuda")
     for bad in (lambda: S.embed(w, ids.float()), lambda: S.embed(w, ids.cpu()), lambda: S.embed(w.t(), ids), lambda: S.embed(w[:0], ids),
