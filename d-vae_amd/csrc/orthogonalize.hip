@@ -8,6 +8,8 @@
 // S = 2^13: 22 bits, with an absolute floor of 2^-38.  A product is three MFMAs, hi hi + hi lo + lo hi, accumulated in
 // fp32; the dropped lo lo is 2^-22 relative, as the planes' own rounding.  That is fp32 accuracy at 1/3 of the fp16 rate:
 // against 64 bits the result is 7e-7 off at 501 x 501 and 3e-6 at 4096 x 4096, where the same iteration in fp32 is 2.2e-6 and 5e-6.
+// With few rows the roundings average out less (8 to 16 rows: up to 1.5e-6, 1.8 times fp32's own error), so up to 64 rows, and
+// wherever the direct kernel runs, lo lo is added (up to 1.2e-6, 1.5 times); latency bounds those products and hides it.
 // G is scaled by a power of two, exactly; the rest of the division by its norm (a factor r in (1, 2]) goes into the
 // coefficients of the first step: a r, b r^3, c r^5.
 //
@@ -229,6 +231,7 @@ __global__ __launch_bounds__(128 * WN * KG) void ns_product_kernel(NsGroup p, in
     const char* b_rows = base + ns_offset(mp, np, PL, MODE == NS_GRAM ? from : MODE == NS_POLY ? 4 : from + 1) + (long)tj * TB * pitch;
     const int blocks = (int)(pitch / 128), stages = (blocks + KG - 1) / KG;
 
+    const bool all_four = m.m() <= 64;  // lo lo too
     const int col0 = tj * TB;
     const bool mirror = MODE == NS_STEP || ((MODE == NS_GRAM || MODE == NS_POLY) && ti != tj);  // a diagonal tile is its own mirror
     const char* src = base + ns_offset(mp, np, PL, MODE == NS_POLY ? 4 : from);
@@ -311,6 +314,7 @@ __global__ __launch_bounds__(128 * WN * KG) void ns_product_kernel(NsGroup p, in
                 };
                 if (mine) {
                     if (PL == 2) {
+                        if (all_four) mma(al, bl);
                         mma(al, bh);
                         mma(ah, bl);
                     }
@@ -451,6 +455,7 @@ __global__ __launch_bounds__(512) void ns_small_kernel(NsGroup p, int from, int 
             if (PL == 2) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
+                    cross = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[n][h + 2], b[n][h + 2], cross, 0, 0, 0);
                     cross = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[n][h + 2], b[n][h], cross, 0, 0, 0);
                     acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[n][h], b[n][h], acc, 0, 0, 0);
                     cross = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[n][h], b[n][h + 2], cross, 0, 0, 0);
