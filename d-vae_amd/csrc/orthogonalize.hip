@@ -50,7 +50,6 @@ typedef unsigned nsu32x4 __attribute__((ext_vector_type(4)));
 constexpr int NS_GROUP = 32;          // matrices per launch
 constexpr int NS_PARTS = 256;         // partial sums of a norm
 constexpr float NS_S = 8192.f;        // 2^13
-constexpr int NS_LDS_ROW = 128 + 16;  // bytes: a 16-lane group's fragments fall on all banks
 
 struct NsMat {
     const void* g;
@@ -202,23 +201,33 @@ template <int MODE> __device__ __forceinline__ void ns_tile_at(int t, int mt, in
     }
 }
 
+// 16 bytes per lane from memory to LDS, without a register in between: lane l's go to `lds` + 16 l.  Not the builtin: the
+// compiler would have every read of LDS wait for all of these loads; here ns_wait counts them.
+__device__ __forceinline__ void ns_load_lds(const char* from, unsigned lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 1\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(from) : "memory", "m0");
+}
+// all but the last N loads of this wave are done and its reads of LDS too; then the workgroup meets
+template <int N> __device__ __forceinline__ void ns_wait() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory"); }
+
 // One of the products, TB x TB output tiles; KG groups of waves, each with every KG-th stage of the sum; a group is 2 x WN
 // waves of TB/2 x TB/WN outputs, TM x TN MFMA blocks of 32 x 32.  A stage of the K
-// loop is one block (32 columns in two planes, 64 in one) of TB rows of either operand.  The loads run PF stages ahead in
-// registers and go to the other half of LDS in the middle of the stage before theirs.
-template <int TB, int WN, int KG, int PL, int PF, int MODE>
+// loop is one block (32 columns in two planes, 64 in one) of TB rows of either operand.  The loads run NB - 1 stages ahead,
+// into the other buffers of LDS.
+template <int TB, int WN, int KG, int PL, int NB, int MODE>
 __global__ __launch_bounds__(128 * WN * KG) void ns_product_kernel(NsGroup p, int from, int first) {
     constexpr int TM = TB / 64, TN = TB / WN / 32, NT = 128 * WN;
     constexpr int LR = NT / 8, PASSES = TB / LR;  // 16 bytes per thread and pass: LR rows of one block
-    constexpr int OPERAND = TB * NS_LDS_ROW;
+    constexpr int OPERAND = TB * 128, LOADS = 2 * PASSES;
     constexpr int TP = TB + 4;                    // row pitch of the output in LDS, floats; 64 rows at a time
-    static_assert(PF % 2 == 0 && 64 * TP * 4 <= 4 * OPERAND, "");
-    __shared__ __attribute__((aligned(16))) char lds[KG][2][2 * OPERAND];
+    // 192 does not divide the padded sides: the last tiles reach over them, read the last row instead and store nothing there
+    constexpr bool OVER = TB == 192;
+    static_assert(NB >= 2 && 64 * TP * 4 <= NB * 2 * OPERAND && LR % 16 == 0 && (!OVER || MODE == NS_GRAM || MODE == NS_POLY), "");
+    __shared__ __attribute__((aligned(128))) char lds[KG][NB][2 * OPERAND];
     const int group = __builtin_amdgcn_readfirstlane(threadIdx.x / NT), tid = threadIdx.x % NT;
     const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int k = ns_find(p, blockIdx.x);
     const NsMat& m = p.mat[k];
-    const int mp = ns_pad(m.m(), p.pad), np = ns_pad(m.n(), p.pad), mt = mp / TB, nt = np / TB;
+    const int mp = ns_pad(m.m(), p.pad), np = ns_pad(m.n(), p.pad), mt = OVER ? (mp + TB - 1) / TB : mp / TB, nt = np / TB;
     // workgroups that share an XCD (equal id mod 8) take neighbouring tiles of a matrix
     const int tiles = MODE == NS_GRAM || MODE == NS_POLY ? mt * (mt + 1) / 2 : mt * nt;
     const int local = blockIdx.x - m.tile0, q = tiles >> 3, rest = tiles & 7, xcd = local & 7;
@@ -260,76 +269,92 @@ __global__ __launch_bounds__(128 * WN * KG) void ns_product_kernel(NsGroup p, in
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
     const int wm = wave / WN, wn = wave % WN;
-    const long my = (long)(tid >> 3) * pitch + (tid & 7) * 16;
-    const int my_lds = (tid >> 3) * NS_LDS_ROW + (tid & 7) * 16;
-    nsu32x4 ra[PF][PASSES], rb[PF][PASSES];
-    auto load = [&](int u, int s) {  // past the last block the last one is loaded again and not used
-        const long at = my + (long)min(s * KG + group, blocks - 1) * 128;
+    // A wave's load writes 1 KB of LDS in the order of its lanes: 8 rows of 128 bytes.  Chunk c of row r goes to place
+    // c ^ (r / 2 mod 8), so that the 16 rows that a read of a fragment takes at a time lie on different banks.
+    const int chunk = (tid & 7) ^ (tid >> 4 & 7);
+    int at_a[PASSES], at_b[PASSES];
 #pragma unroll
-        for (int i = 0; i < PASSES; ++i) {
-            ra[u][i] = *(const nsu32x4*)(a_rows + at + i * LR * pitch);
-            rb[u][i] = *(const nsu32x4*)(b_rows + at + i * LR * pitch);
-        }
+    for (int i = 0; i < PASSES; ++i) {
+        const int row = (tid >> 3) + i * LR;
+        at_a[i] = (OVER ? min(row, mp - 1 - ti * TB) : row) * (int)pitch + chunk * 16;
+        at_b[i] = (OVER ? min(row, mp - 1 - tj * TB) : row) * (int)pitch + chunk * 16;
+    }
+    const unsigned lds0 = __builtin_amdgcn_readfirstlane((unsigned)(size_t)(__attribute__((address_space(3))) char*)&lds[group][0][wave * 1024]);
+    // one of the loads of stage s, into buffer b; past the last block the last one is loaded again and not used
+    auto load = [&](int b, int s, int n) {
+        const long block = (long)min(s * KG + group, blocks - 1) * 128;
+        if (n & 1) ns_load_lds(b_rows + block + at_b[n >> 1], lds0 + b * 2 * OPERAND + OPERAND + (n >> 1) * LR * 128);
+        else ns_load_lds(a_rows + block + at_a[n >> 1], lds0 + b * 2 * OPERAND + (n >> 1) * LR * 128);
     };
-    auto store = [&](int u, char* l) {
-#pragma unroll
-        for (int i = 0; i < PASSES; ++i) {
-            *(nsu32x4*)(l + my_lds + i * LR * NS_LDS_ROW) = ra[u][i];
-            *(nsu32x4*)(l + OPERAND + my_lds + i * LR * NS_LDS_ROW) = rb[u][i];
-        }
-    };
-#pragma unroll
-    for (int u = 0; u < PF; ++u) load(u, u);
-    store(0, lds[group][0]);
-    __syncthreads();
     // lane l of a fragment: row l & 31, columns 8 (l >> 5) .. + 7 of 16
-    const int frag = (lane & 31) * NS_LDS_ROW + (lane >> 5) * 16;
     constexpr int SUB = PL == 2 ? 2 : 4;  // 16-column steps of a stage
-    for (int s0 = 0; s0 < stages; s0 += PF) {
+    const int swizzle = lane >> 1 & 7;
+    int frag[4];  // chunk 2 n + (l >> 5) of the lane's row
 #pragma unroll
-        for (int u = 0; u < PF; ++u) {
-            const int s = s0 + u;
-            if (s >= stages) break;
-            const char* la = lds[group][u & 1] + wm * (TB / 2) * NS_LDS_ROW + frag;
-            const char* lb = lds[group][u & 1] + OPERAND + wn * (TB / WN) * NS_LDS_ROW + frag;
-            const bool mine = KG == 1 || s * KG + group < blocks;
+    for (int n = 0; n < 4; ++n) frag[n] = (lane & 31) * 128 + ((2 * n + (lane >> 5)) ^ swizzle) * 16;
+    h16x8 fa[2][PL][TM], fb[2][PL][TN];
+    auto read = [&](int to, int b, int h) {
+        const char* la = lds[group][b] + wm * (TB / 2) * 128;
+        const char* lb = lds[group][b] + OPERAND + wn * (TB / WN) * 128;
 #pragma unroll
-            for (int h = 0; h < SUB; ++h) {
-                h16x8 ah[TM], al[TM], bh[TN], bl[TN];
+        for (int q = 0; q < PL; ++q) {
+#pragma unroll
+            for (int i = 0; i < TM; ++i) fa[to][q][i] = *(const h16x8*)(la + i * 32 * 128 + frag[h + 2 * q]);
+#pragma unroll
+            for (int j = 0; j < TN; ++j) fb[to][q][j] = *(const h16x8*)(lb + j * 32 * 128 + frag[h + 2 * q]);
+        }
+    };
+    auto arrive = [&](int s) {  // the loads of stage s are done; everyone has read the fragments up to here
+        if (NB > 2 && s + NB - 2 < stages) ns_wait<(NB - 2) * LOADS>();
+        else ns_wait<0>();
+    };
+#pragma unroll
+    for (int s = 0; s < NB - 1; ++s)
+        if (s < stages)
+#pragma unroll
+            for (int n = 0; n < LOADS; ++n) load(s, s, n);
+    arrive(0);
+    read(0, 0, 0);
+    int b = 0;
+    for (int s = 0; s < stages; ++s) {
+        const int after = b + 1 == NB ? 0 : b + 1, before = b == 0 ? NB - 1 : b - 1;
+        const bool mine = KG == 1 || s * KG + group < blocks, more = s + NB - 1 < stages;
+        constexpr int PRODUCTS = PL == 2 ? 3 : 1, GROUPS = (SUB - 1) * PRODUCTS * TM, EACH = (LOADS + GROUPS - 1) / GROUPS;
+        int n = 0;
+#pragma unroll
+        for (int h = 0; h < SUB; ++h) {
+            // the next fragments are on their way while these are multiplied
+            if (h + 1 < SUB) read((h + 1) & 1, b, h + 1);
+            else if (s + 1 < stages) {
+                arrive(s + 1);
+                read(0, after, 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            auto mma = [&](int qa, int qb, int i) {
+#pragma unroll
+                for (int j = 0; j < TN; ++j)
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[h & 1][qa][i], fb[h & 1][qb][j], acc[i][j], 0, 0, 0);
+            };
+#pragma unroll
+            for (int q = 0; q < PRODUCTS; ++q)
 #pragma unroll
                 for (int i = 0; i < TM; ++i) {
-                    ah[i] = *(const h16x8*)(la + i * 32 * NS_LDS_ROW + h * 32);
-                    if (PL == 2) al[i] = *(const h16x8*)(la + i * 32 * NS_LDS_ROW + h * 32 + 64);
-                }
-#pragma unroll
-                for (int j = 0; j < TN; ++j) {
-                    bh[j] = *(const h16x8*)(lb + j * 32 * NS_LDS_ROW + h * 32);
-                    if (PL == 2) bl[j] = *(const h16x8*)(lb + j * 32 * NS_LDS_ROW + h * 32 + 64);
-                }
-                auto mma = [&](const h16x8 (&x)[TM], const h16x8 (&y)[TN]) {
-#pragma unroll
-                    for (int i = 0; i < TM; ++i)
-#pragma unroll
-                        for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[i], y[j], acc[i][j], 0, 0, 0);
-                };
-                if (mine) {
-                    if (PL == 2) {
-                        if (all_four) mma(al, bl);
-                        mma(al, bh);
-                        mma(ah, bl);
+                    if (mine) {
+                        if (PL == 2 && q == 0 && all_four) mma(PL - 1, PL - 1, i);
+                        mma(PL == 2 && q == 0, PL == 2 && q == 1, i);
                     }
-                    mma(ah, bh);
-                }
-                if (h == SUB / 2 - 1) {
-                    store((u + 1) % PF, lds[group][(u & 1) ^ 1]);
+                    // a load among the products: all at once they would hold up the wave until the memory path took them
+                    if (h + 1 < SUB) {
+#pragma unroll
+                        for (int u = 0; u < EACH; ++u, ++n)
+                            if (n < LOADS && more) load(before, s + NB - 1, n);
+                    }
                     __builtin_amdgcn_sched_barrier(0);
-                    load(u, s + PF);
-                    __builtin_amdgcn_sched_barrier(0);
                 }
-            }
-            __syncthreads();
         }
+        b = after;
     }
+    __syncthreads();
 
     // Epilogue: the output goes through LDS, one 32-row block of either wave row at a time, so that every access to memory
     // is 16 bytes of a row in either orientation; the groups' sums meet there, in their order.
@@ -338,7 +363,7 @@ __global__ __launch_bounds__(128 * WN * KG) void ns_product_kernel(NsGroup p, in
     const float from_src = MODE == NS_GRAM ? 0.f : (MODE == NS_POLY ? p.b * r * r * r : p.a * r) / NS_S;
     const float from_acc = (MODE == NS_POLY ? p.c * r * r * r * r * r : 1.f) / (NS_S * NS_S);
     float* const tile = (float*)&lds[0][0][0];
-    constexpr int GROUP_FLOATS = 4 * OPERAND / 4;
+    constexpr int GROUP_FLOATS = NB * 2 * OPERAND / 4;
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
         if (i > 0) __syncthreads();
@@ -351,6 +376,7 @@ __global__ __launch_bounds__(128 * WN * KG) void ns_product_kernel(NsGroup p, in
         __syncthreads();
         for (int u = threadIdx.x; u < 64 * TB / 8; u += NT * KG) {
             const int row = u / (TB / 8), c8 = u % (TB / 8) * 8;
+            if (OVER && (row_of(i, row) >= mp || col0 + c8 >= mp)) continue;
             const long at = (long)row_of(i, row) * row_bytes + ns_col<PL>(col0 + c8);
             float v[8];
 #pragma unroll
@@ -395,6 +421,7 @@ __global__ __launch_bounds__(128 * WN * KG) void ns_product_kernel(NsGroup p, in
             if (MODE != NS_GRAM || KG > 1) __syncthreads();
             for (int u = threadIdx.x; u < 64 * TB / 8; u += NT * KG) {
                 const int c = u / 8, r8 = u % 8 * 8;
+                if (OVER && (row_of(i, r8) >= mp || col0 + c >= mp)) continue;
                 float v[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[e] = tile[(r8 + e) * TP + c] * NS_S;
@@ -621,8 +648,9 @@ extern "C" int dvae_orthogonalize(const dvae_matrix_desc* mats, int32_t count, i
                 const int swap = order[j]; order[j] = order[j - 1]; order[j - 1] = swap;
             }
         long base = 0;
-        int split = 0, square[4] = {}, update[4] = {};  // tiles of all matrices; [b]: of 32 << b
-        int split0[NS_GROUP], square0[4][NS_GROUP], update0[4][NS_GROUP];
+        int split = 0, square[5] = {}, update[5] = {};  // tiles of all matrices, of these sides:
+        constexpr int side[5] = {32, 64, 128, 256, 192};
+        int split0[NS_GROUP], square0[5][NS_GROUP], update0[5][NS_GROUP];
         for (int i = 0; i < n; ++i) {
             const dvae_matrix_desc& d = mats[order[i]];
             NsMat& m = p.mat[i];
@@ -631,8 +659,8 @@ extern "C" int dvae_orthogonalize(const dvae_matrix_desc* mats, int32_t count, i
             const int mp = ns_pad(m.m(), p.pad), np = ns_pad(m.n(), p.pad);
             split0[i] = split;
             split += (mp / 64) * (np / 64);
-            for (int b = 0; b < 4; ++b) {
-                const int mt = mp / (32 << b), nt = np / (32 << b);
+            for (int b = 0; b < 5; ++b) {
+                const int mt = cdiv(mp, side[b]), nt = cdiv(np, side[b]);
                 square0[b][i] = square[b]; update0[b][i] = update[b];
                 square[b] += mt * (mt + 1) / 2;
                 update[b] += mt * nt;
@@ -641,7 +669,8 @@ extern "C" int dvae_orthogonalize(const dvae_matrix_desc* mats, int32_t count, i
         auto size = [&](const int* tiles) {
             return p.pad == 256 && ns_huge(tiles[3]) ? 3 : p.pad >= 128 && ns_big(tiles[2]) ? 2 : tiles[0] <= ns_cus() ? 0 : 1;
         };
-        const int sq = size(square), up = size(update);
+        int sq = size(square), up = size(update);
+        if (sq == 2 && 9 * cdiv(square[4], ns_cus()) <= 4 * cdiv(square[2], ns_cus())) sq = 4;
         auto place = [&](const int* at) { for (int i = 0; i < n; ++i) p.mat[i].tile0 = at[i]; };
         hipLaunchKernelGGL(ns_norm_kernel, dim3(NS_PARTS, n), dim3(256), 0, s, p);
         DVAE_LAUNCH_CHECK();
@@ -649,19 +678,21 @@ extern "C" int dvae_orthogonalize(const dvae_matrix_desc* mats, int32_t count, i
         if (p.planes == 2) hipLaunchKernelGGL((ns_split_kernel<2>), dim3(split), dim3(256), 0, s, p);
         else hipLaunchKernelGGL((ns_split_kernel<1>), dim3(split), dim3(256), 0, s, p);
         DVAE_LAUNCH_CHECK();
-#define NS_LAUNCH(TB, WN, KG, PL, PF, MODE, grid) \
-    hipLaunchKernelGGL((ns_product_kernel<TB, WN, KG, PL, PF, MODE>), dim3(grid), dim3(128 * WN * KG), 0, s, p, 2 * (t & 1), t == 0)
+#define NS_LAUNCH(TB, WN, KG, PL, NB, MODE, grid) \
+    hipLaunchKernelGGL((ns_product_kernel<TB, WN, KG, PL, NB, MODE>), dim3(grid), dim3(128 * WN * KG), 0, s, p, 2 * (t & 1), t == 0)
 #define NS_SMALL(PL, MODE, grid) hipLaunchKernelGGL((ns_small_kernel<PL, MODE>), dim3(grid), dim3(512), 0, s, p, 2 * (t & 1), t == 0)
 #define NS_PRODUCT(MODE, size, grid)                                                      \
     do {                                                                                  \
         if (p.planes == 2) {                                                              \
             if (size == 3) NS_LAUNCH(256, 4, 1, 2, 2, MODE, grid);                        \
+            else if (size == 4) NS_LAUNCH((MODE == NS_GRAM || MODE == NS_POLY ? 192 : 128), 2, 1, 2, (MODE == NS_GRAM || MODE == NS_POLY ? 3 : 2), MODE, grid); \
             else if (size == 2) NS_LAUNCH(128, 2, 1, 2, 2, MODE, grid);                   \
             else if (size == 0) NS_SMALL(2, MODE, grid);                                  \
             else if (grid <= ns_cus()) NS_LAUNCH(64, 2, 4, 2, 2, MODE, grid);             \
             else NS_LAUNCH(64, 2, 1, 2, 4, MODE, grid);                                   \
         } else {                                                                          \
             if (size == 3) NS_LAUNCH(256, 4, 1, 1, 2, MODE, grid);                        \
+            else if (size == 4) NS_LAUNCH((MODE == NS_GRAM || MODE == NS_POLY ? 192 : 128), 2, 1, 1, (MODE == NS_GRAM || MODE == NS_POLY ? 3 : 2), MODE, grid); \
             else if (size == 2) NS_LAUNCH(128, 2, 1, 1, 2, MODE, grid);                   \
             else if (size == 0) NS_SMALL(1, MODE, grid);                                  \
             else if (grid <= ns_cus()) NS_LAUNCH(64, 2, 4, 1, 2, MODE, grid);             \
