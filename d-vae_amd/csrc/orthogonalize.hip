@@ -26,12 +26,17 @@
 // symmetric), B X against the rows of X^T, which is kept beside X: an output tile is written in both orientations.  The
 // two symmetric products compute the tiles on and above the diagonal alone and write each also mirrored.
 //
-// Tiles.  A stage of a 128 x 128 tile in two planes has 24 MFMAs (768 cycles) a wave for 96 KB through LDS (750 cycles): both
-// ends meet.  In one plane LDS would lead (750 to 512), which 256 x 256 tiles even out (2000 to 2048) where they fill whole
-// rounds of the chip: the update product at 4096 x 4096 190 -> 155 us (0.89 PFLOP/s); in two planes a whole call 5.03 -> 4.82 ms
-// (0.86 PFLOP/s of MFMA work).  Fewer tiles than 1.25 per CU take 64 x 64 (the products X X^T of the ENAS model: 60 -> 33 us); at most one
-// 64 x 64 tile per CU, four groups of waves share the sum (1024 x 1024: 217 us a call); at most one 32 x 32 tile per CU, the
-// direct kernel (501 x 501: 155 -> 131 us a call, 256 x 256: 118 -> 96; 768 x 768 would lose: 189 -> 232).
+// Tiles.  The operands go straight from memory to LDS, several stages ahead.  Two things bound the products: what a CU can take
+// in (17 to 21 bytes a cycle measured with all of them loading, whatever the depth; loads alone are 28 of the 29 us of the
+// ENAS model's products X X^T and 35 of its update's 41), and with large tiles the power: the clock is 2.0 GHz where loads and
+// MFMAs run together, 2.5 with either alone.  So a product takes the largest tile that still keeps the CUs busy:
+//   256 x 256, one workgroup per CU, where the last round of them is nearly full: update at 4096 x 4096 bf16 142 us (0.97 PFLOP/s)
+//   192 x 192 for symmetric products where their rounds cover less area than those of 128 x 128: 253 tiles are one round at
+//     4096 x 4096 (78 us), 528 of 128 x 128 two and a bit (120 us)
+//   128 x 128 from 3/4 of a tile per CU on (3000 x 3000 bf16: 1130 -> 990 us a call against 64 x 64; from 1/2 on the ENAS set
+//     would lose: 537 -> 677)
+//   64 x 64; at most one per CU: four groups of waves share the sum (1024 x 1024: 242 us a call)
+//   32 x 32, at most one per CU: the direct kernel (501 x 501: 155 -> 128 us a call; 768 x 768 would lose: 211 -> 232)
 //
 // Launches.  The matrices of a call go through each product together, one grid over all their tiles: an optimiser step on a
 // model's many small matrices is 17 launches, whatever their number (up to 32 per group).
@@ -45,7 +50,7 @@ namespace dvae {
 typedef _Float16 h16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h16x4 __attribute__((ext_vector_type(4)));
 typedef float nsf32x16 __attribute__((ext_vector_type(16)));
-typedef unsigned nsu32x4 __attribute__((ext_vector_type(4)));
+typedef float nsf32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int NS_GROUP = 32;          // matrices per launch
 constexpr int NS_PARTS = 256;         // partial sums of a norm
@@ -87,17 +92,27 @@ __device__ __forceinline__ int ns_find(const NsGroup& p, int unit) {
     return k;
 }
 
-template <typename T> __device__ __forceinline__ void ns_sum(const NsMat& m, double* out) {
-    // NS_PARTS workgroups: as many rows each as there are, and where there are few, shares of the columns
-    const int across = m.rows >= NS_PARTS ? 1 : NS_PARTS / m.rows, down = NS_PARTS / across;
-    const int r0 = blockIdx.x / across, c0 = blockIdx.x % across;
+template <typename T, int V> __device__ __forceinline__ void ns_sum(const NsMat& m, double* out) {
+    typedef T vec __attribute__((ext_vector_type(V)));
+    // NS_PARTS x 4 waves: as many rows each as there are, and where there are few, shares of the columns
+    constexpr int WAVES = NS_PARTS * 4, STEP = 64 * V;
+    const int across = m.rows >= WAVES ? 1 : WAVES / m.rows, down = WAVES / across;
+    const int wave = blockIdx.x * 4 + (threadIdx.x >> 6), r0 = wave / across, c0 = wave % across * STEP + (threadIdx.x & 63) * V;
     double s = 0;
     if (r0 < down)
         for (int r = r0; r < m.rows; r += down) {
             const T* row = (const T*)m.g + r * m.ld_g;
-            for (int c = c0 * 256 + threadIdx.x; c < m.cols; c += across * 256) {
-                const double v = (double)(float)row[c];
-                s += v * v;
+            for (int c = c0; c < m.cols; c += 4 * across * STEP) {  // four loads under way
+                vec v[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const int at = c + u * across * STEP;
+                    v[u] = at < m.cols ? *(const vec*)(row + at) : vec{};
+                }
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+#pragma unroll
+                    for (int e = 0; e < V; ++e) s += (double)(float)v[u][e] * (double)(float)v[u][e];
             }
         }
 #pragma unroll
@@ -106,6 +121,12 @@ template <typename T> __device__ __forceinline__ void ns_sum(const NsMat& m, dou
     if ((threadIdx.x & 63) == 0) w[threadIdx.x >> 6] = s;
     __syncthreads();
     if (threadIdx.x == 0) *out = w[0] + w[1] + w[2] + w[3];
+}
+// 16 bytes a load where all rows allow it
+template <typename T> __device__ __forceinline__ void ns_sum(const NsMat& m, double* out) {
+    constexpr int V = 16 / sizeof(T);
+    if (((size_t)m.g | m.ld_g * sizeof(T)) % 16 == 0 && m.cols % V == 0) ns_sum<T, V>(m, out);
+    else ns_sum<T, 1>(m, out);
 }
 // |G|_F^2 in 64 bits: no range of G overflows or vanishes
 __global__ __launch_bounds__(256) void ns_norm_kernel(NsGroup p) {
@@ -209,10 +230,35 @@ __device__ __forceinline__ void ns_load_lds(const char* from, unsigned lds) {
 // all but the last N loads of this wave are done and its reads of LDS too; then the workgroup meets
 template <int N> __device__ __forceinline__ void ns_wait() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory"); }
 
+// eight neighbours of a row of the result, rounded to its type
+__device__ __forceinline__ void ns_out8(const NsMat& m, int dtype, int row, int col, const float (&v)[8]) {
+    if (row >= m.rows || col >= m.cols) return;
+    const int n = min(8, m.cols - col);
+    char* at = (char*)m.out + (row * m.ld_out + col) * (dtype == DVAE_F32 ? 4 : 2);
+    const bool whole = n == 8 && (size_t)at % 16 == 0;
+    if (dtype == DVAE_F32) {
+        if (whole) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) *(nsf32x4*)(at + 16 * h) = nsf32x4{v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3]};
+        } else
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (e < n) ((float*)at)[e] = v[e];
+        return;
+    }
+    h16x8 bits;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) bits[e] = dtype == DVAE_BF16 ? __builtin_bit_cast(_Float16, (__bf16)v[e]) : (_Float16)v[e];
+    if (whole) *(h16x8*)at = bits;
+    else
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (e < n) ((_Float16*)at)[e] = bits[e];
+}
+
 // One of the products, TB x TB output tiles; KG groups of waves, each with every KG-th stage of the sum; a group is 2 x WN
-// waves of TB/2 x TB/WN outputs, TM x TN MFMA blocks of 32 x 32.  A stage of the K
-// loop is one block (32 columns in two planes, 64 in one) of TB rows of either operand.  The loads run NB - 1 stages ahead,
-// into the other buffers of LDS.
+// waves of TB/2 x TB/WN outputs, TM x TN MFMA blocks of 32 x 32.  A stage of the sum is one block (32 columns in two planes,
+// 64 in one) of TB rows of either operand; NB stages have room in LDS, the loads of all but the current one are under way.
 template <int TB, int WN, int KG, int PL, int NB, int MODE>
 __global__ __launch_bounds__(128 * WN * KG) void ns_product_kernel(NsGroup p, int from, int first) {
     constexpr int TM = TB / 64, TN = TB / WN / 32, NT = 128 * WN;
@@ -221,8 +267,9 @@ __global__ __launch_bounds__(128 * WN * KG) void ns_product_kernel(NsGroup p, in
     constexpr int TP = TB + 4;                    // row pitch of the output in LDS, floats; 64 rows at a time
     // 192 does not divide the padded sides: the last tiles reach over them, read the last row instead and store nothing there
     constexpr bool OVER = TB == 192;
-    static_assert(NB >= 2 && 64 * TP * 4 <= NB * 2 * OPERAND && LR % 16 == 0 && (!OVER || MODE == NS_GRAM || MODE == NS_POLY), "");
-    __shared__ __attribute__((aligned(128))) char lds[KG][NB][2 * OPERAND];
+    static_assert(NB >= 2 && 64 * TP * 4 <= NB * 2 * OPERAND && LR % 16 == 0 && (KG == 1 || TM == 1) && (!OVER || MODE == NS_GRAM || MODE == NS_POLY), "");
+    constexpr int STAGED = KG * NB * 2 * OPERAND, OUT = (TM > 1 ? 2 : 1) * 64 * TP * 4;  // bytes: KG x NB stages; two blocks of the output
+    __shared__ __attribute__((aligned(128))) char lds[STAGED > OUT ? STAGED : OUT];
     const int group = __builtin_amdgcn_readfirstlane(threadIdx.x / NT), tid = threadIdx.x % NT;
     const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int k = ns_find(p, blockIdx.x);
@@ -247,19 +294,26 @@ __global__ __launch_bounds__(128 * WN * KG) void ns_product_kernel(NsGroup p, in
     char* dst = base + ns_offset(mp, np, PL, MODE == NS_GRAM ? 4 : MODE == NS_POLY ? 5 : from ^ 2);
     char* turned = base + ns_offset(mp, np, PL, MODE == NS_GRAM ? 4 : MODE == NS_POLY ? 5 : (from ^ 2) + 1);
     constexpr bool CARRY = PL == 1 && (MODE == NS_STEP || MODE == NS_LAST);  // X's second plane goes through the epilogue alone
-    const char* src_lo = base + ns_offset(mp, np, PL, 6 + from / 2);
+    const char* src_lo_plane = base + ns_offset(mp, np, PL, 6 + from / 2);
     char* dst_lo = base + ns_offset(mp, np, PL, 6 + (from ^ 2) / 2);
     const long row_bytes = (long)(MODE == NS_STEP || MODE == NS_LAST ? np : mp) * 2 * PL;
     auto row_of = [&](int i, int row) { return ti * TB + (row >> 5) * (TB / 2) + i * 32 + (row & 31); };
-    // with one output per thread (the small products, where latency counts) the source is under way from the start
-    constexpr bool EARLY = MODE != NS_GRAM && TM == 1 && 64 * TB / 8 <= NT * KG;
-    h16x8 early_hi = {}, early_lo = {};
-    if (EARLY && threadIdx.x < 64 * TB / 8) {
-        const char* at = src + (long)row_of(0, threadIdx.x / (TB / 8)) * row_bytes + ns_col<PL>(col0 + threadIdx.x % (TB / 8) * 8);
-        early_hi = *(const h16x8*)at;
-        if (PL == 2) early_lo = *(const h16x8*)(at + 64);
-        if (CARRY) early_lo = *(const h16x8*)(src_lo + (at - src));
-    }
+    // The source of the added multiple for block row i, a thread's n-th eight values, is read ahead: for the first one from
+    // the start (64 x 64) or during the last stage, for the others while the one before is written.
+    constexpr int UNITS = (64 * TB / 8 + NT * KG - 1) / (NT * KG);
+    constexpr bool FROM_START = TB == 64, FROM_LAST = !FROM_START && !(TB == 256 && PL == 2);  // (there no registers are left)
+    h16x8 src_hi[UNITS], src_lo[UNITS];
+    auto fetch = [&](int i, int n) {
+        const int u = min((int)threadIdx.x + n * NT * KG, 64 * TB / 8 - 1), row = row_of(i, u / (TB / 8)), c = col0 + u % (TB / 8) * 8;
+        const char* at = src + (long)(OVER ? min(row, mp - 1) : row) * row_bytes + ns_col<PL>(OVER ? min(c, mp - 8) : c);
+        src_hi[n] = *(const h16x8*)at;
+        if (PL == 2) src_lo[n] = *(const h16x8*)(at + 64);
+        else if (CARRY) src_lo[n] = *(const h16x8*)(src_lo_plane + (at - src));
+        else src_lo[n] = h16x8{};
+    };
+    if (MODE != NS_GRAM && FROM_START)
+#pragma unroll
+        for (int n = 0; n < UNITS; ++n) fetch(0, n);
 
     nsf32x16 acc[TM][TN];
 #pragma unroll
@@ -279,7 +333,7 @@ __global__ __launch_bounds__(128 * WN * KG) void ns_product_kernel(NsGroup p, in
         at_a[i] = (OVER ? min(row, mp - 1 - ti * TB) : row) * (int)pitch + chunk * 16;
         at_b[i] = (OVER ? min(row, mp - 1 - tj * TB) : row) * (int)pitch + chunk * 16;
     }
-    const unsigned lds0 = __builtin_amdgcn_readfirstlane((unsigned)(size_t)(__attribute__((address_space(3))) char*)&lds[group][0][wave * 1024]);
+    const unsigned lds0 = __builtin_amdgcn_readfirstlane((unsigned)(size_t)(__attribute__((address_space(3))) char*)(lds + group * NB * 2 * OPERAND + wave * 1024));
     // one of the loads of stage s, into buffer b; past the last block the last one is loaded again and not used
     auto load = [&](int b, int s, int n) {
         const long block = (long)min(s * KG + group, blocks - 1) * 128;
@@ -292,10 +346,13 @@ __global__ __launch_bounds__(128 * WN * KG) void ns_product_kernel(NsGroup p, in
     int frag[4];  // chunk 2 n + (l >> 5) of the lane's row
 #pragma unroll
     for (int n = 0; n < 4; ++n) frag[n] = (lane & 31) * 128 + ((2 * n + (lane >> 5)) ^ swizzle) * 16;
+    // PIPED: a fragment is read while the one before is multiplied, and a stage's loads are issued among the products: all
+    // at once they would hold up the wave until the memory path has taken them.  Two workgroups per CU do that for each other.
+    constexpr bool PIPED = TB != 128 && KG == 1 && !(TB == 256 && PL == 2);  // (nor are there registers for it in the latter)
     h16x8 fa[2][PL][TM], fb[2][PL][TN];
     auto read = [&](int to, int b, int h) {
-        const char* la = lds[group][b] + wm * (TB / 2) * 128;
-        const char* lb = lds[group][b] + OPERAND + wn * (TB / WN) * 128;
+        const char* la = (char*)lds + (group * NB + b) * 2 * OPERAND + wm * (TB / 2) * 128;
+        const char* lb = (char*)lds + (group * NB + b) * 2 * OPERAND + OPERAND + wn * (TB / WN) * 128;
 #pragma unroll
         for (int q = 0; q < PL; ++q) {
 #pragma unroll
@@ -304,7 +361,7 @@ __global__ __launch_bounds__(128 * WN * KG) void ns_product_kernel(NsGroup p, in
             for (int j = 0; j < TN; ++j) fb[to][q][j] = *(const h16x8*)(lb + j * 32 * 128 + frag[h + 2 * q]);
         }
     };
-    auto arrive = [&](int s) {  // the loads of stage s are done; everyone has read the fragments up to here
+    auto arrive = [&](int s) {  // the loads of stage s are done, everywhere; all fragments asked for so far are read
         if (NB > 2 && s + NB - 2 < stages) ns_wait<(NB - 2) * LOADS>();
         else ns_wait<0>();
     };
@@ -313,23 +370,34 @@ __global__ __launch_bounds__(128 * WN * KG) void ns_product_kernel(NsGroup p, in
         if (s < stages)
 #pragma unroll
             for (int n = 0; n < LOADS; ++n) load(s, s, n);
-    arrive(0);
-    read(0, 0, 0);
+    if (PIPED) {
+        arrive(0);
+        read(0, 0, 0);
+    }
     int b = 0;
     for (int s = 0; s < stages; ++s) {
         const int after = b + 1 == NB ? 0 : b + 1, before = b == 0 ? NB - 1 : b - 1;
         const bool mine = KG == 1 || s * KG + group < blocks, more = s + NB - 1 < stages;
         constexpr int PRODUCTS = PL == 2 ? 3 : 1, GROUPS = (SUB - 1) * PRODUCTS * TM, EACH = (LOADS + GROUPS - 1) / GROUPS;
+        if (!PIPED) {
+            arrive(s);
+            if (more)
+#pragma unroll
+                for (int n = 0; n < LOADS; ++n) load(before, s + NB - 1, n);
+        }
+        if (MODE != NS_GRAM && FROM_LAST && s + 1 == stages)
+#pragma unroll
+            for (int n = 0; n < UNITS; ++n) fetch(0, n);
         int n = 0;
 #pragma unroll
         for (int h = 0; h < SUB; ++h) {
-            // the next fragments are on their way while these are multiplied
-            if (h + 1 < SUB) read((h + 1) & 1, b, h + 1);
+            if (!PIPED) read(h & 1, b, h);
+            else if (h + 1 < SUB) read((h + 1) & 1, b, h + 1);
             else if (s + 1 < stages) {
                 arrive(s + 1);
                 read(0, after, 0);
             }
-            __builtin_amdgcn_sched_barrier(0);
+            if (PIPED) __builtin_amdgcn_sched_barrier(0);
             auto mma = [&](int qa, int qb, int i) {
 #pragma unroll
                 for (int j = 0; j < TN; ++j)
@@ -343,89 +411,81 @@ __global__ __launch_bounds__(128 * WN * KG) void ns_product_kernel(NsGroup p, in
                         if (PL == 2 && q == 0 && all_four) mma(PL - 1, PL - 1, i);
                         mma(PL == 2 && q == 0, PL == 2 && q == 1, i);
                     }
-                    // a load among the products: all at once they would hold up the wave until the memory path took them
-                    if (h + 1 < SUB) {
+                    if (PIPED) {
+                        if (h + 1 < SUB)
 #pragma unroll
-                        for (int u = 0; u < EACH; ++u, ++n)
-                            if (n < LOADS && more) load(before, s + NB - 1, n);
+                            for (int u = 0; u < EACH; ++u, ++n)
+                                if (n < LOADS && more) load(before, s + NB - 1, n);
+                        __builtin_amdgcn_sched_barrier(0);
                     }
-                    __builtin_amdgcn_sched_barrier(0);
                 }
         }
         b = after;
     }
+    if (MODE != NS_GRAM && !FROM_START && !FROM_LAST)
+#pragma unroll
+        for (int n = 0; n < UNITS; ++n) fetch(0, n);
     __syncthreads();
 
     // Epilogue: the output goes through LDS, one 32-row block of either wave row at a time, so that every access to memory
-    // is 16 bytes of a row in either orientation; the groups' sums meet there, in their order.
+    // is 16 bytes of a row in either orientation; the groups' sums meet there, in their order.  Column c of row q stands at
+    // c ^ 8 (q / 8 mod 8): rows are read 8 columns at a time and columns 8 rows at a time, both from all banks.
     // Lane l of an MFMA block holds column l & 31 and rows (r & 3) + 8 (r >> 2) + 4 (l >> 5).
     const float r = first ? p.r[k] : 1.f;
     const float from_src = MODE == NS_GRAM ? 0.f : (MODE == NS_POLY ? p.b * r * r * r : p.a * r) / NS_S;
     const float from_acc = (MODE == NS_POLY ? p.c * r * r * r * r * r : 1.f) / (NS_S * NS_S);
-    float* const tile = (float*)&lds[0][0][0];
+    const bool wide = m.rows <= m.cols;  // else the rows of out are the columns of X
+    auto place = [](int row, int c) { return row * TP + (c ^ (row & 56)); };
     constexpr int GROUP_FLOATS = NB * 2 * OPERAND / 4;
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
-        if (i > 0) __syncthreads();
+        float* const tile = (float*)lds + (i & 1) * 64 * TP;
 #pragma unroll
         for (int j = 0; j < TN; ++j)
 #pragma unroll
             for (int e = 0; e < 16; ++e)
-                tile[group * GROUP_FLOATS + (wm * 32 + (e & 3) + 8 * (e >> 2) + 4 * (lane >> 5)) * TP + wn * (TB / WN) + j * 32 + (lane & 31)] =
+                tile[group * GROUP_FLOATS + place(wm * 32 + (e & 3) + 8 * (e >> 2) + 4 * (lane >> 5), wn * (TB / WN) + j * 32 + (lane & 31))] =
                     acc[i][j][e] * from_acc;
         __syncthreads();
-        for (int u = threadIdx.x; u < 64 * TB / 8; u += NT * KG) {
-            const int row = u / (TB / 8), c8 = u % (TB / 8) * 8;
+#pragma unroll
+        for (int n = 0; n < UNITS; ++n) {
+            const int u = threadIdx.x + n * NT * KG, row = u / (TB / 8), c8 = u % (TB / 8) * 8;
+            if (64 * TB / 8 % (NT * KG) && u >= 64 * TB / 8) break;
             if (OVER && (row_of(i, row) >= mp || col0 + c8 >= mp)) continue;
             const long at = (long)row_of(i, row) * row_bytes + ns_col<PL>(col0 + c8);
             float v[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                v[e] = tile[row * TP + c8 + e];
+                v[e] = tile[place(row, c8) + e];
 #pragma unroll
-                for (int g = 1; g < KG; ++g) v[e] += tile[g * GROUP_FLOATS + row * TP + c8 + e];
+                for (int g = 1; g < KG; ++g) v[e] += tile[g * GROUP_FLOATS + place(row, c8) + e];
             }
             if (MODE != NS_GRAM) {
-                h16x8 hi = early_hi, lo = early_lo;
-                if (!EARLY) {
-                    hi = *(const h16x8*)(src + at);
-                    if (PL == 2) lo = *(const h16x8*)(src + at + 64);
-                    if (CARRY) lo = *(const h16x8*)(src_lo + at);
-                }
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = fmaf((float)hi[e] + (float)lo[e], from_src, v[e]);
+                for (int e = 0; e < 8; ++e) v[e] = fmaf((float)src_hi[n][e] + (float)src_lo[n][e], from_src, v[e]);
+                if (i + 1 < TM) fetch(i + 1, n);
             }
-            if ((MODE != NS_GRAM || KG > 1) && (MODE == NS_LAST || mirror))
+            if ((MODE != NS_GRAM || KG > 1) && (MODE == NS_LAST ? !wide : mirror))
 #pragma unroll
-                for (int e = 0; e < 8; ++e) tile[row * TP + c8 + e] = v[e];
+                for (int e = 0; e < 8; ++e) tile[place(row, c8) + e] = v[e];
             if (MODE != NS_LAST) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[e] *= NS_S;
                 ns_put8<PL>(dst + at, v, CARRY ? dst_lo + at : nullptr);
-            }
+            } else if (wide) ns_out8(m, p.dtype, row_of(i, row), col0 + c8, v);
         }
-        if (MODE == NS_LAST) {
-            __syncthreads();
-            const bool wide = m.rows <= m.cols;  // else the rows of out are the columns of X
-            for (int u = threadIdx.x; u < 64 * TB; u += NT * KG) {
-                const int row = wide ? u / TB : u % 64, c = wide ? u % TB : u / 64;
-                const int gr = row_of(i, row), gc = col0 + c;
-                if (gr >= m.m() || gc >= m.n()) continue;
-                const float v = tile[row * TP + c];
-                const long o = wide ? gr * m.ld_out + gc : gc * m.ld_out + gr;
-                if (p.dtype == DVAE_F32) ((float*)m.out)[o] = v;
-                else if (p.dtype == DVAE_BF16) ((__bf16*)m.out)[o] = (__bf16)v;
-                else ((_Float16*)m.out)[o] = (_Float16)v;
-            }
-        } else if (mirror) {
+        if (MODE == NS_LAST ? !wide : mirror) {
             if (MODE != NS_GRAM || KG > 1) __syncthreads();
-            for (int u = threadIdx.x; u < 64 * TB / 8; u += NT * KG) {
-                const int c = u / 8, r8 = u % 8 * 8;
+#pragma unroll
+            for (int n = 0; n < UNITS; ++n) {
+                const int u = threadIdx.x + n * NT * KG, c = u / 8, r8 = u % 8 * 8;
+                if (64 * TB / 8 % (NT * KG) && u >= 64 * TB / 8) break;
                 if (OVER && (row_of(i, r8) >= mp || col0 + c >= mp)) continue;
                 float v[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = tile[(r8 + e) * TP + c] * NS_S;
-                ns_put8<PL>(turned + (long)(col0 + c) * mp * 2 * PL + ns_col<PL>(row_of(i, r8)), v);
+                for (int e = 0; e < 8; ++e) v[e] = tile[place(r8 + e, c)] * (MODE == NS_LAST ? 1.f : NS_S);
+                if (MODE == NS_LAST) ns_out8(m, p.dtype, col0 + c, row_of(i, r8), v);
+                else ns_put8<PL>(turned + (long)(col0 + c) * mp * 2 * PL + ns_col<PL>(row_of(i, r8)), v);
             }
         }
     }
@@ -547,22 +607,24 @@ static int ns_cus() {
     return cus;
 }
 
-// A product runs on 128 x 128 tiles where those fill the chip one and a quarter times, else on 64 x 64.
-static bool ns_big(long tiles128) { return 4 * tiles128 >= 5L * ns_cus(); }
+// A product runs on 128 x 128 tiles from 3/4 of one per CU on, else on 64 x 64.
+static bool ns_big(long tiles128) { return 4 * tiles128 >= 3L * ns_cus(); }
 // 256 x 256 tiles, one workgroup per CU, where the last round of them is nearly full.
 static bool ns_huge(long tiles256) {
     const long rounds = (tiles256 + ns_cus() - 1) / ns_cus();
     return 8 * tiles256 >= 7 * rounds * ns_cus();
 }
-// what the sides are padded to: the largest tile that any product takes; 256 only where that adds little to the work
+// what the sides are padded to: the largest tile that any product takes, where that adds at most an eighth to the work (eight
+// 700 x 700: 449 us a call on 64 x 64, 514 on 128 x 128)
 static int ns_pad_of(const dvae_matrix_desc* d, int32_t count) {
-    long big = 0, huge = 0;
+    long small = 0, big = 0, huge = 0;
     for (int i = 0; i < count; ++i) {
+        small += (long)cdiv(d[i].rows, 64) * cdiv(d[i].cols, 64);
         big += (long)cdiv(d[i].rows, 128) * cdiv(d[i].cols, 128);
         huge += (long)cdiv(d[i].rows, 256) * cdiv(d[i].cols, 256);
     }
     if (ns_huge(huge) && 32 * huge <= 9 * big) return 256;
-    return ns_big(big) ? 128 : 64;
+    return ns_big(big) && 32 * big <= 9 * small ? 128 : 64;
 }
 static long ns_matrix_bytes(const dvae_matrix_desc& d, int pad, int planes) {
     const int mp = ns_pad(d.rows < d.cols ? d.rows : d.cols, pad), np = ns_pad(d.rows < d.cols ? d.cols : d.rows, pad);
@@ -670,6 +732,7 @@ extern "C" int dvae_orthogonalize(const dvae_matrix_desc* mats, int32_t count, i
             return p.pad == 256 && ns_huge(tiles[3]) ? 3 : p.pad >= 128 && ns_big(tiles[2]) ? 2 : tiles[0] <= ns_cus() ? 0 : 1;
         };
         int sq = size(square), up = size(update);
+        // a round of 192 x 192 tiles is 9/4 of one of 128 x 128
         if (sq == 2 && 9 * cdiv(square[4], ns_cus()) <= 4 * cdiv(square[2], ns_cus())) sq = 4;
         auto place = [&](const int* at) { for (int i = 0; i < n; ++i) p.mat[i].tile0 = at[i]; };
         hipLaunchKernelGGL(ns_norm_kernel, dim3(NS_PARTS, n), dim3(256), 0, s, p);
@@ -689,14 +752,14 @@ extern "C" int dvae_orthogonalize(const dvae_matrix_desc* mats, int32_t count, i
             else if (size == 2) NS_LAUNCH(128, 2, 1, 2, 2, MODE, grid);                   \
             else if (size == 0) NS_SMALL(2, MODE, grid);                                  \
             else if (grid <= ns_cus()) NS_LAUNCH(64, 2, 4, 2, 2, MODE, grid);             \
-            else NS_LAUNCH(64, 2, 1, 2, 4, MODE, grid);                                   \
+            else NS_LAUNCH(64, 2, 1, 2, 3, MODE, grid);                                   \
         } else {                                                                          \
             if (size == 3) NS_LAUNCH(256, 4, 1, 1, 2, MODE, grid);                        \
             else if (size == 4) NS_LAUNCH((MODE == NS_GRAM || MODE == NS_POLY ? 192 : 128), 2, 1, 1, (MODE == NS_GRAM || MODE == NS_POLY ? 3 : 2), MODE, grid); \
             else if (size == 2) NS_LAUNCH(128, 2, 1, 1, 2, MODE, grid);                   \
             else if (size == 0) NS_SMALL(1, MODE, grid);                                  \
             else if (grid <= ns_cus()) NS_LAUNCH(64, 2, 4, 1, 2, MODE, grid);             \
-            else NS_LAUNCH(64, 2, 1, 1, 4, MODE, grid);                                   \
+            else NS_LAUNCH(64, 2, 1, 1, 3, MODE, grid);                                   \
         }                                                                                 \
         DVAE_LAUNCH_CHECK();                                                              \
     } while (0)
