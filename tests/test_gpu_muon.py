@@ -127,6 +127,24 @@ def test_orthogonalize_strides_and_outputs():
     assert torch.equal(mine[0], want[0])
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("shape", [(700, 901), (901, 700), (1500, 1300), (2600, 2801), (2801, 2600), (4001, 3901)])
+def test_orthogonalize_rows_at_any_address(shape, dtype):
+    """wide and tall, on every size of tile: rows of the result and of the input that begin at no multiple of 16 bytes"""
+    m, n = shape
+    g = torch.randn(m, n, device="cuda", generator=torch.Generator(device="cuda").manual_seed(7)).to(DT[dtype])
+    want = O.orthogonalize(g)
+    hole = torch.zeros(m + 2, n + 5, device="cuda", dtype=g.dtype)
+    O.orthogonalize(g, out=hole[1:m + 1, 3:n + 3])
+    assert torch.equal(hole[1:m + 1, 3:n + 3], want)
+    hole[1:m + 1, 3:n + 3] = 0
+    assert not hole.any()  # nothing beside it was written
+    hole[1:m + 1, 3:n + 3] = g
+    got = O.orthogonalize(hole[1:m + 1, 3:n + 3])
+    # the norm is summed in another order: 2^-24 of a factor, which moves an entry of X by as much, and its rounding by a step
+    assert float((got.double() - want.double()).norm() / want.double().norm()) < 341 * 16 * 2.0 ** -22 + torch.finfo(g.dtype).eps
+
+
 def test_orthogonalize_captured_and_replayed():
     g = gen(5)
     mats = [torch.randn(s, generator=g).cuda() for s in ((130, 70), (200, 200), (3, 50))]
