@@ -5,6 +5,7 @@ object is missing, or a compute entry point is called without a HIP device, the
 call fails loudly.
 """
 import ctypes as C
+import importlib.util
 import os
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -153,6 +154,25 @@ def load():
         fn.argtypes = args
     _lib = lib
     return lib
+
+
+def load_sequence_ops():
+    """The host side of the sequence operators (csrc/sequence_ops.cpp), bound to the functions of this library."""
+    path = os.path.join(HERE, "csrc", "_dvae_sequence.so")
+    if not os.path.exists(path):
+        raise DvaeHipError(
+            "%s is missing. Run `python -c 'import __graft_entry__ as g; g.build()'` or `make -C d-vae_amd/csrc`. "
+            "There is no fallback." % path)
+    import torch  # noqa: F401  (the module uses its libraries)
+    lib = load()
+    try:
+        spec = importlib.util.spec_from_file_location("_dvae_sequence", path)
+        ops = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(ops)
+    except ImportError as e:
+        raise DvaeHipError("cannot load %s: %s" % (path, e))
+    ops.bind({name: C.cast(getattr(lib, name), C.c_void_p).value for name in ops.functions}, DvaeHipError)
+    return ops
 
 
 def check(rc, what=""):

@@ -1,0 +1,212 @@
+// The host side of the sequence operators (sequence.py) in C++: outputs and workspaces, the launch on the current stream and
+// the autograd nodes.  This bounds small calls: through ctypes and Python autograd functions a lookup of 256 tokens took 8.7 us,
+// a single-token step 8.8, a lookup of 8192 with its gradient 85 and a short scan with its gradient 111 (kernels 3, 3, 30
+// and 29 us); from here 4.9, 5.3, 51 and 62, of which 42 are what torch takes to run any function's gradient.
+// The arguments are checked in sequence.py; the kernels and their C-ABI are in libdvae_hip.so, whose functions bind() gets.
+#include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/utils/pybind.h>
+
+#include <stdexcept>
+
+#include "dvae_hip.h"
+
+namespace {
+
+using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+typedef std::optional<Tensor> Maybe;
+
+struct DvaeError : std::runtime_error {  // DvaeHipError in Python
+    using std::runtime_error::runtime_error;
+};
+
+#define DVAE_FUNCTIONS(F)                                                                                                     \
+    F(dvae_last_error) F(dvae_embed_fwd) F(dvae_embed_bwd_ws_bytes) F(dvae_embed_bwd) F(dvae_scan_state_floats) F(dvae_scan_ws_bytes) \
+    F(dvae_scan_fwd) F(dvae_scan_bwd) F(dvae_scan_step)
+#define F(name) decltype(&::name) p_##name = nullptr;
+DVAE_FUNCTIONS(F)
+#undef F
+
+void bind(const std::map<std::string, size_t>& addresses) {
+#define F(name) p_##name = reinterpret_cast<decltype(p_##name)>(addresses.at(#name));
+    DVAE_FUNCTIONS(F)
+#undef F
+}
+
+[[noreturn]] void fail(const char* what, long rc) {
+    const char* why = p_dvae_last_error();
+    throw DvaeError(std::string(what) + " failed (" + std::to_string(rc) + "): " + (why ? why : "?"));
+}
+
+int code(const Tensor& t) {
+    return t.scalar_type() == at::kFloat ? DVAE_F32 : t.scalar_type() == at::kBFloat16 ? DVAE_BF16 : DVAE_F16;
+}
+int wide(const Tensor& t) { return t.scalar_type() == at::kLong; }
+int wide(const Maybe& t) { return t && wide(*t); }
+void* ptr(const Maybe& t) { return t ? t->data_ptr() : nullptr; }
+
+// calls a function of the library with the current stream of `device`, that device being the current one
+template <typename Fn, typename... Args> void enqueue(const char* what, at::Device device, Fn* fn, Args... args) {
+    c10::DeviceGuard guard(device);
+    const int rc = fn(args..., c10::hip::getCurrentHIPStream(device.index()).stream());
+    if (rc != 0) fail(what, rc);
+}
+
+Tensor workspace(const char* what, int64_t bytes, at::Device device) {
+    if (bytes < 0) fail(what, bytes);
+    return at::empty({bytes}, at::TensorOptions(at::kByte).device(device));
+}
+
+// The rows of a [N, D] or [B, T, D] matrix whose elements lie side by side in a row: in place where the rows have one
+// stride of at most 2^23 elements (the recurrence addresses a few rows with 32-bit offsets), else of a copy.
+struct Rows {
+    Tensor keep;
+    int64_t n, d, ld;
+    explicit Rows(const Tensor& t) : keep(t), d(t.size(-1)) {
+        const bool flat = t.dim() == 2;
+        const int64_t B = t.size(0), T = flat ? 1 : t.size(1), step = flat || T == 1 ? t.stride(0) : t.stride(1);
+        n = B * T;
+        ld = n > 1 ? step : d;
+        const bool one = B == 1 || T <= 1 || t.stride(0) == T * step;
+        if (!one || (d > 1 && t.stride(-1) != 1) || (n > 1 && ((0 < ld && ld < d) || ld > (1 << 23)))) {
+            keep = t.contiguous();
+            ld = d;
+        }
+    }
+    void* p() const { return keep.data_ptr(); }
+};
+
+void once(const char* what) {  // create_graph=True: the backward pass itself is not recorded
+    if (at::GradMode::is_enabled()) throw std::runtime_error(std::string(what) + ": the gradient is not differentiable again");
+}
+
+// -------------------------------------------------------------------------------------------------------------- embed
+
+Tensor embed_forward(const Tensor& weight, const Tensor& ids, double scale) {
+    const int64_t V = weight.size(0), D = weight.size(1);
+    at::DimVector shape(ids.sizes());
+    shape.push_back(D);
+    Tensor out = at::empty(shape, at::TensorOptions(weight.scalar_type()).device(weight.device()));
+    enqueue("dvae_embed_fwd", weight.device(), p_dvae_embed_fwd, weight.data_ptr(), V > 1 ? weight.stride(0) : D, ids.data_ptr(), wide(ids),
+            out.data_ptr(), ids.numel(), V, D, (float)scale, code(weight));
+    return out;
+}
+
+struct Embed : torch::autograd::Function<Embed> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& weight, const Tensor& ids, double scale) {
+        ctx->save_for_backward({ids});
+        ctx->saved_data["rows"] = weight.size(0);
+        ctx->saved_data["scale"] = scale;
+        return embed_forward(weight, ids, scale);
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        once("embed");
+        const Tensor ids = ctx->get_saved_variables()[0];
+        const int64_t n = ids.numel(), V = ctx->saved_data["rows"].toInt(), D = grads[0].size(-1);
+        const Rows dout(grads[0].dim() == 2 ? grads[0] : grads[0].reshape({n, D}));
+        const at::Device dev = grads[0].device();
+        Tensor dw = at::empty({V, D}, at::TensorOptions(grads[0].scalar_type()).device(dev));
+        Tensor ws = workspace("dvae_embed_bwd_ws_bytes", p_dvae_embed_bwd_ws_bytes(n, V, D), dev);
+        enqueue("dvae_embed_bwd", dev, p_dvae_embed_bwd, dout.p(), dout.ld, ids.data_ptr(), wide(ids), dw.data_ptr(), ws.data_ptr(), n, V, D,
+                (float)ctx->saved_data["scale"].toDouble(), code(dw));
+        return {dw, Tensor(), Tensor()};
+    }
+};
+
+Tensor embed(const Tensor& weight, const Tensor& ids, double scale) {
+    if (weight.requires_grad() && at::GradMode::is_enabled()) return Embed::apply(weight, ids, scale);
+    return embed_forward(weight, ids, scale);
+}
+
+// --------------------------------------------------------------------------------------------------------- recurrence
+
+// h, last and, if `keep`, the states that the backward pass reads
+std::tuple<Tensor, Tensor, Tensor> scan_forward(const Tensor& gate, const Tensor& x, const Maybe& offsets, const Maybe& h0, int64_t seqs, bool keep) {
+    const Rows g(gate), y(x);
+    const at::Device dev = x.device();
+    const at::TensorOptions f32 = at::TensorOptions(at::kFloat).device(dev);
+    Tensor h = at::empty(x.sizes(), at::TensorOptions(x.scalar_type()).device(dev)), last = at::empty({seqs, g.d}, f32), states;
+    if (keep) states = at::empty({p_dvae_scan_state_floats(g.n, g.d)}, f32);
+    Tensor ws = workspace("dvae_scan_ws_bytes", p_dvae_scan_ws_bytes(g.n, g.d), dev);
+    enqueue("dvae_scan_fwd", dev, p_dvae_scan_fwd, g.p(), g.ld, y.p(), y.ld, ptr(offsets), wide(offsets), (const float*)ptr(h0), h.data_ptr(),
+            (float*)last.data_ptr(), keep ? (float*)states.data_ptr() : nullptr, ws.data_ptr(), g.n, seqs, g.d, code(x));
+    return {h, last, states};
+}
+
+struct Scan : torch::autograd::Function<Scan> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& gate, const Tensor& x, const Maybe& offsets, const Maybe& h0, int64_t seqs) {
+        auto [h, last, states] = scan_forward(gate, x, offsets, h0, seqs, true);
+        ctx->save_for_backward({gate, x, offsets.value_or(Tensor()), h0.value_or(Tensor()), states});
+        ctx->saved_data["seqs"] = seqs;
+        ctx->set_materialize_grads(false);
+        return {h, last};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        once("gated_scan");
+        const variable_list saved = ctx->get_saved_variables();
+        auto maybe = [](const Tensor& t) { return t.defined() ? Maybe(t) : Maybe(); };
+        const Tensor &gate = saved[0], &x = saved[1], &states = saved[4];
+        const Maybe offsets = maybe(saved[2]), h0 = maybe(saved[3]);
+        const int64_t seqs = ctx->saved_data["seqs"].toInt();
+        const Rows g(gate), y(x);
+        const at::Device dev = x.device();
+        std::optional<Rows> dh;
+        if (grads[0].defined()) dh.emplace(grads[0]);
+        const Maybe dlast = grads[1].defined() ? Maybe(grads[1].contiguous()) : Maybe();
+        const at::TensorOptions like = at::TensorOptions(x.scalar_type()).device(dev);
+        Tensor dgate = at::empty(gate.sizes(), like), dx = at::empty(x.sizes(), like), dh0;
+        // (the edges are those of the tensors that were given: gate, x, offsets if any, h0)
+        if (h0 && ctx->needs_input_grad(offsets ? 3 : 2)) dh0 = at::empty({seqs, g.d}, like.dtype(at::kFloat));
+        Tensor ws = workspace("dvae_scan_ws_bytes", p_dvae_scan_ws_bytes(g.n, g.d), dev);
+        enqueue("dvae_scan_bwd", dev, p_dvae_scan_bwd, g.p(), g.ld, y.p(), y.ld, ptr(offsets), wide(offsets), (const float*)ptr(h0),
+                (const float*)states.data_ptr(), dh ? dh->p() : nullptr, dh ? dh->ld : (int64_t)0, (const float*)ptr(dlast), dgate.data_ptr(),
+                dx.data_ptr(), dh0.defined() ? (float*)dh0.data_ptr() : nullptr, ws.data_ptr(), g.n, seqs, g.d, code(x));
+        return {dgate, dx, Tensor(), dh0, Tensor()};
+    }
+};
+
+std::tuple<Tensor, Tensor> scan(const Tensor& gate, const Tensor& x, const Maybe& offsets, const Maybe& h0, int64_t seqs) {
+    if (at::GradMode::is_enabled() && (gate.requires_grad() || x.requires_grad() || (h0 && h0->requires_grad()))) {
+        variable_list out = Scan::apply(gate, x, offsets, h0, seqs);
+        return {out[0], out[1]};
+    }
+    auto [h, last, states] = scan_forward(gate, x, offsets, h0, seqs, false);
+    return {h, last};
+}
+
+Tensor step(const Tensor& gate, const Tensor& x, const Tensor& state, const Maybe& slots) {
+    const Rows g(gate), y(x);
+    const int64_t P = state.size(0);
+    Tensor h = at::empty(x.sizes(), at::TensorOptions(x.scalar_type()).device(x.device()));
+    enqueue("dvae_scan_step", x.device(), p_dvae_scan_step, g.p(), g.ld, y.p(), y.ld, (float*)state.data_ptr(), P > 1 ? state.stride(0) : g.d, P,
+            ptr(slots), wide(slots), h.data_ptr(), g.n, g.d, code(x));
+    if (!state.is_inference()) torch::autograd::impl::bump_version(state);  // as by an in-place operation
+    return h;
+}
+
+}  // namespace
+
+PYBIND11_MODULE(_dvae_sequence, m) {
+    static PyObject* error = nullptr;
+    m.def("bind", [](const std::map<std::string, size_t>& addresses, py::object cls) {
+        bind(addresses);
+        error = cls.release().ptr();
+    });
+    py::register_exception_translator([](std::exception_ptr p) {
+        try {
+            if (p) std::rethrow_exception(p);
+        } catch (const DvaeError& e) {
+            PyErr_SetString(error ? error : PyExc_RuntimeError, e.what());
+        }
+    });
+#define F(name) #name,
+    m.attr("functions") = std::vector<std::string>{DVAE_FUNCTIONS(F)};
+#undef F
+    m.def("embed", &embed, py::call_guard<py::gil_scoped_release>());
+    m.def("scan", &scan, py::call_guard<py::gil_scoped_release>());
+    m.def("step", &step, py::call_guard<py::gil_scoped_release>());
+}

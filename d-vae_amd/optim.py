@@ -13,7 +13,33 @@ import torch
 
 from . import _lib
 from .dist import GradSumReducer
-from .sequence import _enqueue, _matrix, _workspace, _written
+from .sequence import _matrix
+
+
+def _enqueue(device, name, *args):
+    """calls the library's function `name` with the current stream of `device`, that device being the current one"""
+    fn = getattr(_lib.load(), name)
+    index = device.index
+    if index == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc != 0:
+        _lib.check(rc, name)
+
+
+def _workspace(n_bytes, device, what):
+    if n_bytes < 0:
+        _lib.check(-1, what)
+    return torch.empty(n_bytes, dtype=torch.uint8, device=device)
+
+
+def _written(*tensors):
+    """the library wrote into these: their autograd versions move as by an in-place operation"""
+    for t in tensors:
+        if not t.is_inference():
+            torch.autograd.graph.increment_version(t)
 
 
 QUINTIC = (3.4445, -4.7750, 2.0315)  # p(s) = a s + b s^3 + c s^5: five steps take singular values from 0.002 up to 0.7 .. 1.2
