@@ -17,9 +17,10 @@
 // states, products and sums are fp32; outputs are rounded once.
 //
 // One pass over the data in either direction (forward 3, backward 5 matrices of memory traffic), tiles chained through
-// look_back.  Measured on 131072 x 1024 bf16: forward 225 us (3.6 TB/s), backward 372 us (3.6 TB/s), where a large copy
-// reaches 4.9.  Without the look-back the forward pass takes 166 us, so the chain and not the arithmetic is what is left there;
-// the backward pass with trivial gates and no look-back 320: reads and writes of five matrices, at the vector units' rate nearly.
+// look_back.  Measured on 131072 x 1024 bf16: forward 225 us (3.6 TB/s), backward 367 us (3.7 TB/s), where a large copy
+// reaches 4.9.  With the look-back left out they take 187 and 272: what a tile waits for is two trips to device memory, its
+// neighbours' maps and back, about 5 us of the 28 (17) that it lives, whatever the length of the chain: a second level of
+// look-back over groups of 8 tiles, and other waves to publish than those that wait, made 223 and 354 of it, and 1 us more of a prompt.
 // Forward tiles of 64 rows: 318 us (a longer chain), of 256: 239; backward of 128: 392 (fewer workgroups a CU).  A look-back of
 // 16 tiles: 277 us forward (more words read per tile than it saves waits).
 #include "seq_common.h"
@@ -342,6 +343,9 @@ __global__ __launch_bounds__(TRB / RW * 64) void scan_bwd_kernel(ScanParams p) {
         for (int i = 0; i < RW; ++i)
 #pragma unroll
             for (int j = 0; j < V; ++j) d[i].e[j] = (T)0.f;
+    float begin[V];  // the state before the tile
+#pragma unroll
+    for (int j = 0; j < V; ++j) begin[j] = p.states[tile * p.D + min(c, p.D - V) + j];
     const Marks m = mark_rows(p.q, t0);
     const bool plain = m.start == 0 && m.end == 0 && m.cover == (unsigned)((1ull << RW) - 1);
     auto row_grad = [&](auto mixed, int i, float (&e)[V]) {  // dh of row i, and dlast where the sequence ends
@@ -423,7 +427,7 @@ __global__ __launch_bounds__(TRB / RW * 64) void scan_bwd_kernel(ScanParams p) {
     float C[V], prev[RW][V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        float s = p.states[tile * p.D + c + j];
+        float s = begin[j];
         for (int w = 0; w < wave; ++w) s = through(As[w][lane * V + j], Fs[w][lane * V + j], s);
         h[j] = s;
         s = Cs[lane * V + j];
