@@ -7,6 +7,7 @@ of every state, a convex combination of them).  A step of the recurrence rounds 
 import numpy as np
 import pytest
 import torch
+import torch.utils.checkpoint
 
 from _dvae_pkg import dvae_amd
 
@@ -459,6 +460,74 @@ def test_gradients_are_not_differentiable_again():
     gate = torch.randn(1, 5, 8).cuda().requires_grad_(True)
     with pytest.raises(RuntimeError, match="differentiable again"):
         torch.autograd.grad(S.gated_scan(gate, gate.detach())[0].sum(), [gate], create_graph=True)
+
+
+def test_the_graph_keeps_its_rules():
+    """kept graphs, recomputed segments, hooks on saved tensors, freed graphs, inputs changed in place, gradients of some inputs only"""
+    g = gen(41)
+    N, D = 300, 24
+    w = torch.randn(30, D, generator=g).cuda().requires_grad_(True)
+    gate = torch.randn(N, D, generator=g).cuda().requires_grad_(True)
+    h0 = torch.randn(3, D, generator=g).cuda().requires_grad_(True)
+    ids, off = torch.randint(0, 30, (N,), generator=g).cuda(), torch.tensor([0, 7, 7, N]).cuda()
+    up = torch.randn(N, D, generator=g).cuda()
+
+    def work(w, gate, h0):
+        return S.gated_scan(gate, S.embed(w, ids), off, h0)[0]
+
+    h = work(w, gate, h0)
+    first = torch.autograd.grad(h, [w, gate, h0], up, retain_graph=True)
+    again = torch.autograd.grad(h, [w, gate, h0], up)
+    assert all(torch.equal(a, b) for a, b in zip(first, again))
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad(h, [w], up)
+    h = torch.utils.checkpoint.checkpoint(work, w, gate, h0, use_reentrant=False)
+    assert all(torch.equal(a, b) for a, b in zip(first, torch.autograd.grad(h, [w, gate, h0], up)))
+    with torch.autograd.graph.save_on_cpu():
+        h = work(w, gate, h0)
+    assert all(torch.equal(a, b) for a, b in zip(first, torch.autograd.grad(h, [w, gate, h0], up)))
+    for k, only in enumerate((w, gate, h0)):  # the others need none
+        args = [t if t is only else t.detach() for t in (w, gate, h0)]
+        assert torch.equal(first[k], torch.autograd.grad(work(*args), [only], up)[0])
+        assert torch.equal(first[k], torch.autograd.grad(work(w, gate, h0), [only], up)[0])
+    x = S.embed(w, ids).detach()
+    h = S.gated_scan(gate, x, off)[0]
+    x.zero_()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(h, [gate], up)
+    # h0 without offsets
+    g3, x3, h3 = gate.detach().view(3, 100, D).requires_grad_(True), x.view(3, 100, D), h0.detach().requires_grad_(True)
+    dg, dh = torch.autograd.grad(S.gated_scan(g3, x3, h0=h3)[0], [g3, h3], up.view(3, 100, D))
+    even = torch.tensor([0, 100, 200, 300]).cuda()
+    dg2, dh2 = torch.autograd.grad(S.gated_scan(gate, x, even, h0)[0], [gate, h0], up)
+    assert torch.equal(dg.view(N, D), dg2) and torch.equal(dh, dh2)
+
+
+def test_two_threads_at_once():
+    import threading
+    g = gen(42)
+    jobs = [(torch.randn(40, 64, generator=g).cuda().requires_grad_(True), torch.randint(0, 40, (9000,), generator=g).cuda(),
+             torch.randn(9000, 64, generator=g).cuda()) for _ in range(4)]
+
+    def work(w, ids, up):
+        return torch.autograd.grad(S.gated_scan(up.view(3, 3000, 64), S.embed(w, ids).view(3, 3000, 64))[0], [w], up.view(3, 3000, 64))[0]
+
+    want = [work(*j) for j in jobs]
+    torch.cuda.synchronize()
+    got = [None] * len(jobs)
+
+    def run(k):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got[k] = work(*jobs[k])
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=run, args=(k,)) for k in range(len(jobs))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
 
 
 def test_operators_in_inference_mode():

@@ -98,3 +98,11 @@ def test_the_matrix_description_has_the_header_layout(tmp_path):
     subprocess.run(["gcc", "-std=c99", "-Wall", "-Werror", "-I", os.path.join(root, "include"), str(src), "-o", str(tmp_path / "layout")], check=True)
     out = subprocess.run([str(tmp_path / "layout")], check=True, capture_output=True, text=True).stdout.split()
     assert [int(v) for v in out] == [C.sizeof(L.MatrixDesc)] + [getattr(L.MatrixDesc, f).offset for f in names]
+
+
+def test_the_host_module_uses_declared_functions_and_has_no_fallback(monkeypatch, tmp_path):
+    ops = L.load_sequence_ops()
+    assert set(ops.functions) <= set(L.SIGNATURES)
+    monkeypatch.setattr(L, "HERE", str(tmp_path))
+    with pytest.raises(L.DvaeHipError, match="no fallback"):
+        L.load_sequence_ops()
