@@ -1,12 +1,13 @@
 // The host side of the sequence operators (sequence.py) in C++: outputs and workspaces, the launch on the current stream and
 // the autograd nodes.  This bounds small calls: through ctypes and Python autograd functions a lookup of 256 tokens took 8.7 us,
 // a single-token step 8.8, a lookup of 8192 with its gradient 85 and a short scan with its gradient 111 (kernels 3, 3, 30
-// and 29 us); from here 4.9, 5.3, 51 and 62, of which 42 are what torch takes to run any function's gradient.
-// The arguments are checked in sequence.py; the kernels and their C-ABI are in libdvae_hip.so, whose functions bind() gets.
+// and 29 us); from here 3.7, 3.8, 51 and 60, of which 42 are what torch takes to run any function's gradient.
+// The arguments are checked in sequence.py, those of a usual call here; the kernels and their C-ABI are in libdvae_hip.so, whose functions bind() gets.
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <stdexcept>
@@ -188,6 +189,80 @@ Tensor step(const Tensor& gate, const Tensor& x, const Tensor& state, const Mayb
     return h;
 }
 
+// ------------------------------------------------------------------------------------- what the checks would let pass as it is
+
+// The usual call, whose arguments sequence.py would find in order and change nothing of, is recognised here; nothing (None) is
+// returned for any other, which sequence.py then checks one by one: it refuses it, or brings it in order first.
+const Tensor* tensor(py::handle h) { return THPVariable_Check(h.ptr()) ? &THPVariable_Unpack(h.ptr()) : nullptr; }
+bool matrix(const Tensor* t, int64_t dims) {
+    return t && t->dim() == dims && t->is_cuda() &&
+           (t->scalar_type() == at::kFloat || t->scalar_type() == at::kBFloat16 || t->scalar_type() == at::kHalf);
+}
+bool alike(const Tensor& a, const Tensor& b) { return a.scalar_type() == b.scalar_type() && a.device() == b.device() && a.sizes() == b.sizes(); }
+bool index(const Tensor* t, at::Device device) {
+    return t && (t->scalar_type() == at::kInt || t->scalar_type() == at::kLong) && t->device() == device && t->is_contiguous();
+}
+bool rows_side_by_side(const Tensor& t) { return (t.size(1) == 1 || t.stride(1) == 1) && (t.size(0) <= 1 || t.stride(0) >= t.size(1)); }
+
+py::object usual_embed(py::handle weight, py::handle ids, double scale) {
+    const Tensor *w = tensor(weight), *t = tensor(ids);
+    if (!matrix(w, 2) || w->numel() == 0 || !rows_side_by_side(*w) || !index(t, w->device())) return py::none();
+    Tensor out;
+    {
+        py::gil_scoped_release without_gil;
+        out = embed(*w, *t, scale);
+    }
+    return py::cast(out);
+}
+
+py::object usual_scan(py::handle gate, py::handle x, py::handle offsets, py::handle h0) {
+    const Tensor *g = tensor(gate), *y = tensor(x);
+    Maybe off, first;
+    const int64_t dims = offsets.is_none() ? 3 : 2;
+    if (!matrix(g, dims) || !matrix(y, dims) || !alike(*g, *y) || y->size(-1) == 0) return py::none();
+    if (dims == 2) {
+        const Tensor* o = tensor(offsets);
+        if (!index(o, y->device()) || o->dim() != 1 || o->numel() < 1) return py::none();
+        off = *o;
+    }
+    const int64_t seqs = dims == 2 ? off->numel() - 1 : y->size(0);
+    if (!h0.is_none()) {
+        const Tensor* h = tensor(h0);
+        if (!h || h->scalar_type() != at::kFloat || h->device() != y->device() || h->dim() != 2 || h->size(0) != seqs ||
+            h->size(1) != y->size(-1) || !h->is_contiguous())
+            return py::none();
+        first = *h;
+    }
+    std::tuple<Tensor, Tensor> out;
+    {
+        py::gil_scoped_release without_gil;
+        out = scan(*g, *y, off, first, seqs);
+    }
+    return py::cast(out);
+}
+
+py::object usual_step(py::handle gate, py::handle x, py::handle state, py::handle slots) {
+    const Tensor *g = tensor(gate), *y = tensor(x), *s = tensor(state);
+    Maybe which;
+    if (!matrix(g, 2) || !matrix(y, 2) || !alike(*g, *y) || y->size(1) == 0 || !s || s->dim() != 2 || s->scalar_type() != at::kFloat ||
+        s->device() != y->device() || s->size(1) != y->size(1) || !rows_side_by_side(*s))
+        return py::none();
+    if (at::GradMode::is_enabled() && (g->requires_grad() || y->requires_grad() || s->requires_grad())) return py::none();
+    if (slots.is_none()) {
+        if (y->size(0) > s->size(0)) return py::none();
+    } else {
+        const Tensor* i = tensor(slots);
+        if (!index(i, y->device()) || i->dim() != 1 || i->size(0) != y->size(0)) return py::none();
+        which = *i;
+    }
+    Tensor out;
+    {
+        py::gil_scoped_release without_gil;
+        out = step(*g, *y, *s, which);
+    }
+    return py::cast(out);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_dvae_sequence, m) {
@@ -209,4 +284,7 @@ PYBIND11_MODULE(_dvae_sequence, m) {
     m.def("embed", &embed, py::call_guard<py::gil_scoped_release>());
     m.def("scan", &scan, py::call_guard<py::gil_scoped_release>());
     m.def("step", &step, py::call_guard<py::gil_scoped_release>());
+    m.def("usual_embed", &usual_embed);
+    m.def("usual_scan", &usual_scan);
+    m.def("usual_step", &usual_step);
 }

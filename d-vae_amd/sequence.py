@@ -55,6 +55,9 @@ def embed(weight, ids, scale=1.0):
     returns [*ids.shape, D].  A token outside [0, V) (padding) gives a row of zeros and takes no part in the gradient.
     The gradient of `weight` is dense, summed in float32 in the order of the tokens' positions and rounded once; it does
     not vary from run to run."""
+    out = (_ops or _native()).usual_embed(weight, ids, scale)
+    if out is not None:
+        return out
     _matrix(weight, "weight", 2)
     V, D = weight.shape
     if V == 0 or D == 0:
@@ -62,7 +65,7 @@ def embed(weight, ids, scale=1.0):
     if D > 1 and weight.stride(1) != 1 or V > 1 and weight.stride(0) < D:
         raise ValueError("the elements of a row of weight must lie side by side")
     ids = _index(ids, "ids", weight.device)
-    return (_ops or _native()).embed(weight, ids, float(scale))
+    return _ops.embed(weight, ids, float(scale))
 
 
 # ------------------------------------------------------------------------------------------------------------- recurrence
@@ -77,6 +80,9 @@ def gated_scan(gate, x, offsets=None, h0=None):
 
     gate and x may be the two halves of one projection's output: rows of any stride are read in place.  Differentiable in
     gate, x and h0; the states are float32 inside, h and the gradients of gate and x are rounded once to x's type."""
+    out = (_ops or _native()).usual_scan(gate, x, offsets, h0)
+    if out is not None:
+        return out
     dims = 2 if offsets is not None else 3
     _matrix(gate, "gate", dims)
     _matrix(x, "x", dims)
@@ -98,7 +104,7 @@ def gated_scan(gate, x, offsets=None, h0=None):
         if not torch.is_tensor(h0) or h0.dtype != torch.float32 or h0.device != x.device or tuple(h0.shape) != (seqs, D):
             raise ValueError("h0 must be a float32 tensor of shape (%d, %d) on %s" % (seqs, D, x.device))
         h0 = h0.contiguous()
-    return (_ops or _native()).scan(gate, x, offsets, h0, seqs)
+    return _ops.scan(gate, x, offsets, h0, seqs)
 
 
 def gated_step(gate, x, state, slots=None):
@@ -107,6 +113,9 @@ def gated_step(gate, x, state, slots=None):
     marks a padding row: its h is zero and no state changes.  Rows that name the same slot advance it one after the other,
     in their order.
     For serving: not differentiable, inputs that need gradients are refused outside torch.no_grad()."""
+    out = (_ops or _native()).usual_step(gate, x, state, slots)
+    if out is not None:
+        return out
     _matrix(gate, "gate", 2)
     _matrix(x, "x", 2)
     dev = x.device
@@ -128,4 +137,4 @@ def gated_step(gate, x, state, slots=None):
             raise ValueError("slots must have the shape (%d,)" % B)
     elif B > P:
         raise ValueError("%d rows, but %d states" % (B, P))
-    return (_ops or _native()).step(gate, x, state, slots)
+    return _ops.step(gate, x, state, slots)
