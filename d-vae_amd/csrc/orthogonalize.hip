@@ -224,9 +224,12 @@ template <int MODE> __device__ __forceinline__ void ns_tile_at(int t, int mt, in
 
 // 16 bytes per lane from memory to LDS, without a register in between: lane l's go to `lds` + 16 l.  Not the builtin: the
 // compiler would have every read of LDS wait for all of these loads; here ns_wait counts them.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"  // m0 is no register of the compiler's: that it is clobbered is said all the same
 __device__ __forceinline__ void ns_load_lds(const char* from, unsigned lds) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 1\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(from) : "memory", "m0");
 }
+#pragma clang diagnostic pop
 // all but the last N loads of this wave are done and its reads of LDS too; then the workgroup meets
 template <int N> __device__ __forceinline__ void ns_wait() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory"); }
 
