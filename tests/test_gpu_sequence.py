@@ -228,6 +228,32 @@ def test_gated_scan_and_its_gradient(dtype, dim, k):
     assert torch.equal(h, h2) and torch.equal(last, last2)
 
 
+@pytest.mark.parametrize("dim", [5, 70, 516])
+@pytest.mark.parametrize("lengths", [[64], [0, 60, 0, 4], [65, 0], [0, 128, 0], [129], [0] * 150 + [3, 0, 70] + [0] * 150, [1] * 64, [2] * 65])
+def test_gated_scan_of_one_tile_and_just_more(lengths, dim):
+    g = gen(len(lengths) * 1000 + dim)
+    off = offsets_of(lengths)
+    N, Sn = off[-1], len(lengths)
+    gate = (torch.randn(N, dim, generator=g) * 2 + 1).clamp(-5, 5)
+    x, h0 = torch.randn(N, dim, generator=g).clamp(-3, 3), torch.randn(Sn, dim, generator=g).clamp(-3, 3)
+    dh, dlast = torch.randn(N, dim, generator=g), torch.randn(Sn, dim, generator=g)
+    ref = plain_scan(gate.double(), x.double(), off, h0.double(), dh.double(), dlast.double())
+    gd, xd, hd = (t.cuda().requires_grad_(True) for t in (gate, x, h0))
+    h, last = S.gated_scan(gd, xd, torch.tensor(off, device="cuda"), hd)
+    mem, big = min(max(lengths), 1 + np.exp(5.0)), max(ref[5], 1.0)
+    tol_h, tol_G = (8 * mem + 32) * U * 3.0, (8 * mem + 32) * U * big  # as above
+    close(h, ref[0], tol_h, "h")
+    close(last, ref[1], tol_h, "last")
+    got = torch.autograd.grad([h, last], [gd, xd, hd], [dh.cuda(), dlast.cuda()])
+    close(got[0], ref[2], (tol_G * 6 + big * tol_h + 32 * U * big * 6) / 4, "dgate")
+    close(got[1], ref[3], tol_G + 4 * U * big, "dx")
+    close(got[2], ref[4], tol_G, "dh0")
+    none = [k for k in range(Sn) if lengths[k] == 0]
+    assert torch.equal(last[none], hd[none]) and torch.equal(got[2][none].cpu(), dlast[none])
+    again = S.gated_scan(gd, xd, torch.tensor(off, device="cuda"), hd)
+    assert torch.equal(h, again[0]) and torch.equal(last, again[1])
+
+
 def test_gated_scan_gradient_against_differences():
     g = gen(5)
     off, D, N = [0, 3, 70, 75], 5, 75
