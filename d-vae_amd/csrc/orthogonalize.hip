@@ -13,13 +13,15 @@
 // G is scaled by a power of two, exactly; the rest of the division by its norm (a factor r in (1, 2]) goes into the
 // coefficients of the first step: a r, b r^3, c r^5.
 //
-// bf16 matrices whose sides are all at least 512 multiply the hi planes alone, one MFMA instead of three.  A, B and the
-// operands X are then rounded to 11 bits; X itself keeps its second plane, which takes part in a X.  That is what matters:
-// where a few singular values are far above the rest, as in gradients, the rounding of X would bury the small ones, which
-// reach the result through a X (B is small there), while the same rounding inside a product meets the large directions only.
-// Measured against 64 bits, at 4096 x 4096 with four directions 0, 30 and 300 times the noise: 2.0e-3, 1.7e-3 and 1.6e-3,
-// of which the result's own rounding to bf16 is 1.7e-3 (without X's second plane 1.9e-3, 8.7e-3 and 3.7e-2; the iteration in
-// bf16 1.8e-2, 0.19 and 0.8), in 2.1 ms instead of 4.8.  Below 512 the roundings no longer average out (5e-3 at 9 x 1).
+// Half products, where the caller asks for them (DVAE_HALF_PRODUCTS) and a bf16 matrix has sides of at least 512: the hi planes
+// alone, one MFMA instead of three.  A, B and the operands X are then rounded to 11 bits; X itself keeps its second plane, which
+// takes part in a X.  That is what matters: where a few singular values are far above the rest, as in gradients, the rounding of
+// X would bury the small ones, which reach the result through a X (B is small there), while the same rounding inside a product
+// meets the large directions only.  Measured against 64 bits, at 4096 x 4096 with four directions 0, 30 and 300 times the noise:
+// 2.0e-3, 1.7e-3 and 1.6e-3, of which the result's own rounding to bf16 is 1.7e-3 (without X's second plane 1.9e-3, 8.7e-3 and
+// 3.7e-2; the iteration in bf16 1.8e-2, 0.19 and 0.8).  Where many singular values end near each other it loses more: 2.5e-3 at
+// 512 x 512 with equal ones.  A call takes 1490 us where full products take 3640 (1024 x 1024: 152 and 212).  Below 512 the roundings no longer average out (5e-3 at 9 x 1), so smaller matrices keep both planes;
+// the choice looks at each matrix alone, and matrices of one and of two planes are launched apart.
 //
 // Layout.  A row of any matrix is a run of 128-byte blocks: 32 hi followed by 32 lo of the same columns, padded with zeros
 // to whole tiles.  All three products contract over contiguous rows ("N T" form): X X^T and A A as they are (A is
@@ -619,12 +621,13 @@ static bool ns_huge(long tiles256) {
 }
 // what the sides are padded to: the largest tile that any product takes, where that adds at most an eighth to the work (eight
 // 700 x 700: 449 us a call on 64 x 64, 514 on 128 x 128)
-static int ns_pad_of(const dvae_matrix_desc* d, int32_t count) {
+static int ns_pad_of(const dvae_matrix_desc* mats, const int* group, int n) {
     long small = 0, big = 0, huge = 0;
-    for (int i = 0; i < count; ++i) {
-        small += (long)cdiv(d[i].rows, 64) * cdiv(d[i].cols, 64);
-        big += (long)cdiv(d[i].rows, 128) * cdiv(d[i].cols, 128);
-        huge += (long)cdiv(d[i].rows, 256) * cdiv(d[i].cols, 256);
+    for (int i = 0; i < n; ++i) {
+        const dvae_matrix_desc& d = mats[group[i]];
+        small += (long)cdiv(d.rows, 64) * cdiv(d.cols, 64);
+        big += (long)cdiv(d.rows, 128) * cdiv(d.cols, 128);
+        huge += (long)cdiv(d.rows, 256) * cdiv(d.cols, 256);
     }
     if (ns_huge(huge) && 32 * huge <= 9 * big) return 256;
     return ns_big(big) && 32 * big <= 9 * small ? 128 : 64;
@@ -633,16 +636,23 @@ static long ns_matrix_bytes(const dvae_matrix_desc& d, int pad, int planes) {
     const int mp = ns_pad(d.rows < d.cols ? d.rows : d.cols, pad), np = ns_pad(d.rows < d.cols ? d.cols : d.rows, pad);
     return ns_offset(mp, np, planes, planes == 1 ? 8 : 6);
 }
-// One plane in the products of a group of bf16 matrices whose sides are all at least 512; see the head of the file.
-static int ns_planes(const dvae_matrix_desc* d, int32_t count, int dtype) {
-    if (dtype != DVAE_BF16) return 2;
-    for (int i = 0; i < count; ++i)
-        if (d[i].rows < 512 || d[i].cols < 512) return 2;
-    return 1;
+// planes in the products of a matrix; see the head of the file
+static int ns_planes(const dvae_matrix_desc& d, int half) { return half && d.rows >= 512 && d.cols >= 512 ? 1 : 2; }
+// The call's matrices in groups that share their launches: up to NS_GROUP of the same number of planes, in the order of the call.
+// First those of two planes; `at` and `planes` say where the next group begins.  Returns the group's size, 0 behind the last.
+static int ns_next(const dvae_matrix_desc* d, int count, int half, int& planes, int& at, int (&group)[NS_GROUP]) {
+    int n = 0;
+    for (;; planes = 1, at = 0) {
+        for (; at < count && n < NS_GROUP; ++at)
+            if (ns_planes(d[at], half) == planes) group[n++] = at;
+        if (n > 0 || planes == 1) return n;
+    }
 }
 constexpr long NS_HEAD = NS_GROUP * (NS_PARTS * 8 + 8);
 
-static int ns_check(const char* who, const dvae_matrix_desc* d, int32_t count) {
+static int ns_check(const char* who, const dvae_matrix_desc* d, int32_t count, int32_t dtype) {
+    DVAE_REQUIRE(known_dtype(dtype & ~DVAE_HALF_PRODUCTS), "%s: unknown element type %d", who, dtype);
+    DVAE_REQUIRE(!(dtype & DVAE_HALF_PRODUCTS) || dtype == (DVAE_BF16 | DVAE_HALF_PRODUCTS), "%s: half products are for bf16 matrices", who);
     DVAE_REQUIRE(count >= 0 && (count == 0 || d), "%s: null pointer", who);
     for (int i = 0; i < count; ++i)
         DVAE_REQUIRE(d[i].rows >= 1 && d[i].cols >= 1 && d[i].rows <= 32768 && d[i].cols <= 32768,
@@ -654,13 +664,13 @@ static int ns_check(const char* who, const dvae_matrix_desc* d, int32_t count) {
 
 extern "C" int64_t dvae_orthogonalize_ws_bytes(const dvae_matrix_desc* mats, int32_t count, int32_t dtype) {
     using namespace dvae;
-    DVAE_REQUIRE(known_dtype(dtype), "orthogonalize_ws_bytes: unknown element type %d", dtype);
-    DVAE_TRY(ns_check("orthogonalize_ws_bytes", mats, count));
+    DVAE_TRY(ns_check("orthogonalize_ws_bytes", mats, count, dtype));
     int64_t most = 0;
-    for (int g0 = 0; g0 < count; g0 += NS_GROUP) {  // the groups follow each other on the stream and share the space
-        const int n = count - g0 < NS_GROUP ? count - g0 : NS_GROUP, planes = ns_planes(mats + g0, n, dtype), pad = ns_pad_of(mats + g0, n);
+    int group[NS_GROUP], planes = 2, at = 0;
+    while (const int n = ns_next(mats, count, dtype & DVAE_HALF_PRODUCTS, planes, at, group)) {  // the groups follow each other on the stream and share the space
+        const int pad = ns_pad_of(mats, group, n);
         int64_t sum = NS_HEAD;
-        for (int i = 0; i < n; ++i) sum += ns_matrix_bytes(mats[g0 + i], pad, planes);
+        for (int i = 0; i < n; ++i) sum += ns_matrix_bytes(mats[group[i]], pad, planes);
         most = sum > most ? sum : most;
     }
     return most;
@@ -669,8 +679,7 @@ extern "C" int64_t dvae_orthogonalize_ws_bytes(const dvae_matrix_desc* mats, int
 extern "C" int dvae_orthogonalize(const dvae_matrix_desc* mats, int32_t count, int32_t steps, const float* coefficients,
                                   void* ws, int32_t dtype, void* stream) {
     using namespace dvae;
-    DVAE_TRY(ns_check("orthogonalize", mats, count));
-    DVAE_REQUIRE(known_dtype(dtype), "orthogonalize: unknown element type %d", dtype);
+    DVAE_TRY(ns_check("orthogonalize", mats, count, dtype));
     DVAE_REQUIRE(steps >= 1 && steps <= 32 && coefficients, "orthogonalize: %d steps are not in 1 .. 32", steps);
     for (int i = 0; i < count; ++i)
         DVAE_REQUIRE(mats[i].g && mats[i].out && mats[i].ld_g >= mats[i].cols && mats[i].ld_out >= mats[i].cols,
@@ -693,19 +702,17 @@ extern "C" int dvae_orthogonalize(const dvae_matrix_desc* mats, int32_t count, i
     if (count == 0) return DVAE_OK;
     DVAE_REQUIRE(ws && (uintptr_t)ws % 16 == 0, "orthogonalize: the workspace must be 16-byte aligned");
     hipStream_t s = (hipStream_t)stream;
-    for (int g0 = 0; g0 < count; g0 += NS_GROUP) {
-        const int n = count - g0 < NS_GROUP ? count - g0 : NS_GROUP;
+    int order[NS_GROUP], planes = 2, next = 0;
+    while (const int n = ns_next(mats, count, dtype & DVAE_HALF_PRODUCTS, planes, next, order)) {
         NsGroup p = {};
         p.count = n;
-        p.dtype = dtype;
-        p.planes = ns_planes(mats + g0, n, dtype);
-        p.pad = ns_pad_of(mats + g0, n);
+        p.dtype = dtype & ~DVAE_HALF_PRODUCTS;
+        p.planes = planes;
+        p.pad = ns_pad_of(mats, order, n);
         p.parts = (double*)ws;
         p.r = (float*)((char*)ws + NS_GROUP * NS_PARTS * 8);
         p.ws = (char*)ws + NS_HEAD;
         // the matrices with the longest sums first: their tiles are the last to end
-        int order[NS_GROUP];
-        for (int i = 0; i < n; ++i) order[i] = g0 + i;
         for (int i = 1; i < n; ++i)
             for (int j = i; j > 0; --j) {
                 auto longer = [&](int k) { return mats[k].rows > mats[k].cols ? mats[k].rows : mats[k].cols; };

@@ -42,18 +42,21 @@ def _written(*tensors):
             torch.autograd.graph.increment_version(t)
 
 
+HALF_PRODUCTS = 16  # DVAE_HALF_PRODUCTS
 QUINTIC = (3.4445, -4.7750, 2.0315)  # p(s) = a s + b s^3 + c s^5: five steps take singular values from 0.002 up to 0.7 .. 1.2
 
 
-def orthogonalize(updates, steps=5, coefficients=QUINTIC, out=None):
+def orthogonalize(updates, steps=5, coefficients=QUINTIC, out=None, products="full"):
     """The nearest (semi-)orthogonal matrix to each of `updates`, approximately: `steps` Newton-Schulz steps
     X <- a X + (b A + c A A) X with A = X X^T (on the smaller side) from X = G / |G|_F.
 
     updates: a matrix or a list of matrices (float32, bfloat16 or float16, one type, on one HIP device); a list goes through
     every product in one launch.  coefficients: (a, b, c), or one such triple for each step; a set that lets a singular value
     leave [-2, 2] is refused.  out: where to write (same shapes and type; a matrix may be its own output), default new tensors.
-    Accuracy of float32 (for bfloat16 of its own rounding), rounded once to the matrices' type.  A zero matrix gives zeros, one with a NaN or an
-    infinity NaN.  Not differentiable (it acts on updates): inputs that need gradients are refused outside torch.no_grad()."""
+    Accuracy of float32, rounded once to the matrices' type.  products="half" (bfloat16 only): matrices with both sides of at
+    least 512 multiply operands of 11 bits, for a third of the work; their error is then of the order of the result's own
+    rounding and adds to it.  What other matrices a call has changes a result by the order of its sums alone (float32).
+    A zero matrix gives zeros, one with a NaN or an infinity NaN.  Not differentiable (it acts on updates): inputs that need gradients are refused outside torch.no_grad()."""
     one = torch.is_tensor(updates)
     mats = [updates] if one else list(updates)
     if out is not None:
@@ -71,6 +74,12 @@ def orthogonalize(updates, steps=5, coefficients=QUINTIC, out=None):
     if torch.is_grad_enabled() and any(torch.is_tensor(g) and g.requires_grad for g in mats):
         raise ValueError("orthogonalize is not differentiable: call it under torch.no_grad()")
     code = _matrix(mats[0], "updates", 2)
+    if products not in ("full", "half"):
+        raise ValueError("products must be 'full' or 'half'")
+    if products == "half":
+        if mats[0].dtype != torch.bfloat16:
+            raise ValueError("products='half' is for bfloat16 matrices")
+        code |= HALF_PRODUCTS
     dtype, device = mats[0].dtype, mats[0].device
     with torch.no_grad():
         srcs = []

@@ -106,3 +106,18 @@ def test_the_host_module_uses_declared_functions_and_has_no_fallback(monkeypatch
     monkeypatch.setattr(L, "HERE", str(tmp_path))
     with pytest.raises(L.DvaeHipError, match="no fallback"):
         L.load_sequence_ops()
+
+
+def test_half_products_are_refused_but_for_bf16():
+    d = (L.MatrixDesc * 1)(L.MatrixDesc(4096, 4096, 600, 600, 600, 600))
+    abc = (C.c_float * 15)(*[3.4445, -4.7750, 2.0315] * 5)
+    assert "half products" in rc("dvae_orthogonalize", d, 1, 5, abc, C.c_void_p(4096), 16, None)
+    assert "half products" in rc("dvae_orthogonalize_ws_bytes", d, 1, 18)
+    lib = L.load()
+    full, half = lib.dvae_orthogonalize_ws_bytes(d, 1, 1), lib.dvae_orthogonalize_ws_bytes(d, 1, 17)
+    assert 0 < half < full  # one plane of A, B and the turned X
+    small = (L.MatrixDesc * 1)(L.MatrixDesc(4096, 4096, 600, 600, 511, 600))
+    assert lib.dvae_orthogonalize_ws_bytes(small, 1, 1) == lib.dvae_orthogonalize_ws_bytes(small, 1, 17)
+    mixed = (L.MatrixDesc * 34)(*[L.MatrixDesc(4096, 4096, 600, 600, 511 + k % 2, 600) for k in range(34)])
+    seventeen = (L.MatrixDesc * 17)(*[L.MatrixDesc(4096, 4096, 600, 600, 511, 600) for k in range(17)])
+    assert lib.dvae_orthogonalize_ws_bytes(mixed, 34, 17) == lib.dvae_orthogonalize_ws_bytes(seventeen, 17, 17)
