@@ -50,10 +50,22 @@ int wide(const Tensor& t) { return t.scalar_type() == at::kLong; }
 int wide(const Maybe& t) { return t && wide(*t); }
 void* ptr(const Maybe& t) { return t ? t->data_ptr() : nullptr; }
 
+// A size that the library takes in 32 bits.  Its own limits are lower, but a size cut to 32 bits would pass them.
+int32_t size32(const char* what, int64_t v) {
+    if (v > INT32_MAX) throw DvaeError(std::string(what) + ": " + std::to_string(v) + " are not supported");
+    return (int32_t)v;
+}
+// a function of the library; no argument may be wider than its parameter
+template <typename P, typename A> constexpr bool cut = std::is_integral_v<P> && std::is_integral_v<A> && sizeof(P) < sizeof(A);
+template <typename R, typename... Ps, typename... As> R call(R (*fn)(Ps...), As... args) {
+    static_assert(!(cut<Ps, As> || ...), "narrow it with size32");
+    return fn(args...);
+}
+
 // calls a function of the library with the current stream of `device`, that device being the current one
 template <typename Fn, typename... Args> void enqueue(const char* what, at::Device device, Fn* fn, Args... args) {
     c10::DeviceGuard guard(device);
-    const int rc = fn(args..., c10::hip::getCurrentHIPStream(device.index()).stream());
+    const int rc = call(fn, args..., (void*)c10::hip::getCurrentHIPStream(device.index()).stream());
     if (rc != 0) fail(what, rc);
 }
 
@@ -88,11 +100,12 @@ void once(const char* what) {  // create_graph=True: the backward pass itself is
 // -------------------------------------------------------------------------------------------------------------- embed
 
 Tensor embed_forward(const Tensor& weight, const Tensor& ids, double scale) {
-    const int64_t V = weight.size(0), D = weight.size(1);
+    const int64_t V = weight.size(0);
+    const int32_t D = size32("embed: elements of a row", weight.size(1));
     at::DimVector shape(ids.sizes());
     shape.push_back(D);
     Tensor out = at::empty(shape, at::TensorOptions(weight.scalar_type()).device(weight.device()));
-    enqueue("dvae_embed_fwd", weight.device(), p_dvae_embed_fwd, weight.data_ptr(), V > 1 ? weight.stride(0) : D, ids.data_ptr(), wide(ids),
+    enqueue("dvae_embed_fwd", weight.device(), p_dvae_embed_fwd, weight.data_ptr(), V > 1 ? weight.stride(0) : (int64_t)D, ids.data_ptr(), wide(ids),
             out.data_ptr(), ids.numel(), V, D, (float)scale, code(weight));
     return out;
 }
@@ -107,11 +120,12 @@ struct Embed : torch::autograd::Function<Embed> {
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         once("embed");
         const Tensor ids = ctx->get_saved_variables()[0];
-        const int64_t n = ids.numel(), V = ctx->saved_data["rows"].toInt(), D = grads[0].size(-1);
+        const int64_t n = ids.numel(), V = ctx->saved_data["rows"].toInt();
+        const int32_t D = (int32_t)grads[0].size(-1);  // (as the forward pass had it)
         const Rows dout(grads[0].dim() == 2 ? grads[0] : grads[0].reshape({n, D}));
         const at::Device dev = grads[0].device();
         Tensor dw = at::empty({V, D}, at::TensorOptions(grads[0].scalar_type()).device(dev));
-        Tensor ws = workspace("dvae_embed_bwd_ws_bytes", p_dvae_embed_bwd_ws_bytes(n, V, D), dev);
+        Tensor ws = workspace("dvae_embed_bwd_ws_bytes", call(p_dvae_embed_bwd_ws_bytes, n, V, D), dev);
         enqueue("dvae_embed_bwd", dev, p_dvae_embed_bwd, dout.p(), dout.ld, ids.data_ptr(), wide(ids), dw.data_ptr(), ws.data_ptr(), n, V, D,
                 (float)ctx->saved_data["scale"].toDouble(), code(dw));
         return {dw, Tensor(), Tensor()};
@@ -127,14 +141,15 @@ Tensor embed(const Tensor& weight, const Tensor& ids, double scale) {
 
 // h, last and, if `keep`, the states that the backward pass reads
 std::tuple<Tensor, Tensor, Tensor> scan_forward(const Tensor& gate, const Tensor& x, const Maybe& offsets, const Maybe& h0, int64_t seqs, bool keep) {
+    const int32_t D = size32("gated_scan: channels", x.size(-1));
     const Rows g(gate), y(x);
     const at::Device dev = x.device();
     const at::TensorOptions f32 = at::TensorOptions(at::kFloat).device(dev);
-    Tensor h = at::empty(x.sizes(), at::TensorOptions(x.scalar_type()).device(dev)), last = at::empty({seqs, g.d}, f32), states;
-    if (keep) states = at::empty({p_dvae_scan_state_floats(g.n, g.d)}, f32);
-    Tensor ws = workspace("dvae_scan_ws_bytes", p_dvae_scan_ws_bytes(g.n, g.d), dev);
+    Tensor h = at::empty(x.sizes(), at::TensorOptions(x.scalar_type()).device(dev)), last = at::empty({seqs, D}, f32), states;
+    if (keep) states = at::empty({call(p_dvae_scan_state_floats, g.n, D)}, f32);
+    Tensor ws = workspace("dvae_scan_ws_bytes", call(p_dvae_scan_ws_bytes, g.n, D), dev);
     enqueue("dvae_scan_fwd", dev, p_dvae_scan_fwd, g.p(), g.ld, y.p(), y.ld, ptr(offsets), wide(offsets), (const float*)ptr(h0), h.data_ptr(),
-            (float*)last.data_ptr(), keep ? (float*)states.data_ptr() : nullptr, ws.data_ptr(), g.n, seqs, g.d, code(x));
+            (float*)last.data_ptr(), keep ? (float*)states.data_ptr() : nullptr, ws.data_ptr(), g.n, seqs, D, code(x));
     return {h, last, states};
 }
 
@@ -153,6 +168,7 @@ struct Scan : torch::autograd::Function<Scan> {
         const Tensor &gate = saved[0], &x = saved[1], &states = saved[4];
         const Maybe offsets = maybe(saved[2]), h0 = maybe(saved[3]);
         const int64_t seqs = ctx->saved_data["seqs"].toInt();
+        const int32_t D = (int32_t)x.size(-1);  // (as the forward pass had it)
         const Rows g(gate), y(x);
         const at::Device dev = x.device();
         std::optional<Rows> dh;
@@ -161,11 +177,11 @@ struct Scan : torch::autograd::Function<Scan> {
         const at::TensorOptions like = at::TensorOptions(x.scalar_type()).device(dev);
         Tensor dgate = at::empty(gate.sizes(), like), dx = at::empty(x.sizes(), like), dh0;
         // (the edges are those of the tensors that were given: gate, x, offsets if any, h0)
-        if (h0 && ctx->needs_input_grad(offsets ? 3 : 2)) dh0 = at::empty({seqs, g.d}, like.dtype(at::kFloat));
-        Tensor ws = workspace("dvae_scan_ws_bytes", p_dvae_scan_ws_bytes(g.n, g.d), dev);
+        if (h0 && ctx->needs_input_grad(offsets ? 3 : 2)) dh0 = at::empty({seqs, D}, like.dtype(at::kFloat));
+        Tensor ws = workspace("dvae_scan_ws_bytes", call(p_dvae_scan_ws_bytes, g.n, D), dev);
         enqueue("dvae_scan_bwd", dev, p_dvae_scan_bwd, g.p(), g.ld, y.p(), y.ld, ptr(offsets), wide(offsets), (const float*)ptr(h0),
                 (const float*)states.data_ptr(), dh ? dh->p() : nullptr, dh ? dh->ld : (int64_t)0, (const float*)ptr(dlast), dgate.data_ptr(),
-                dx.data_ptr(), dh0.defined() ? (float*)dh0.data_ptr() : nullptr, ws.data_ptr(), g.n, seqs, g.d, code(x));
+                dx.data_ptr(), dh0.defined() ? (float*)dh0.data_ptr() : nullptr, ws.data_ptr(), g.n, seqs, D, code(x));
         return {dgate, dx, Tensor(), dh0, Tensor()};
     }
 };
@@ -180,11 +196,12 @@ std::tuple<Tensor, Tensor> scan(const Tensor& gate, const Tensor& x, const Maybe
 }
 
 Tensor step(const Tensor& gate, const Tensor& x, const Tensor& state, const Maybe& slots) {
+    const int32_t B = size32("gated_step: rows", x.size(0)), D = size32("gated_step: channels", x.size(1));
     const Rows g(gate), y(x);
     const int64_t P = state.size(0);
     Tensor h = at::empty(x.sizes(), at::TensorOptions(x.scalar_type()).device(x.device()));
-    enqueue("dvae_scan_step", x.device(), p_dvae_scan_step, g.p(), g.ld, y.p(), y.ld, (float*)state.data_ptr(), P > 1 ? state.stride(0) : g.d, P,
-            ptr(slots), wide(slots), h.data_ptr(), g.n, g.d, code(x));
+    enqueue("dvae_scan_step", x.device(), p_dvae_scan_step, g.p(), g.ld, y.p(), y.ld, (float*)state.data_ptr(), P > 1 ? state.stride(0) : (int64_t)D, P,
+            ptr(slots), wide(slots), h.data_ptr(), B, D, code(x));
     if (!state.is_inference()) torch::autograd::impl::bump_version(state);  // as by an in-place operation
     return h;
 }

@@ -64,6 +64,8 @@ def orthogonalize(updates, steps=5, coefficients=QUINTIC, out=None, products="fu
         if len(outs) != len(mats):
             raise ValueError("out has %d matrices, updates %d" % (len(outs), len(mats)))
     steps, coefficients = int(steps), list(coefficients)
+    if not 1 <= steps <= 32:
+        raise ValueError("steps must lie in 1 .. 32")
     if coefficients and not hasattr(coefficients[0], "__len__"):
         coefficients = [coefficients] * steps
     triples = [tuple(c) for c in coefficients]
@@ -89,6 +91,8 @@ def orthogonalize(updates, steps=5, coefficients=QUINTIC, out=None, products="fu
                 raise ValueError("the matrices of one call must have one type and one device")
             if g.numel() == 0:
                 raise ValueError("updates: an empty matrix")
+            if max(g.shape) > 32768:  # (the descriptions below hold the sides in 32 bits)
+                raise ValueError("updates: a matrix of %d x %d; sides of up to 32768 are supported" % tuple(g.shape))
             srcs.append(g if (g.shape[1] == 1 or g.stride(1) == 1) and (g.shape[0] == 1 or g.stride(0) >= g.shape[1]) else g.contiguous())
         if out is None:
             outs = [torch.empty(g.shape, dtype=dtype, device=device) for g in mats]

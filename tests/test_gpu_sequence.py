@@ -641,3 +641,12 @@ def test_a_training_step_of_a_sequence_encoder():
         s = x @ x.t()
         x = 3.4445 * x + (-4.7750 * s + 2.0315 * (s @ s)) @ x
     assert float((update.double().cpu() - x).norm() / x.norm()) < 341 * 16 * 2.0 ** -22
+
+
+def test_rows_and_sides_past_32_bits_are_refused():
+    n = 2 ** 32 + 5  # would arrive as 5
+    one = torch.zeros(1, 1, device="cuda")
+    with pytest.raises(dvae_amd._lib.DvaeHipError, match="rows"):
+        S.gated_step(one.expand(n, 1), one.expand(n, 1), torch.empty(n, 1, device="cuda"))  # 17 GB, not touched
+    with pytest.raises(ValueError, match="32768"):
+        dvae_amd.optim.orthogonalize(one.expand(n, 1))

@@ -121,3 +121,27 @@ def test_half_products_are_refused_but_for_bf16():
     mixed = (L.MatrixDesc * 34)(*[L.MatrixDesc(4096, 4096, 600, 600, 511 + k % 2, 600) for k in range(34)])
     seventeen = (L.MatrixDesc * 17)(*[L.MatrixDesc(4096, 4096, 600, 600, 511, 600) for k in range(17)])
     assert lib.dvae_orthogonalize_ws_bytes(mixed, 34, 17) == lib.dvae_orthogonalize_ws_bytes(seventeen, 17, 17)
+
+
+@pytest.mark.parametrize("extra", [0, 5])
+def test_sizes_past_32_bits_are_refused_not_cut(extra):
+    """the library takes rows of a step and row lengths in 32 bits; tensors without memory, nothing is launched"""
+    ops, n = S._native(), 2 ** 32 + extra
+
+    def meta(*shape, dtype=torch.float32):
+        return torch.empty(*shape, dtype=dtype, device="meta")
+
+    ids, off = meta(2, dtype=torch.int64), meta(2, dtype=torch.int64)
+    with pytest.raises(L.DvaeHipError, match="elements of a row: %d are not supported" % n):
+        ops.embed(meta(1, n), ids, 1.0)
+    with pytest.raises(L.DvaeHipError, match="channels: %d are not supported" % n):
+        ops.scan(meta(1, n), meta(1, n), off, None, 1)
+    with pytest.raises(L.DvaeHipError, match="rows: %d are not supported" % n):
+        ops.step(meta(1, 1).expand(n, 1), meta(1, 1).expand(n, 1), meta(n, 1), None)
+    with pytest.raises(L.DvaeHipError, match="channels: %d are not supported" % n):
+        ops.step(meta(1, n), meta(1, n), meta(1, n), None)
+
+
+def test_many_newton_schulz_steps_are_refused_before_they_are_listed():
+    with pytest.raises(ValueError, match="steps"):
+        dvae_amd.optim.orthogonalize(torch.zeros(3, 3), steps=2 ** 32 + 5)
