@@ -93,8 +93,15 @@ struct Rows {
     void* p() const { return keep.data_ptr(); }
 };
 
-void once(const char* what) {  // create_graph=True: the backward pass itself is not recorded
+// Raw buffers carry no tangent: a dual tensor would give an output whose derivative is silently zero.
+template <typename... Ts> void no_tangent(const char* what, const Ts&... tensors) {
+    auto has = [](const Tensor& t) { return t.defined() && t._fw_grad(/* level */ 0).defined(); };
+    if ((has(tensors) || ...)) throw std::invalid_argument(std::string(what) + " has no forward-mode derivative");
+}
+
+void once(const char* what, const variable_list& grads) {  // create_graph=True: the backward pass itself is not recorded
     if (at::GradMode::is_enabled()) throw std::runtime_error(std::string(what) + ": the gradient is not differentiable again");
+    for (const Tensor& g : grads) no_tangent(what, g);
 }
 
 // -------------------------------------------------------------------------------------------------------------- embed
@@ -118,7 +125,7 @@ struct Embed : torch::autograd::Function<Embed> {
         return embed_forward(weight, ids, scale);
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
-        once("embed");
+        once("embed", grads);
         const Tensor ids = ctx->get_saved_variables()[0];
         const int64_t n = ids.numel(), V = ctx->saved_data["rows"].toInt();
         const int32_t D = (int32_t)grads[0].size(-1);  // (as the forward pass had it)
@@ -133,6 +140,7 @@ struct Embed : torch::autograd::Function<Embed> {
 };
 
 Tensor embed(const Tensor& weight, const Tensor& ids, double scale) {
+    no_tangent("embed", weight);
     if (weight.requires_grad() && at::GradMode::is_enabled()) return Embed::apply(weight, ids, scale);
     return embed_forward(weight, ids, scale);
 }
@@ -162,7 +170,7 @@ struct Scan : torch::autograd::Function<Scan> {
         return {h, last};
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
-        once("gated_scan");
+        once("gated_scan", grads);
         const variable_list saved = ctx->get_saved_variables();
         auto maybe = [](const Tensor& t) { return t.defined() ? Maybe(t) : Maybe(); };
         const Tensor &gate = saved[0], &x = saved[1], &states = saved[4];
@@ -187,6 +195,7 @@ struct Scan : torch::autograd::Function<Scan> {
 };
 
 std::tuple<Tensor, Tensor> scan(const Tensor& gate, const Tensor& x, const Maybe& offsets, const Maybe& h0, int64_t seqs) {
+    no_tangent("gated_scan", gate, x, h0.value_or(Tensor()));
     if (at::GradMode::is_enabled() && (gate.requires_grad() || x.requires_grad() || (h0 && h0->requires_grad()))) {
         variable_list out = Scan::apply(gate, x, offsets, h0, seqs);
         return {out[0], out[1]};
@@ -196,6 +205,7 @@ std::tuple<Tensor, Tensor> scan(const Tensor& gate, const Tensor& x, const Maybe
 }
 
 Tensor step(const Tensor& gate, const Tensor& x, const Tensor& state, const Maybe& slots) {
+    no_tangent("gated_step", gate, x, state);
     const int32_t B = size32("gated_step: rows", x.size(0)), D = size32("gated_step: channels", x.size(1));
     const Rows g(gate), y(x);
     const int64_t P = state.size(0);

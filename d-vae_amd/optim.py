@@ -10,6 +10,7 @@ encoder's when unidirectional) are left alone, exactly as torch's Adam skips the
 import ctypes as C
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .dist import GradSumReducer
@@ -75,6 +76,9 @@ def orthogonalize(updates, steps=5, coefficients=QUINTIC, out=None, products="fu
         return []
     if torch.is_grad_enabled() and any(torch.is_tensor(g) and g.requires_grad for g in mats):
         raise ValueError("orthogonalize is not differentiable: call it under torch.no_grad()")
+    if forward_ad._current_level >= 0 and any(torch.is_tensor(g) and forward_ad.unpack_dual(g).tangent is not None
+                                              for g in mats + (outs if out is not None else [])):
+        raise ValueError("orthogonalize has no forward-mode derivative")
     code = _matrix(mats[0], "updates", 2)
     if products not in ("full", "half"):
         raise ValueError("products must be 'full' or 'half'")

@@ -7,7 +7,8 @@
 The DAG model keeps its own paths (at most 32 vertex types as a table inside the GRU kernels, chains of at most 64
 vertices); these are for encoders of long or many token sequences beside it -- the reference's sequence baselines
 (models.py:18-338) run on one-hot inputs and nn.GRU.  Matrices are float32, bfloat16 or float16, the states of the
-recurrence always float32.  Like the rest of the package there is no CPU or PyTorch fallback.
+recurrence always float32.  Like the rest of the package there is no CPU or PyTorch fallback.  Gradients are those of the
+backward pass alone: tensors that carry a tangent (forward-mode derivatives) are refused.
 """
 import torch
 

@@ -650,3 +650,21 @@ def test_rows_and_sides_past_32_bits_are_refused():
         S.gated_step(one.expand(n, 1), one.expand(n, 1), torch.empty(n, 1, device="cuda"))  # 17 GB, not touched
     with pytest.raises(ValueError, match="32768"):
         dvae_amd.optim.orthogonalize(one.expand(n, 1))
+
+
+def test_forward_mode_is_refused_not_dropped():
+    import torch.autograd.forward_ad as fwd
+    w, ids = torch.randn(4, 8).cuda(), torch.tensor([1, 2], device="cuda")
+    gate, off = torch.randn(6, 8).cuda(), torch.tensor([0, 6], device="cuda")
+    for call in (lambda t: S.embed(t[:4], ids), lambda t: S.gated_scan(t, gate, off)[0], lambda t: S.gated_scan(gate, t, off)[0],
+                 lambda t: S.gated_step(t, gate, gate.clone()), lambda t: dvae_amd.optim.orthogonalize(t)):
+        with fwd.dual_level(), pytest.raises(ValueError, match="forward-mode"):
+            call(fwd.make_dual(gate.clone(), gate))
+        with fwd.dual_level():
+            call(gate)  # no tangent: as ever
+        with pytest.raises((ValueError, RuntimeError)):
+            torch.func.jvp(call, (gate,), (gate,))
+    wl = w.clone().requires_grad_(True)
+    out = S.embed(wl, ids)
+    with fwd.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):  # a tangent of the upstream gradient
+        torch.autograd.grad(out, [wl], fwd.make_dual(torch.ones_like(out), torch.ones_like(out)))

@@ -145,3 +145,20 @@ def test_sizes_past_32_bits_are_refused_not_cut(extra):
 def test_many_newton_schulz_steps_are_refused_before_they_are_listed():
     with pytest.raises(ValueError, match="steps"):
         dvae_amd.optim.orthogonalize(torch.zeros(3, 3), steps=2 ** 32 + 5)
+
+
+def test_tensors_with_a_tangent_are_refused():
+    """forward-mode derivatives would be dropped; also where nothing is recorded for the backward pass"""
+    import torch.autograd.forward_ad as fwd
+    ops, t = S._native(), torch.ones(3, 4)
+    ids, off = torch.zeros(2, dtype=torch.int64), torch.tensor([0, 3])
+    with fwd.dual_level():
+        d = fwd.make_dual(t, t)
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad):
+                for call in (lambda: ops.embed(d, ids, 1.0), lambda: ops.scan(d, t, off, None, 1), lambda: ops.scan(t, d, off, None, 1),
+                             lambda: ops.scan(t, t, off, d[:1], 1), lambda: ops.step(d, t, t, None), lambda: ops.step(t, d, t, None),
+                             lambda: ops.step(t, t, d, None), lambda: dvae_amd.optim.orthogonalize(d),
+                             lambda: dvae_amd.optim.orthogonalize([t], out=[d])):
+                    with pytest.raises(ValueError, match="forward-mode"):
+                        call()
