@@ -7,7 +7,9 @@ the views of `dist.GradSumReducer`'s flat buffer, and `step()` is `dvae_adam_ste
 Parameters the step never touches (grad None in the reference: `hv_unify`, the backward
 encoder's when unidirectional) are left alone, exactly as torch's Adam skips them.
 """
+import bisect
 import ctypes as C
+import itertools
 
 import torch
 from torch.autograd import forward_ad
@@ -43,6 +45,24 @@ def _written(*tensors):
             torch.autograd.graph.increment_version(t)
 
 
+def _kept_apart(srcs, outs):
+    """`srcs`, copied where they share memory with the output of another matrix: the library reads and writes the matrices in
+    groups, and a group's outputs must not reach what a later one reads.  (Address ranges: rows between those of a matrix count.)"""
+    def span(t):
+        return t.data_ptr(), t.data_ptr() + ((t.shape[0] - 1) * t.stride(0) + t.shape[1]) * t.element_size()
+    spans = sorted(span(o) + (k,) for k, o in enumerate(outs))
+    begins = [b for b, _, _ in spans]
+    reach = list(itertools.accumulate((e for _, e, _ in spans), max))
+    apart = []
+    for k, g in enumerate(srcs):
+        begin, end = span(g)
+        j = bisect.bisect_left(begins, end) - 1
+        while j >= 0 and reach[j] > begin and not (spans[j][1] > begin and spans[j][2] != k):
+            j -= 1
+        apart.append(g.clone() if j >= 0 and reach[j] > begin else g)
+    return apart
+
+
 HALF_PRODUCTS = 16  # DVAE_HALF_PRODUCTS
 QUINTIC = (3.4445, -4.7750, 2.0315)  # p(s) = a s + b s^3 + c s^5: five steps take singular values from 0.002 up to 0.7 .. 1.2
 
@@ -53,7 +73,7 @@ def orthogonalize(updates, steps=5, coefficients=QUINTIC, out=None, products="fu
 
     updates: a matrix or a list of matrices (float32, bfloat16 or float16, one type, on one HIP device); a list goes through
     every product in one launch.  coefficients: (a, b, c), or one such triple for each step; a set that lets a singular value
-    leave [-2, 2] is refused.  out: where to write (same shapes and type; a matrix may be its own output), default new tensors.
+    leave [-2, 2] is refused.  out: where to write (same shapes and type; matrices may be their own outputs, or each other's), default new tensors.
     Accuracy of float32, rounded once to the matrices' type.  products="half" (bfloat16 only): matrices with both sides of at
     least 512 multiply operands of 11 bits, for a third of the work; their error is then of the order of the result's own
     rounding and adds to it.  What other matrices a call has changes a result by the order of its sums alone (float32).
@@ -106,6 +126,8 @@ def orthogonalize(updates, steps=5, coefficients=QUINTIC, out=None, products="fu
                     raise ValueError("out must have the shapes, type and device of updates")
                 if (o.shape[1] > 1 and o.stride(1) != 1) or (o.shape[0] > 1 and o.stride(0) < o.shape[1]):
                     raise ValueError("out: the elements of a row must lie side by side")
+            if len(mats) > 32 or products == "half":  # more than one group
+                srcs = _kept_apart(srcs, outs)
         lib = _lib.load()
         descs = (_lib.MatrixDesc * len(mats))(*[
             _lib.MatrixDesc(g.data_ptr(), o.data_ptr(), g.stride(0) if g.shape[0] > 1 else g.shape[1],

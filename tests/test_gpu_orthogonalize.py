@@ -115,3 +115,24 @@ def test_float32_accuracy_of_special_inputs(shape, kind):
     one = plain(m, 1)
     got = off(O.orthogonalize(given, steps=1), one.cpu())
     assert got <= 8 * max(off(plain(m, 1, dtype=torch.float32), one.cpu()), 2.0 ** -22), got
+
+
+def test_outputs_in_the_place_of_other_inputs():
+    """more matrices than one launch group holds: what a later group reads is not overwritten by an earlier one's outputs"""
+    g = torch.Generator().manual_seed(7)
+    buffer = torch.randn(60, 20, 33, generator=g).cuda()
+    want = O.orthogonalize([m.clone() for m in buffer])
+    for shift in (0, 5, 59):
+        mine = buffer.clone()
+        O.orthogonalize(list(mine), out=[mine[(k + shift) % 60] for k in range(60)])
+        assert torch.equal(mine, torch.stack([want[(k - shift) % 60] for k in range(60)])), shift
+    mine = buffer[:40].clone().view(40 * 20, 33)  # rows of two matrices in turn, in one range of addresses
+    pairs = [mine[40 * k + b:40 * k + 40:2] for k in range(20) for b in (0, 1)]
+    want = O.orthogonalize([p.clone() for p in pairs])
+    O.orthogonalize(pairs, out=pairs)
+    assert all(torch.equal(a, b) for a, b in zip(pairs, want))
+    large, small = torch.randn(512, 512, generator=g).bfloat16().cuda(), torch.randn(512, 511, generator=g).bfloat16().cuda()
+    mine = torch.cat([large, small], 1)  # the small one's group is launched first, and writes where the large one begins
+    want = O.orthogonalize([large, small], products="half")
+    O.orthogonalize([mine[:, :512], mine[:, 512:]], out=[mine[:, 511:], mine[:, :511]], products="half")
+    assert torch.equal(mine[:, 511:], want[0]) and torch.equal(mine[:, :511], want[1])

@@ -162,3 +162,20 @@ def test_tensors_with_a_tangent_are_refused():
                              lambda: dvae_amd.optim.orthogonalize([t], out=[d])):
                     with pytest.raises(ValueError, match="forward-mode"):
                         call()
+
+
+def test_inputs_are_copied_only_where_another_output_shares_their_memory():
+    apart = dvae_amd.optim._kept_apart
+    flat = torch.zeros(10, 4, 6)
+    mats = list(flat)
+
+    def copied(srcs, outs):
+        return [a.data_ptr() != s.data_ptr() for a, s in zip(apart(srcs, outs), srcs)]
+
+    assert copied(mats, mats) == [False] * 10 and copied(mats, list(torch.zeros(10, 4, 6))) == [False] * 10
+    assert copied(mats, mats[1:] + mats[:1]) == [True] * 10
+    assert copied(mats, mats[:8] + [mats[9], mats[8]]) == [False] * 8 + [True] * 2
+    assert copied(mats, mats[:8] + [mats[8], torch.zeros(4, 6)]) == [False] * 10
+    wide = torch.zeros(4, 100)
+    assert copied([wide[:, :50], mats[0]], [mats[0], wide[:, 50:]]) == [True, True]
+    assert copied([mats[3][:2], mats[3][2:], mats[4]], [wide[:2, :6], mats[5][:2], mats[3]]) == [True, True, False]
