@@ -684,20 +684,27 @@ extern "C" int dvae_orthogonalize(const dvae_matrix_desc* mats, int32_t count, i
     for (int i = 0; i < count; ++i)
         DVAE_REQUIRE(mats[i].g && mats[i].out && mats[i].ld_g >= mats[i].cols && mats[i].ld_out >= mats[i].cols,
                      "orthogonalize: matrix %d has a null pointer or a row stride below its columns", i);
-    {  // the planes hold |X| <= 2, |A| <= 4, |B| < 8: follow the singular values through the steps
-        constexpr int GRID = 4096;
-        static thread_local float sigma[GRID + 1];
-        for (int i = 0; i <= GRID; ++i) sigma[i] = (float)i / GRID;
-        for (int t = 0; t < steps; ++t) {
-            const float a = coefficients[3 * t], b = coefficients[3 * t + 1], c = coefficients[3 * t + 2];
-            for (int i = 0; i <= GRID; ++i) {
-                const float l = sigma[i] * sigma[i], poly = b * l + c * l * l;
-                sigma[i] = (a + poly) * sigma[i];
-                // (the first step's B carries r <= 2)
-                DVAE_REQUIRE(fabsf(poly) * (t == 0 ? 2.f : 1.f) < 7.5f && fabsf(sigma[i]) < 1.95f,
-                             "orthogonalize: with the coefficients of step %d singular values leave [-2, 2]", t);
-            }
+    // The planes hold |X| <= 2, |A| <= 4, |B| < 8.  The singular values of X fill at most [0, most], whose image under the odd
+    // p(s) = a s + b s^3 + c s^5 is [0, max |p|] again in absolute values; with l = s^2 the maximum is at the end or where
+    // a + 3 b l + 5 c l^2 = 0, that of B's |b l + c l^2| at the end or at l = -b / 2 c.
+    double most = 1;
+    for (int t = 0; t < steps; ++t) {
+        const double a = coefficients[3 * t], b = coefficients[3 * t + 1], c = coefficients[3 * t + 2], end = most * most;
+        auto p_at = [&](double l) { return fabs((a + b * l + c * l * l) * sqrt(l)); };
+        auto b_at = [&](double l) { return fabs(b * l + c * l * l); };
+        double big = b_at(end);
+        most = p_at(end);
+        const double d = 9 * b * b - 20 * a * c;
+        // (both roots of the quadratic without cancellation; infinite ones, as with c = 0, lie outside)
+        const double q = d >= 0 ? -(3 * b + copysign(sqrt(d), b)) / 2 : 0, roots[3] = {q / (5 * c), a / q, -b / (2 * c)};
+        for (int i = 0; i < 3; ++i) {
+            if (!(roots[i] > 0 && roots[i] < end)) continue;
+            if (i < 2) most = fmax(most, p_at(roots[i]));
+            else big = fmax(big, b_at(roots[i]));
         }
+        DVAE_REQUIRE(most < 1.95, "orthogonalize: with the coefficients of step %d singular values leave [-2, 2]", t);
+        // (the first step's B carries r <= 2)
+        DVAE_REQUIRE(big * (t == 0 ? 2 : 1) < 7.5, "orthogonalize: the coefficients b and c of step %d are too large", t);
     }
     if (count == 0) return DVAE_OK;
     DVAE_REQUIRE(ws && (uintptr_t)ws % 16 == 0, "orthogonalize: the workspace must be 16-byte aligned");

@@ -495,7 +495,8 @@ int dvae_scan_step(const void* gate, int64_t ld_gate, const void* x, int64_t ld_
  * out = the last X of `steps` Newton-Schulz steps X <- a X + (b A + c A A) X, A = X X^T (on the smaller side), from
  * X = g / |g|_F, for `count` matrices of one element type (HOST array of descriptors; g, out device pointers, row strides in
  * elements; a matrix may be its own output, but no out overlaps another matrix's g or out).  coefficients (host): a, b, c of
- * every step, 3 * steps floats; sets that let a singular value leave [-2, 2] are refused.  fp32 accuracy (split fp16 planes, see
+ * every step, 3 * steps floats; sets that let a singular value leave [-2, 2] (or |b s^2 + c s^4|, twice that in the first step,
+ * reach 7.5) are refused.  fp32 accuracy (split fp16 planes, see
  * csrc/orthogonalize.hip), rounded once at the end; a zero matrix gives zeros, one that holds a NaN or an infinity gives NaN.
  * Sides up to 32768.
  * dtype DVAE_BF16 | DVAE_HALF_PRODUCTS: matrices with both sides of at least 512 multiply operands of 11 bits, at a third of the

@@ -179,3 +179,58 @@ def test_inputs_are_copied_only_where_another_output_shares_their_memory():
     wide = torch.zeros(4, 100)
     assert copied([wide[:, :50], mats[0]], [mats[0], wide[:, 50:]]) == [True, True]
     assert copied([mats[3][:2], mats[3][2:], mats[4]], [wide[:2, :6], mats[5][:2], mats[3]]) == [True, True, False]
+
+
+def accepts(triples):
+    lib = L.load()
+    flat = [v for t in triples for v in t]
+    return lib.dvae_orthogonalize((L.MatrixDesc * 1)(), 0, len(triples), (C.c_float * len(flat))(*flat), None, 0, None) == 0
+
+
+def walk(triples, samples):
+    """largest singular value and largest |b s^2 + c s^4| over the steps, by following samples of [0, 1]"""
+    import numpy as np
+    s, most, big = samples, 0.0, 0.0
+    for t, (a, b, c) in enumerate(np.float32(triples).astype(np.float64)):
+        l = s * s
+        big = max(big, float(np.abs(b * l + c * l * l).max()) * (2 if t == 0 else 1))
+        s = np.abs(s * (a + b * l + c * l * l))
+        most = max(most, float(s.max()))
+    return most, big
+
+
+def test_the_bound_on_coefficients_agrees_with_a_walk_over_samples():
+    import numpy as np
+    rng, samples = np.random.default_rng(0), np.linspace(0.0, 1.0, 20001)
+    seen = [0, 0]
+    for k in range(3000):
+        n = int(rng.integers(1, 3))
+        scale = rng.choice([1.0, 0.5, 0.25])
+        triples = (rng.uniform(-1, 1, (n, 3)) * [4, 6, 3] * scale).round(3)
+        triples[rng.random((n, 3)) < 0.1] = 0
+        most, big = walk(triples, samples)
+        # what the samples reach is reached; a point is at most 1 / 40000 from a sample and the slopes are at most 37 and 61,
+        # so that the samples fall short by less than 0.06
+        if most >= 1.95 or big >= 7.5:
+            assert not accepts(triples), (triples, most, big)
+            seen[0] += 1
+        elif most < 1.2 and big < 7:
+            assert accepts(triples), (triples, most, big)
+            seen[1] += 1
+    assert min(seen) > 200, seen
+
+
+def test_coefficients_whose_peak_lies_between_samples_are_refused():
+    quintic = (3.4445, -4.7750, 2.0315)
+    assert accepts([quintic] * 5) and accepts([quintic] * 32) and accepts([(1.5, -0.5, 0.0)] * 20) and accepts([(2.0, -1.5, 0.5)] * 12)
+    assert accepts([(0.0, 0.0, 0.0)] * 3) and accepts([(1.0, 0.0, 0.0)] * 32)
+    # all but singular values next to 1 shrink, those grow to 1.94 and then to 5: 4097 samples of [0, 1] miss them
+    narrow = [(0.6994, 1.0379, 0.2027), (0.1041, 0.0456, -0.0901), (-0.2401, 0.0324, 0.0787), (-0.1292, 0.4203, -0.1734),
+              (0.1413, -0.0517, 0.0743), (0.9625, -3.9394, 0.9085)]
+    import numpy as np
+    assert walk(narrow, np.linspace(0.0, 1.0, 4097))[0] < 1.95 and walk(narrow, np.linspace(0.999, 1.0, 100001))[0] > 5
+    assert accepts(narrow[:5]) and not accepts(narrow)
+    for bad in ((float("nan"), 0.0, 0.0), (0.0, float("inf"), 0.0), (0.0, 0.0, float("-inf")), (1.96, 0.0, 0.0), (-1.96, 0.0, 0.0)):
+        assert not accepts([bad])
+    # p stays below 1.84, but the first step's B, which carries the rest of the norm (up to 2), reaches 8
+    assert "b and c" in rc("dvae_orthogonalize", (L.MatrixDesc * 1)(), 0, 1, (C.c_float * 3)(4.5, -4.0, 0.0), None, 0, None)
