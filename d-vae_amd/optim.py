@@ -346,13 +346,13 @@ class FlatMuon(FlatAdam):
     matrices: names of the parameters that take this update; by default every weight matrix the train step touches except
     those that act on one-hot inputs (*.weight_ih, and the gates and mappers of DVAE_BN: rows of a table) and the last layers
     of the two predictors.  The rest, and `extra_params`, take Adam's with adam_lr, betas, eps.  param_groups[0] holds the
-    matrices (lr, momentum, nesterov, weight_decay), param_groups[1] the rest; schedulers see both."""
+    matrices (lr, momentum, nesterov, weight_decay, ns_steps, ns_coefficients, adjust_lr_fn), param_groups[1] the rest;
+    schedulers see both and checkpoints hold both."""
 
     def __init__(self, model, lr=2e-2, momentum=0.95, nesterov=True, weight_decay=0.0, adam_lr=1e-4, betas=(0.9, 0.999),
                  eps=1e-8, ns_steps=5, ns_coefficients=QUINTIC, adjust_lr_fn="original", matrices=None, reducer=None,
                  extra_params=None):
-        if adjust_lr_fn not in ("original", "match_rms_adamw"):
-            raise ValueError("adjust_lr_fn must be 'original' or 'match_rms_adamw'")
+        self._check_adjust(adjust_lr_fn)
         if not 0.0 <= momentum < 1.0 or lr < 0.0 or weight_decay < 0.0:
             raise ValueError("FlatMuon: momentum must lie in [0, 1), lr and weight_decay must not be negative")
         super(FlatMuon, self).__init__(model, lr=adam_lr, betas=betas, eps=eps, reducer=reducer, extra_params=extra_params)
@@ -369,22 +369,36 @@ class FlatMuon(FlatAdam):
                 raise ValueError("FlatMuon: %s is not a weight matrix of the train step" % k)
         self.matrices = [k for k in r.names if k in set(matrices)]
         self.is_matrix = [k in set(matrices) for k in r.names]
-        self.ns_steps, self.ns_coefficients = int(ns_steps), ns_coefficients
         rest = self.param_groups[0]
         first = dict(rest, params=[p for p, mat in zip(r.params, self.is_matrix) if mat], lr=lr, momentum=momentum,
-                     nesterov=bool(nesterov), weight_decay=weight_decay)
+                     nesterov=bool(nesterov), weight_decay=weight_decay, ns_steps=int(ns_steps), ns_coefficients=ns_coefficients,
+                     adjust_lr_fn=adjust_lr_fn)
         del first["betas"], first["eps"]
         rest["params"] = [p for p, mat in zip(r.params, self.is_matrix) if not mat]
         self.param_groups[:] = [first, rest]
+        self._set_factor()
+        self.flat_u = torch.zeros_like(self.flat_p)
+        self.updates = [self.flat_u[o:o + p.numel()].view_as(p) for p, o, mat in zip(r.params, r.offsets, self.is_matrix) if mat]
+
+    @staticmethod
+    def _check_adjust(fn):
+        if fn not in ("original", "match_rms_adamw"):
+            raise ValueError("adjust_lr_fn must be 'original' or 'match_rms_adamw'")
+
+    ns_steps = property(lambda self: self.param_groups[0]["ns_steps"])
+    ns_coefficients = property(lambda self: self.param_groups[0]["ns_coefficients"])
+
+    def _set_factor(self):
+        """the learning-rate factors of the matrices, for every 64 elements of the flat buffers; 0 elsewhere"""
+        r, fn = self.reducer, self.param_groups[0]["adjust_lr_fn"]
+        self._check_adjust(fn)
         factor = torch.zeros(r.numel // 64, dtype=torch.float32)
         for p, o, mat in zip(r.params, r.offsets, self.is_matrix):
             if mat:
                 rows, cols = p.shape
-                f = max(1.0, rows / cols) ** 0.5 if adjust_lr_fn == "original" else 0.2 * max(rows, cols) ** 0.5
+                f = max(1.0, rows / cols) ** 0.5 if fn == "original" else 0.2 * max(rows, cols) ** 0.5
                 factor[o // 64:(o + p.numel() + 63) // 64] = f
-        self.factor = factor.to(self.flat_p.device)
-        self.flat_u = torch.zeros_like(self.flat_p)
-        self.updates = [self.flat_u[o:o + p.numel()].view_as(p) for p, o, mat in zip(r.params, r.offsets, self.is_matrix) if mat]
+        self.factor, self._factor_fn = factor.to(self.flat_p.device), fn
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -392,6 +406,8 @@ class FlatMuon(FlatAdam):
         mats, rest = self.param_groups
         r = self.reducer
         self._check_views()
+        if mats["adjust_lr_fn"] != self._factor_fn:
+            self._set_factor()
         zero = int(bool(getattr(self.model, "_grad_sink", False)) and getattr(self.model, "_reducer", None) is r)
         n = self.flat_p.numel()
         self.steps += 1
@@ -401,7 +417,7 @@ class FlatMuon(FlatAdam):
                  int(mats["nesterov"]), float(rest["lr"]), float(rest["betas"][0]), float(rest["betas"][1]), float(rest["eps"]),
                  self.steps, zero)
         if self.updates:
-            orthogonalize(self.updates, self.ns_steps, self.ns_coefficients, out=self.updates)
+            orthogonalize(self.updates, mats["ns_steps"], mats["ns_coefficients"], out=self.updates)
             _enqueue(dev, "dvae_muon_apply_f32", self.flat_p.data_ptr(), self.flat_u.data_ptr(), self.factor.data_ptr(), n,
                      float(mats["lr"]), float(mats["weight_decay"]))
         r.clean = bool(zero)
@@ -446,6 +462,7 @@ class FlatMuon(FlatAdam):
         params, mats = self._ordered_params(), self._matrix_numbers()
         if list(sd["param_groups"][0]["params"]) != mats:
             raise ValueError("the state belongs to another choice of matrices")
+        self._check_adjust(sd["param_groups"][0].get("adjust_lr_fn", self.param_groups[0]["adjust_lr_fn"]))
         state = {}
         for i, st in sd["state"].items():
             if int(i) in mats:

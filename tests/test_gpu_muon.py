@@ -303,3 +303,38 @@ def test_flat_muon_refusals():
     with pytest.raises(dvae_amd._lib.DvaeHipError, match="singular values leave"):
         O.orthogonalize(m, coefficients=(4.0, 0.0, 0.0))
     assert O.orthogonalize([]) == []
+
+
+def test_flat_muon_checkpoint_holds_the_iteration_and_the_factor(tmp_path):
+    """resumed by an optimizer built with the defaults"""
+    model, ga = model_and_batch()
+    convergent = [(2.0, -1.5, 0.5)] * 7
+    opt = O.FlatMuon(model, lr=0.01, ns_steps=7, ns_coefficients=convergent, adjust_lr_fn="match_rms_adamw", nesterov=False, momentum=0.8)
+    g = gen(11)
+    eps = [torch.randn(24, 16, generator=g) for _ in range(2)]
+    opt.zero_grad()
+    grads_of(model, ga, eps[0])
+    opt.step()
+    dvae_amd.harness.save_checkpoint(str(tmp_path), 1, model, opt)
+    other, _ = model_and_batch(seed=5)
+    opt2 = O.FlatMuon(other)
+    dvae_amd.harness.load_module_state(other, str(tmp_path / "model_checkpoint1.pth"))
+    dvae_amd.harness.load_module_state(opt2, str(tmp_path / "optimizer_checkpoint1.pth"))
+    assert opt2.ns_steps == 7 and list(map(tuple, opt2.ns_coefficients)) == convergent
+    for m, o in ((model, opt), (other, opt2)):
+        o.zero_grad()
+        grads_of(m, ga, eps[1])
+    opt2.reducer.flat.copy_(opt.reducer.flat)  # (the step's own gradients vary in the last bits: atomics)
+    opt.step(), opt2.step()
+    assert torch.equal(opt.flat_p, opt2.flat_p) and torch.equal(opt.factor, opt2.factor)
+    old = opt.state_dict()  # a state without these keys keeps what the optimizer was built with
+    for k in ("ns_steps", "ns_coefficients", "adjust_lr_fn"):
+        del old["param_groups"][0][k]
+    opt3 = O.FlatMuon(model_and_batch()[0], ns_steps=3)
+    opt3.load_state_dict(old)
+    assert opt3.ns_steps == 3 and opt3.param_groups[0]["adjust_lr_fn"] == "original"
+    old["param_groups"][0]["adjust_lr_fn"] = "none"
+    before = opt3.exp_avg.clone()
+    with pytest.raises(ValueError, match="adjust_lr_fn"):
+        opt3.load_state_dict(old)
+    assert torch.equal(before, opt3.exp_avg)
