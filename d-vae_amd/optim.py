@@ -67,23 +67,8 @@ HALF_PRODUCTS = 16  # DVAE_HALF_PRODUCTS
 QUINTIC = (3.4445, -4.7750, 2.0315)  # p(s) = a s + b s^3 + c s^5: five steps take singular values from 0.002 up to 0.7 .. 1.2
 
 
-def orthogonalize(updates, steps=5, coefficients=QUINTIC, out=None, products="full"):
-    """The nearest (semi-)orthogonal matrix to each of `updates`, approximately: `steps` Newton-Schulz steps
-    X <- a X + (b A + c A A) X with A = X X^T (on the smaller side) from X = G / |G|_F.
-
-    updates: a matrix or a list of matrices (float32, bfloat16 or float16, one type, on one HIP device); a list goes through
-    every product in one launch.  coefficients: (a, b, c), or one such triple for each step; a set that lets a singular value
-    leave [-2, 2] is refused.  out: where to write (same shapes and type; matrices may be their own outputs, or each other's), default new tensors.
-    Accuracy of float32, rounded once to the matrices' type.  products="half" (bfloat16 only): matrices with both sides of at
-    least 512 multiply operands of 11 bits, for a third of the work; their error is then of the order of the result's own
-    rounding and adds to it.  What other matrices a call has changes a result by the order of its sums alone (float32).
-    A zero matrix gives zeros, one with a NaN or an infinity NaN.  Not differentiable (it acts on updates): inputs that need gradients are refused outside torch.no_grad()."""
-    one = torch.is_tensor(updates)
-    mats = [updates] if one else list(updates)
-    if out is not None:
-        outs = [out] if one else list(out)
-        if len(outs) != len(mats):
-            raise ValueError("out has %d matrices, updates %d" % (len(outs), len(mats)))
+def _iteration(steps, coefficients):
+    """(number of steps, their coefficients as the library takes them); refuses what the library would"""
     steps, coefficients = int(steps), list(coefficients)
     if not 1 <= steps <= 32:
         raise ValueError("steps must lie in 1 .. 32")
@@ -92,6 +77,31 @@ def orthogonalize(updates, steps=5, coefficients=QUINTIC, out=None, products="fu
     triples = [tuple(c) for c in coefficients]
     if len(triples) != steps or any(len(c) != 3 for c in triples):
         raise ValueError("coefficients must be (a, b, c) or one such triple for each of the %d steps" % steps)
+    abc = (C.c_float * (3 * steps))(*[v for c in triples for v in c])
+    _lib.check(_lib.load().dvae_orthogonalize((_lib.MatrixDesc * 1)(), 0, steps, abc, None, 0, None), "dvae_orthogonalize")  # of no matrix
+    return steps, abc
+
+
+def orthogonalize(updates, steps=5, coefficients=QUINTIC, out=None, products="full"):
+    """The nearest (semi-)orthogonal matrix to each of `updates`, approximately: `steps` Newton-Schulz steps
+    X <- a X + (b A + c A A) X with A = X X^T (on the smaller side) from X = G / |G|_F.
+
+    updates: a matrix or a list of matrices (float32, bfloat16 or float16, one type, on one HIP device); a list goes through
+    every product in one launch.  coefficients: (a, b, c), or one such triple for each step; a set that lets a singular value
+    leave [-2, 2] is refused.  out: where to write (same shapes and type; matrices may be their own outputs, or each other's),
+    default new tensors.  A zero matrix gives zeros, one with a NaN or an infinity NaN.  Not differentiable (it acts on updates):
+    inputs that need gradients are refused outside torch.no_grad().
+
+    Accuracy of float32, rounded once to the matrices' type.  products="half" (bfloat16 only): matrices with both sides of at
+    least 512 multiply operands of 11 bits, for a third of the work; their error is then of the order of the result's own
+    rounding and adds to it.  What other matrices a call has changes a result by the order of its sums alone (float32)."""
+    one = torch.is_tensor(updates)
+    mats = [updates] if one else list(updates)
+    if out is not None:
+        outs = [out] if one else list(out)
+        if len(outs) != len(mats):
+            raise ValueError("out has %d matrices, updates %d" % (len(outs), len(mats)))
+    steps, abc = _iteration(steps, coefficients)
     if not mats:
         return []
     if torch.is_grad_enabled() and any(torch.is_tensor(g) and g.requires_grad for g in mats):
@@ -132,7 +142,6 @@ def orthogonalize(updates, steps=5, coefficients=QUINTIC, out=None, products="fu
         descs = (_lib.MatrixDesc * len(mats))(*[
             _lib.MatrixDesc(g.data_ptr(), o.data_ptr(), g.stride(0) if g.shape[0] > 1 else g.shape[1],
                             o.stride(0) if o.shape[0] > 1 else o.shape[1], g.shape[0], g.shape[1]) for g, o in zip(srcs, outs)])
-        abc = (C.c_float * (3 * steps))(*[v for c in triples for v in c])
         ws = _workspace(lib.dvae_orthogonalize_ws_bytes(descs, len(mats), code), device, "dvae_orthogonalize_ws_bytes")
         _enqueue(device, "dvae_orthogonalize", descs, len(mats), steps, abc, ws.data_ptr(), code)
         if out is not None:
@@ -353,6 +362,7 @@ class FlatMuon(FlatAdam):
                  eps=1e-8, ns_steps=5, ns_coefficients=QUINTIC, adjust_lr_fn="original", matrices=None, reducer=None,
                  extra_params=None):
         self._check_adjust(adjust_lr_fn)
+        _iteration(ns_steps, ns_coefficients)
         if not 0.0 <= momentum < 1.0 or lr < 0.0 or weight_decay < 0.0:
             raise ValueError("FlatMuon: momentum must lie in [0, 1), lr and weight_decay must not be negative")
         super(FlatMuon, self).__init__(model, lr=adam_lr, betas=betas, eps=eps, reducer=reducer, extra_params=extra_params)
@@ -406,6 +416,8 @@ class FlatMuon(FlatAdam):
         mats, rest = self.param_groups
         r = self.reducer
         self._check_views()
+        # what may be refused is, before anything has moved
+        _iteration(mats["ns_steps"], mats["ns_coefficients"])
         if mats["adjust_lr_fn"] != self._factor_fn:
             self._set_factor()
         zero = int(bool(getattr(self.model, "_grad_sink", False)) and getattr(self.model, "_reducer", None) is r)
@@ -462,7 +474,9 @@ class FlatMuon(FlatAdam):
         params, mats = self._ordered_params(), self._matrix_numbers()
         if list(sd["param_groups"][0]["params"]) != mats:
             raise ValueError("the state belongs to another choice of matrices")
-        self._check_adjust(sd["param_groups"][0].get("adjust_lr_fn", self.param_groups[0]["adjust_lr_fn"]))
+        first = dict(self.param_groups[0], **sd["param_groups"][0])
+        self._check_adjust(first["adjust_lr_fn"])
+        _iteration(first["ns_steps"], first["ns_coefficients"])
         state = {}
         for i, st in sd["state"].items():
             if int(i) in mats:

@@ -338,3 +338,24 @@ def test_flat_muon_checkpoint_holds_the_iteration_and_the_factor(tmp_path):
     with pytest.raises(ValueError, match="adjust_lr_fn"):
         opt3.load_state_dict(old)
     assert torch.equal(before, opt3.exp_avg)
+
+
+def test_flat_muon_refuses_an_iteration_before_anything_moves():
+    model, ga = model_and_batch()
+    for bad in (dict(ns_coefficients=(4.0, 0.0, 0.0)), dict(ns_coefficients=(1.0, 2.0)), dict(ns_steps=0), dict(ns_coefficients=[(1.5, -0.5, 0.0)] * 2)):
+        with pytest.raises((ValueError, dvae_amd._lib.DvaeHipError)):
+            O.FlatMuon(model_and_batch()[0], **bad)
+    opt = O.FlatMuon(model)
+    opt.zero_grad()
+    grads_of(model, ga, torch.randn(24, 16, generator=gen(12)))
+    opt.param_groups[0]["ns_coefficients"] = (4.0, 0.0, 0.0)
+    kept = [t.clone() for t in (opt.flat_p, opt.exp_avg, opt.exp_avg_sq, opt.reducer.flat)]
+    with pytest.raises(dvae_amd._lib.DvaeHipError, match="singular values leave"):
+        opt.step()
+    assert opt.steps == 0 and all(torch.equal(a, b) for a, b in zip(kept, (opt.flat_p, opt.exp_avg, opt.exp_avg_sq, opt.reducer.flat)))
+    state = opt.state_dict()
+    with pytest.raises(dvae_amd._lib.DvaeHipError, match="singular values leave"):
+        O.FlatMuon(model_and_batch()[0]).load_state_dict(state)
+    opt.param_groups[0]["ns_coefficients"] = O.QUINTIC
+    opt.step()
+    assert opt.steps == 1 and not torch.equal(kept[0], opt.flat_p)
