@@ -32,6 +32,7 @@ constexpr int TILE_THREADS = 256;
 constexpr int TILE_N = TILE_THREADS * SORT_ITEMS;
 constexpr int MAX_SORT_BLOCKS = 256; // every block of a pass reads every block's digit counts
 constexpr int ZERO_ROWS = 64;       // table rows per zeroing workgroup
+constexpr int JOIN_THREADS = 512;
 
 // ---------------------------------------------------------------------------------------------------------- lookup
 __device__ __forceinline__ int token_key(const void* ids, int i64, long i, int V) {
@@ -339,7 +340,7 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const T* __restrict__ do
 // The run that begins in this chunk and goes on in the next: its partials are summed per wave in chunk order, then the
 // waves' sums in wave order.  The eight waves are G groups of 256 columns times 8 / G shares of the partials.
 template <typename T>
-__global__ __launch_bounds__(512) void embed_join_kernel(const int* __restrict__ key, int n, int vocab, int D, float scale,
+__global__ __launch_bounds__(JOIN_THREADS) void embed_join_kernel(const int* __restrict__ key, int n, int vocab, int D, float scale,
                                                          T* __restrict__ dw, const float* __restrict__ part, int G) {
     constexpr int U = 8;
     __shared__ float sums[8][256];
@@ -411,6 +412,14 @@ static int embed_sizes(const char* who, int64_t n, int64_t vocab, int32_t D, int
     DVAE_REQUIRE(D >= 1 && D <= (1 << 20), "%s: row length %d is not in 1 .. 2^20", who, D);
     return DVAE_OK;
 }
+// the gradient's launches: a workgroup per chunk of tokens, and one per ZERO_ROWS rows of the table
+static int embed_grad_sizes(const char* who, int64_t n, int64_t vocab, int32_t D, int32_t dtype) {
+    DVAE_TRY(embed_sizes(who, n, vocab, D, dtype));
+    DVAE_REQUIRE(grid_fits((n + EC - 1) / EC, JOIN_THREADS), "%s: %lld tokens are not supported; at most 2^28 - 32", who, (long long)n);
+    DVAE_REQUIRE(grid_fits((vocab + ZERO_ROWS - 1) / ZERO_ROWS, 256), "%s: a table of %lld rows is not supported; at most 2^30 - 64", who,
+                 (long long)vocab);
+    return DVAE_OK;
+}
 
 }  // namespace dvae
 
@@ -436,19 +445,25 @@ extern "C" int dvae_embed_fwd(const void* w, int64_t ld_w, const void* ids, int3
 
 extern "C" int64_t dvae_embed_bwd_ws_bytes(int64_t n, int64_t vocab, int32_t D) {
     using namespace dvae;
-    DVAE_TRY(embed_sizes("embed_bwd_ws_bytes", n, vocab, D, DVAE_F32));
+    DVAE_TRY(embed_grad_sizes("embed_bwd_ws_bytes", n, vocab, D, DVAE_F32));
     return embed_ws(n, vocab, D).bytes;
 }
 
 extern "C" int dvae_embed_bwd(const void* dout, int64_t ld_dout, const void* ids, int32_t ids_i64, void* dw, void* ws, int64_t n,
                               int64_t vocab, int32_t D, float scale, int32_t dtype, void* stream) {
     using namespace dvae;
-    DVAE_TRY(embed_sizes("embed_bwd", n, vocab, D, dtype));
+    DVAE_TRY(embed_grad_sizes("embed_bwd", n, vocab, D, dtype));
     DVAE_REQUIRE(ld_dout == 0 || ld_dout >= D, "embed_bwd: row stride %lld is below the row length %d", (long long)ld_dout, D);
     DVAE_REQUIRE(dw, "embed_bwd: null pointer");
     DVAE_REQUIRE(n == 0 || (dout && ids && ws), "embed_bwd: null pointer");
     DVAE_REQUIRE((uintptr_t)ws % 16 == 0, "embed_bwd: the workspace must be 16-byte aligned");
     const EmbedWs L = embed_ws(n, vocab, D);
+    const int es = elem_size(dtype);
+    const int vec = widest(es, 16, {(int64_t)D, ld_dout}, {(const void*)dout, (const void*)dw});
+    const int slabs = cdiv(D, 64 * vec), zero_blocks = cdiv(vocab, ZERO_ROWS);
+    const long units = (long)L.chunks * slabs;
+    const long sum_blocks = (units + 3) / 4;
+    DVAE_REQUIRE(grid_fits(sum_blocks + zero_blocks, 256), "embed_bwd: %lld tokens of %d elements are too many", (long long)n, D);
     hipStream_t s = (hipStream_t)stream;
     char* b = (char*)ws;
     int at = 0;  // which of the two lists holds the sorted tokens
@@ -468,12 +483,6 @@ extern "C" int dvae_embed_bwd(const void* dout, int64_t ld_dout, const void* ids
             DVAE_LAUNCH_CHECK();
         }
     }
-    const int es = elem_size(dtype);
-    const int vec = widest(es, 16, {(int64_t)D, ld_dout}, {(const void*)dout, (const void*)dw});
-    const int slabs = cdiv(D, 64 * vec), zero_blocks = cdiv(vocab, ZERO_ROWS);
-    const long units = (long)L.chunks * slabs;
-    const long sum_blocks = (units + 3) / 4;
-    DVAE_REQUIRE(sum_blocks + zero_blocks < (1LL << 31), "embed_bwd: too many rows");
     const int* key = (const int*)(b + L.key[at]);
     const int* pos = (const int*)(b + L.pos[at]);
     float* part = (float*)(b + L.part);
@@ -486,7 +495,7 @@ extern "C" int dvae_embed_bwd(const void* dout, int64_t ld_dout, const void* ids
     if (L.chunks > 1) {
         const int groups = D <= 256 ? 1 : D <= 512 ? 2 : D <= 1024 ? 4 : 8;
 #define EMBED_JOIN(T)                                                                                                        \
-    hipLaunchKernelGGL((embed_join_kernel<T>), dim3(L.chunks), dim3(512), 0, s, key, (int)n, (int)vocab, D, scale, (T*)dw, \
+    hipLaunchKernelGGL((embed_join_kernel<T>), dim3(L.chunks), dim3(JOIN_THREADS), 0, s, key, (int)n, (int)vocab, D, scale, (T*)dw, \
                        (const float*)part, groups)
         if (dtype == DVAE_F32) EMBED_JOIN(float);
         else if (dtype == DVAE_BF16) EMBED_JOIN(__bf16);

@@ -111,6 +111,7 @@ constexpr float A_MIN = 1.17549435e-38f;
 // scope; a word that still holds the fill pattern has not been published, so no fences are needed.
 constexpr int LOOK = 8;
 constexpr unsigned long long UNSET = ~0ull;
+constexpr long FILL_BLOCKS = 2048;  // at most, before a pass
 constexpr int SPINS = 1 << 22;  // never reached: every tile waits for earlier tickets only; then NaN rather than a hang
 __device__ __forceinline__ void publish(unsigned long long* at, float A, float B) {
     const unsigned long long w = ((unsigned long long)__float_as_uint(A) << 32) | __float_as_uint(B);
@@ -627,12 +628,22 @@ static long scan_empty_blocks(const ScanParams& p, const float* to) {
     return to && p.q.S > 0 && (p.q.off || p.q.len == 0) ? (p.q.S + 3) / 4 : 0;
 }
 
+// the launches of a pass: one workgroup per tile and slab, and those that look for sequences without rows beside them or, with
+// several tiles, in the launch before
+static int scan_grid(const char* who, const ScanParams& p, const ScanWs& L, int threads, const float* to, dim3& grid) {
+    const long empty = scan_empty_blocks(p, to), blocks = L.tiles * p.slabs + (L.tiles == 1 ? empty : 0);
+    DVAE_REQUIRE(grid_fits(blocks, threads) && grid_fits(FILL_BLOCKS + empty, 256), "%s: %lld rows of %d channels in %lld sequences are too many", who,
+                 (long long)p.q.N, p.D, (long long)p.q.S);
+    grid = dim3((unsigned)blocks);
+    return DVAE_OK;
+}
+
 static int scan_begin(ScanParams& p, void* ws, const ScanWs& L, const float* from, float* to, hipStream_t s) {
     p.words = (unsigned long long*)((char*)ws + L.words);
     if (L.tiles == 1) return DVAE_OK;
     p.ticket = (unsigned*)ws;
     const long pairs = (L.tiles * p.D + 1) / 2;
-    const int fill = L.tiles == 0 ? 0 : (int)min((pairs + 255) / 256, 2048L);
+    const int fill = L.tiles == 0 ? 0 : (int)min((pairs + 255) / 256, FILL_BLOCKS);
     const long blocks = fill + scan_empty_blocks(p, to);
     if (blocks == 0) return DVAE_OK;
     hipLaunchKernelGGL(scan_begin_kernel, dim3((unsigned)blocks), dim3(256), 0, s, (ulonglong2*)p.words, pairs, p.ticket, fill,
@@ -670,10 +681,10 @@ extern "C" int dvae_scan_fwd(const void* gate, int64_t ld_gate, const void* x, i
     p.gate = gate; p.x = x; p.ld_gate = ld_gate; p.ld_x = ld_x; p.h = h; p.h0 = h0; p.last = last; p.states = states;
     p.q = {off, off_i64, seqs, seqs > 0 ? rows / seqs : 0, rows};
     p.D = D; p.slabs = cdiv(D, 64 * vec);
-    DVAE_REQUIRE(L.tiles * p.slabs < (1LL << 31), "scan_fwd: %lld rows of %d channels are too many", (long long)rows, D);
+    dim3 grid;
+    DVAE_TRY(scan_grid("scan_fwd", p, L, TRF / RW * 64, last, grid));
     DVAE_TRY(scan_begin(p, ws, L, h0, last, s));
     if (rows == 0) return DVAE_OK;
-    const dim3 grid((unsigned)(L.tiles * p.slabs + (p.ticket ? 0 : scan_empty_blocks(p, last))));
 #define SCAN_FWD(T, V) hipLaunchKernelGGL((scan_fwd_kernel<T, V>), grid, dim3(TRF / RW * 64), 0, s, p)
     SCAN_BY_TYPE(dtype, vec, SCAN_FWD);
 #undef SCAN_FWD
@@ -700,10 +711,10 @@ extern "C" int dvae_scan_bwd(const void* gate, int64_t ld_gate, const void* x, i
     p.dgate = dgate; p.dx = dx; p.h0 = h0; p.dlast = dlast; p.dh0 = dh0; p.states = const_cast<float*>(states);
     p.q = {off, off_i64, seqs, seqs > 0 ? rows / seqs : 0, rows};
     p.D = D; p.slabs = cdiv(D, 64 * vec);
-    DVAE_REQUIRE(L.tiles * p.slabs < (1LL << 31), "scan_bwd: %lld rows of %d channels are too many", (long long)rows, D);
+    dim3 grid;
+    DVAE_TRY(scan_grid("scan_bwd", p, L, TRB / RW * 64, dh0, grid));
     DVAE_TRY(scan_begin(p, ws, L, dlast, dh0, s));
     if (rows == 0) return DVAE_OK;
-    const dim3 grid((unsigned)(L.tiles * p.slabs + (p.ticket ? 0 : scan_empty_blocks(p, dh0))));
 #define SCAN_BWD(T, V) hipLaunchKernelGGL((scan_bwd_kernel<T, V>), grid, dim3(TRB / RW * 64), 0, s, p)
     SCAN_BY_TYPE(dtype, vec, SCAN_BWD);
 #undef SCAN_BWD
@@ -727,7 +738,7 @@ extern "C" int dvae_scan_step(const void* gate, int64_t ld_gate, const void* x, 
     const int vec = widest(elem_size(dtype), 16, {(int64_t)D, ld_gate, ld_x}, {gate, x, (const void*)h});
     const int slabs = cdiv(D, 64 * vec);
     const long units = (long)rows * slabs;
-    DVAE_REQUIRE(units < (1LL << 31), "scan_step: %d rows of %d channels are too many", rows, D);
+    DVAE_REQUIRE(grid_fits((units + 3) / 4, 256), "scan_step: %d rows of %d channels are too many", rows, D);
     const dim3 grid((unsigned)((units + 3) / 4));
 #define SCAN_STEP_BY(T, V, I)                                                                                                   \
     hipLaunchKernelGGL((scan_step_kernel<T, V, I>), grid, dim3(256), 0, (hipStream_t)stream, (const T*)gate, (long)ld_gate,       \

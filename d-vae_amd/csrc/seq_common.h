@@ -51,6 +51,9 @@ __device__ __forceinline__ void hold(float& v) { asm volatile("" : "+v"(v)); }
 static inline int elem_size(int dtype) { return dtype == DVAE_F32 ? 4 : 2; }
 static inline bool known_dtype(int dtype) { return dtype == DVAE_F32 || dtype == DVAE_BF16 || dtype == DVAE_F16; }
 
+// the runtime takes less than 2^32 threads along a grid
+static inline bool grid_fits(int64_t blocks, int threads) { return blocks * threads < (1LL << 32); }
+
 // The widest vector (in elements, at most `bytes` bytes) that divides every listed extent / stride and to which every
 // base pointer is aligned.  An odd row length leaves single elements, which a wave still reads as one 128- or 256-byte run.
 template <size_t NE, size_t NP>

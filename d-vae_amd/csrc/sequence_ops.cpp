@@ -154,7 +154,11 @@ std::tuple<Tensor, Tensor, Tensor> scan_forward(const Tensor& gate, const Tensor
     const at::Device dev = x.device();
     const at::TensorOptions f32 = at::TensorOptions(at::kFloat).device(dev);
     Tensor h = at::empty(x.sizes(), at::TensorOptions(x.scalar_type()).device(dev)), last = at::empty({seqs, D}, f32), states;
-    if (keep) states = at::empty({call(p_dvae_scan_state_floats, g.n, D)}, f32);
+    if (keep) {
+        const int64_t floats = call(p_dvae_scan_state_floats, g.n, D);
+        if (floats < 0) fail("dvae_scan_state_floats", floats);
+        states = at::empty({floats}, f32);
+    }
     Tensor ws = workspace("dvae_scan_ws_bytes", call(p_dvae_scan_ws_bytes, g.n, D), dev);
     enqueue("dvae_scan_fwd", dev, p_dvae_scan_fwd, g.p(), g.ld, y.p(), y.ld, ptr(offsets), wide(offsets), (const float*)ptr(h0), h.data_ptr(),
             (float*)last.data_ptr(), keep ? (float*)states.data_ptr() : nullptr, ws.data_ptr(), g.n, seqs, D, code(x));

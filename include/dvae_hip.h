@@ -461,7 +461,8 @@ int dvae_embed_fwd(const void* w, int64_t ld_w, const void* ids, int32_t ids_i64
                    int32_t D, float scale, int32_t dtype, void* stream);
 /* dw[v][0:D] = scale * sum over t with ids[t] = v of dout[t][0:D] (dw [vocab][D] contiguous, every row written; dout rows
  * of stride ld_dout, 0 = one row for all; tokens outside [0, vocab) take no part).  Sums in fp32 over the sorted tokens,
- * rounded once; the result does not vary from run to run.  ws: dvae_embed_bwd_ws_bytes() bytes, 16-byte aligned. */
+ * rounded once; the result does not vary from run to run.  Up to 2^28 - 32 tokens and 2^30 - 64 rows.
+ * ws: dvae_embed_bwd_ws_bytes() bytes, 16-byte aligned. */
 int64_t dvae_embed_bwd_ws_bytes(int64_t n, int64_t vocab, int32_t D);
 int dvae_embed_bwd(const void* dout, int64_t ld_dout, const void* ids, int32_t ids_i64, void* dw, void* ws, int64_t n,
                    int64_t vocab, int32_t D, float scale, int32_t dtype, void* stream);
@@ -470,8 +471,9 @@ int dvae_embed_bwd(const void* dout, int64_t ld_dout, const void* ids, int32_t i
  * sequence s is the rows [off[s], off[s+1]) (off: seqs + 1 values that do not decrease, int32 or int64; NULL: sequences of
  * rows / seqs rows each); values outside [0, rows] count as the nearer end.  The state before a sequence is h0[s] (fp32
  * [seqs][D]; NULL: zeros).  gate, x: row strides ld_* in elements (halves of one projection's output are allowed; 0 = one
- * row for all; at most 2^23); h [rows][D] contiguous, rounded once; last [seqs][D] fp32: the state after each sequence (h0 where it is
- * empty).  Rows of no sequence give zeros.  states: dvae_scan_state_floats() floats that the backward pass reads (NULL if
+ * row for all; at most 2^23); h [rows][D] contiguous, rounded once; last [seqs][D] fp32: the state after each sequence (h0
+ * where it is empty).  rows times D / 64, rounded up, stays below 2^30 - 128, and there are less than 2^26 - 8192 sequences
+ * (without off and with rows: any number).  Rows of no sequence give zeros.  states: dvae_scan_state_floats() floats that the backward pass reads (NULL if
  * there is none); ws: dvae_scan_ws_bytes() bytes, 16-byte aligned, for this call alone. */
 int64_t dvae_scan_state_floats(int64_t rows, int32_t D);
 int64_t dvae_scan_ws_bytes(int64_t rows, int32_t D);

@@ -234,3 +234,20 @@ def test_coefficients_whose_peak_lies_between_samples_are_refused():
         assert not accepts([bad])
     # p stays below 1.84, but the first step's B, which carries the rest of the norm (up to 2), reaches 8
     assert "b and c" in rc("dvae_orthogonalize", (L.MatrixDesc * 1)(), 0, 1, (C.c_float * 3)(4.5, -4.0, 0.0), None, 0, None)
+
+
+def test_what_no_launch_can_hold_is_refused_before_the_first_one():
+    """a grid has less than 2^32 threads"""
+    p, lib = C.c_void_p(4096), L.load()
+    most = (1 << 28) - 32
+    assert lib.dvae_embed_bwd_ws_bytes(most, 8, 8) > 0 and "tokens" in rc("dvae_embed_bwd_ws_bytes", most + 1, 8, 8)
+    assert lib.dvae_embed_bwd_ws_bytes(8, (1 << 30) - 64, 8) > 0 and "table" in rc("dvae_embed_bwd_ws_bytes", 8, (1 << 30) - 63, 8)
+    assert "tokens" in rc("dvae_embed_bwd", p, 8, p, 0, p, p, most + 1, 4, 8, 1.0, 0, None)
+    assert "too many" in rc("dvae_embed_bwd", p, 4096, p, 0, p, p, most, 4, 4096, 1.0, 0, None)
+    for name, args in (("dvae_scan_fwd", (p, 65, p, 65, p, 0, None, p, p, None, p)), ("dvae_scan_bwd", (p, 65, p, 65, p, 0, None, p, p, 65, p, p, p, p, p))):
+        assert "too many" in rc(name, *args, 1 << 30, 2, 64, 0, None)
+        assert "too many" in rc(name, *args, 1 << 29, 2, 65, 0, None)  # two slabs of 64 channels
+        assert "too many" in rc(name, *args, 300, 1 << 26, 64, 0, None)
+        assert "too many" in rc(name, *args, 30, 1 << 26, 64, 0, None)  # one tile
+        assert "too many" in rc(name, *args, 0, 1 << 26, 64, 0, None)
+    assert "too many" in rc("dvae_scan_step", p, 1 << 13, p, 1 << 13, p, 1 << 13, 1 << 24, None, 0, p, 1 << 24, 1 << 13, 0, None)
