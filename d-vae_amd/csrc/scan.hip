@@ -13,7 +13,7 @@
 //
 // Layout: N rows (time, all sequences end to end) x D channels.  A workgroup's tile is W waves x RW rows by 64 V channels;
 // each wave holds its RW rows in registers, the waves compose their (A, B) through LDS.  The tiles do not follow the
-// sequences: a sequence's first row just makes A = 0, so that many short sequences and one long one cost the same.  All
+// sequences: a sequence's first row just makes A = -0, so that many short sequences and one long one cost the same.  All
 // states, products and sums are fp32; outputs are rounded once.
 //
 // One pass over the data in either direction (forward 3, backward 5 matrices of memory traffic), tiles chained through
@@ -99,10 +99,15 @@ __device__ __forceinline__ void gate_of_code(float code, float& z, float& omz) {
     omz = open ? less : more;
 }
 
-// A run of rows as a map of the state (or of the gradient that flows back) before it: s -> A s + B.  A = 0 says that a
-// sequence begins inside, so that nothing of s is left, not even a NaN; a product of gates is kept above 0 for that.
-__device__ __forceinline__ float through(float A, float B, float s) { return A == 0.f ? B : fmaf(A, s, B); }
-constexpr float A_MIN = 1.17549435e-38f;
+// A run of rows as a map of the state (or of the gradient that flows back) before it: s -> A s + B.  A = -0 says that a
+// sequence begins inside, so that nothing of s is left, not even a NaN; a product of gates is never below +0.  (Told from that by
+// its sign, not by keeping products above 0: a state of 1e38, as inputs masked with their type's lowest value leave it, comes
+// through the smallest number above 0 with a size of 1 behind gates that are closed.)
+constexpr unsigned BEGINS = 0x80000000u;
+__device__ __forceinline__ bool begins(float A) { return __float_as_uint(A) == BEGINS; }
+__device__ __forceinline__ float through(float A, float B, float s) { return begins(A) ? B : fmaf(A, s, B); }
+// two runs, the later one first
+__device__ __forceinline__ float both(float A, float before) { return begins(A) || begins(before) ? __uint_as_float(BEGINS) : A * before; }
 
 // Carries between the tiles of a slab.  Every tile publishes its (A, B) per channel as soon as it has it, and then the
 // state behind it as (0, state), which is the same map with everything before it folded in.  A tile looks back over up to
@@ -131,21 +136,21 @@ __device__ __forceinline__ float look_back(const unsigned long long* nearest, lo
     do {
         open = true;
 #pragma unroll
-        for (int i = 0; i < LOOK; ++i) w[i] = i < n ? read_word(nearest + i * step) : 0;  // 0: before the first tile the state is 0
+        for (int i = 0; i < LOOK; ++i) w[i] = i < n ? read_word(nearest + i * step) : (unsigned long long)BEGINS << 32;
 #pragma unroll
         for (int i = 0; i < LOOK; ++i) {
             open = open && w[i] != UNSET;
-            if ((w[i] >> 32) == 0) break;  // whole: nothing farther matters
+            if ((w[i] >> 32) == BEGINS) break;  // whole: nothing farther matters
         }
     } while (!__all(open) && ++spins < SPINS);
     bool whole = count < LOOK;
 #pragma unroll
-    for (int i = 0; i < LOOK; ++i) whole = whole || (w[i] >> 32) == 0;
+    for (int i = 0; i < LOOK; ++i) whole = whole || (w[i] >> 32) == BEGINS;
     if (count == LOOK) whole = true;
     while (!__all(whole) && ++spins < SPINS) {
         __builtin_amdgcn_s_sleep(1);
         const unsigned long long far = read_word(nearest + (LOOK - 1) * step);
-        if (!whole && (far >> 32) == 0) { w[LOOK - 1] = far; whole = true; }
+        if (!whole && (far >> 32) == BEGINS) { w[LOOK - 1] = far; whole = true; }
     }
     float s = spins < SPINS ? 0.f : __uint_as_float(0x7FC00000u);
 #pragma unroll
@@ -271,7 +276,7 @@ __global__ __launch_bounds__(TRF / RW * 64) void scan_fwd_kernel(ScanParams p) {
     if (plain) local(No()); else local(Yes());
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        As[wave][lane * V + j] = m.start ? 0.f : fmaxf(A[j], A_MIN);
+        As[wave][lane * V + j] = m.start ? __uint_as_float(BEGINS) : A[j];
         Bs[wave][lane * V + j] = h[j];
     }
     __syncthreads();
@@ -281,12 +286,12 @@ __global__ __launch_bounds__(TRF / RW * 64) void scan_fwd_kernel(ScanParams p) {
 #pragma unroll
         for (int w = 0; w < W; ++w) {
             y = through(As[w][k], Bs[w][k], y);
-            a = As[w][k] == 0.f ? 0.f : a == 0.f ? 0.f : fmaxf(a * As[w][k], A_MIN);
+            a = both(As[w][k], a);
         }
         unsigned long long* word = p.words + tile * p.D + c0 + k;
         publish(word, a, y);
         const float s = tile == 0 ? 0.f : look_back(word - p.D, -(long)p.D, tile);
-        if (a != 0.f) publish(word, 0.f, through(a, y, s));
+        if (!begins(a)) publish(word, __uint_as_float(BEGINS), through(a, y, s));
         Cs[k] = s;
     }
     __syncthreads();
@@ -409,7 +414,7 @@ __global__ __launch_bounds__(TRB / RW * 64) void scan_bwd_kernel(ScanParams p) {
     if (plain) local(No()); else local(Yes());
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        As[wave][lane * V + j] = m.start ? 0.f : fmaxf(A[j], A_MIN);
+        As[wave][lane * V + j] = m.start ? __uint_as_float(BEGINS) : A[j];
         Bs[wave][lane * V + j] = B[j];
         Fs[wave][lane * V + j] = h[j];
     }
@@ -420,12 +425,12 @@ __global__ __launch_bounds__(TRB / RW * 64) void scan_bwd_kernel(ScanParams p) {
 #pragma unroll
         for (int w = W - 1; w >= 0; --w) {
             y = through(As[w][k], Bs[w][k], y);
-            a = As[w][k] == 0.f ? 0.f : a == 0.f ? 0.f : fmaxf(a * As[w][k], A_MIN);
+            a = both(As[w][k], a);
         }
         unsigned long long* word = p.words + tile * p.D + c0 + k;
         publish(word, a, y);
         const float s = tile == tiles - 1 ? 0.f : look_back(word + p.D, p.D, tiles - 1 - tile);
-        if (a != 0.f) publish(word, 0.f, through(a, y, s));
+        if (!begins(a)) publish(word, __uint_as_float(BEGINS), through(a, y, s));
         Cs[k] = s;
     }
     __syncthreads();
