@@ -476,7 +476,8 @@ __global__ __launch_bounds__(TRB / RW * 64) void scan_bwd_kernel(ScanParams p) {
                 float z, omz;
                 gate_of_code(code[i][j], z, omz);
                 const float G = e[j] + C[j];
-                og[j] = cover ? G * (prev[i][j] - (float)x[i].e[j]) * z * omz : 0.f;
+                // (the gates first: z (1 - z) keeps what a closed one meets, an input of its type's lowest value, from overflowing)
+                og[j] = cover ? G * z * omz * (prev[i][j] - (float)x[i].e[j]) : 0.f;
                 ox[j] = cover ? G * omz : 0.f;
                 if (cover) C[j] = z * G;
             }

@@ -41,3 +41,27 @@ def test_masked_rows_leave_nothing_behind_a_closed_gate(dtype):
     close(h[~keep.cuda()], ref[~keep], float(ref[rows].abs().max()) * 64 * U, "masked rows")
     one = S.gated_step(gate[16:17].cuda(), x[16:17].cuda(), h[15:16].float())
     close(one, ref[16:17], tol, "step")
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+def test_gradients_of_masked_rows_are_finite(dtype):
+    gate, x, keep, rows = masked(dtype)
+    dt, g, off = DT[dtype], gen(4), [0, 300]
+    dh = torch.randn(x.shape, generator=g).clamp(-2, 2).to(dt)  # nothing comes back through a closed gate: G = dh in a masked row
+    dlast = torch.randn(1, x.shape[1], generator=g)
+    ref = plain_scan(gate.double(), x.double(), off, None, dh.double(), dlast.double())
+    leaves = [gate.cuda().requires_grad_(True), x.cuda().requires_grad_(True)]
+    h, last = S.gated_scan(*leaves, torch.tensor(off).cuda())
+    dg, dx = torch.autograd.grad([h, last], leaves, [dh.cuda(), dlast.cuda()])
+    big = max(ref[5], 1.0)
+    tol_G, tol_h = (8 * 149 + 32) * U * big, (8 * 149 + 32) * U * 3.0
+    close(dx, ref[3], tol_G + 4 * U * big, "dx")
+    closed = keep.clone()
+    closed[:] = False
+    closed[rows + 1] = True
+    closed[192] = True
+    plain = keep & ~closed
+    close(dg[plain.cuda()], ref[2][plain], (tol_G * 6 + big * tol_h + 32 * U * big * 6) / 4, "dgate")
+    assert not dg[closed.cuda()].any()  # z (1 - z) is 0 in 32 bits, whatever the state before
+    # a masked row: G = dh exactly, (prev - x) z (1 - z) off by its roundings alone, a few u relative (and u |h| of prev)
+    close(dg[rows.cuda()], ref[2][rows], ref[2][rows].abs() * 32 * U + 2 * tol_h, "dgate of masked rows")
