@@ -74,12 +74,14 @@ Tensor workspace(const char* what, int64_t bytes, at::Device device) {
     return at::empty({bytes}, at::TensorOptions(at::kByte).device(device));
 }
 
+// Tensors whose elements torch holds negated (x.conj().imag) are written out first, here and below: the library reads memory.
 // The rows of a [N, D] or [B, T, D] matrix whose elements lie side by side in a row: in place where the rows have one
 // stride of at most 2^23 elements (the recurrence addresses a few rows with 32-bit offsets), else of a copy.
 struct Rows {
     Tensor keep;
     int64_t n, d, ld;
-    explicit Rows(const Tensor& t) : keep(t), d(t.size(-1)) {
+    explicit Rows(const Tensor& given) : keep(given.resolve_neg()), d(given.size(-1)) {
+        const Tensor t = keep;
         const bool flat = t.dim() == 2;
         const int64_t B = t.size(0), T = flat ? 1 : t.size(1), step = flat || T == 1 ? t.stride(0) : t.stride(1);
         n = B * T;
@@ -141,8 +143,9 @@ struct Embed : torch::autograd::Function<Embed> {
 
 Tensor embed(const Tensor& weight, const Tensor& ids, double scale) {
     no_tangent("embed", weight);
-    if (weight.requires_grad() && at::GradMode::is_enabled()) return Embed::apply(weight, ids, scale);
-    return embed_forward(weight, ids, scale);
+    const Tensor w = weight.resolve_neg();
+    if (w.requires_grad() && at::GradMode::is_enabled()) return Embed::apply(w, ids, scale);
+    return embed_forward(w, ids, scale);
 }
 
 // --------------------------------------------------------------------------------------------------------- recurrence
@@ -185,7 +188,7 @@ struct Scan : torch::autograd::Function<Scan> {
         const at::Device dev = x.device();
         std::optional<Rows> dh;
         if (grads[0].defined()) dh.emplace(grads[0]);
-        const Maybe dlast = grads[1].defined() ? Maybe(grads[1].contiguous()) : Maybe();
+        const Maybe dlast = grads[1].defined() ? Maybe(grads[1].resolve_neg().contiguous()) : Maybe();
         const at::TensorOptions like = at::TensorOptions(x.scalar_type()).device(dev);
         Tensor dgate = at::empty(gate.sizes(), like), dx = at::empty(x.sizes(), like), dh0;
         // (the edges are those of the tensors that were given: gate, x, offsets if any, h0)
@@ -198,8 +201,9 @@ struct Scan : torch::autograd::Function<Scan> {
     }
 };
 
-std::tuple<Tensor, Tensor> scan(const Tensor& gate, const Tensor& x, const Maybe& offsets, const Maybe& h0, int64_t seqs) {
-    no_tangent("gated_scan", gate, x, h0.value_or(Tensor()));
+std::tuple<Tensor, Tensor> scan(const Tensor& gate, const Tensor& x, const Maybe& offsets, const Maybe& first, int64_t seqs) {
+    no_tangent("gated_scan", gate, x, first.value_or(Tensor()));
+    const Maybe h0 = first ? Maybe(first->resolve_neg()) : first;
     if (at::GradMode::is_enabled() && (gate.requires_grad() || x.requires_grad() || (h0 && h0->requires_grad()))) {
         variable_list out = Scan::apply(gate, x, offsets, h0, seqs);
         return {out[0], out[1]};
@@ -231,7 +235,7 @@ bool matrix(const Tensor* t, int64_t dims) {
 }
 bool alike(const Tensor& a, const Tensor& b) { return a.scalar_type() == b.scalar_type() && a.device() == b.device() && a.sizes() == b.sizes(); }
 bool index(const Tensor* t, at::Device device) {
-    return t && (t->scalar_type() == at::kInt || t->scalar_type() == at::kLong) && t->device() == device && t->is_contiguous();
+    return t && (t->scalar_type() == at::kInt || t->scalar_type() == at::kLong) && t->device() == device && t->is_contiguous() && !t->is_neg();
 }
 bool rows_side_by_side(const Tensor& t) { return (t.size(1) == 1 || t.stride(1) == 1) && (t.size(0) <= 1 || t.stride(0) >= t.size(1)); }
 
@@ -276,7 +280,7 @@ py::object usual_step(py::handle gate, py::handle x, py::handle state, py::handl
     const Tensor *g = tensor(gate), *y = tensor(x), *s = tensor(state);
     Maybe which;
     if (!matrix(g, 2) || !matrix(y, 2) || !alike(*g, *y) || y->size(1) == 0 || !s || s->dim() != 2 || s->scalar_type() != at::kFloat ||
-        s->device() != y->device() || s->size(1) != y->size(1) || !rows_side_by_side(*s))
+        s->device() != y->device() || s->size(1) != y->size(1) || !rows_side_by_side(*s) || s->is_neg())
         return py::none();
     if (at::GradMode::is_enabled() && (g->requires_grad() || y->requires_grad() || s->requires_grad())) return py::none();
     if (slots.is_none()) {

@@ -127,6 +127,7 @@ def orthogonalize(updates, steps=5, coefficients=QUINTIC, out=None, products="fu
                 raise ValueError("updates: an empty matrix")
             if max(g.shape) > 32768:  # (the descriptions below hold the sides in 32 bits)
                 raise ValueError("updates: a matrix of %d x %d; sides of up to 32768 are supported" % tuple(g.shape))
+            g = g.resolve_neg()  # (the library reads memory)
             srcs.append(g if (g.shape[1] == 1 or g.stride(1) == 1) and (g.shape[0] == 1 or g.stride(0) >= g.shape[1]) else g.contiguous())
         if out is None:
             outs = [torch.empty(g.shape, dtype=dtype, device=device) for g in mats]
@@ -134,6 +135,8 @@ def orthogonalize(updates, steps=5, coefficients=QUINTIC, out=None, products="fu
             for o, g in zip(outs, mats):
                 if o.shape != g.shape or o.dtype != dtype or o.device != device:
                     raise ValueError("out must have the shapes, type and device of updates")
+                if o.is_neg():
+                    raise ValueError("out is a view of negated elements")
                 if (o.shape[1] > 1 and o.stride(1) != 1) or (o.shape[0] > 1 and o.stride(0) < o.shape[1]):
                     raise ValueError("out: the elements of a row must lie side by side")
             if len(mats) > 32 or products == "half":  # more than one group

@@ -35,7 +35,7 @@ def _index(t, name, device):
         raise ValueError("%s must be an int32 or int64 tensor" % name)
     if t.device != device:
         raise ValueError("%s is on %s, the matrices on %s" % (name, t.device, device))
-    return t.contiguous()
+    return t.resolve_neg().contiguous()
 
 
 _ops = None
@@ -130,6 +130,8 @@ def gated_step(gate, x, state, slots=None):
     P = state.shape[0]
     if D > 1 and state.stride(1) != 1 or P > 1 and state.stride(0) < D:
         raise ValueError("the elements of a row of state must lie side by side")
+    if state.is_neg():
+        raise ValueError("state is a view of negated elements and cannot be updated in place")
     if (gate.requires_grad or x.requires_grad or state.requires_grad) and torch.is_grad_enabled():
         raise ValueError("gated_step is not differentiable: call it under torch.no_grad(), or use gated_scan")
     if slots is not None:

@@ -668,3 +668,37 @@ def test_forward_mode_is_refused_not_dropped():
     out = S.embed(wl, ids)
     with fwd.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):  # a tangent of the upstream gradient
         torch.autograd.grad(out, [wl], fwd.make_dual(torch.ones_like(out), torch.ones_like(out)))
+
+
+def test_views_of_negated_elements():
+    """z.conj().imag holds -imag(z) as imag(z) and a mark"""
+    g = gen(50)
+
+    def negated(*shape):
+        z = torch.complex(torch.randn(*shape, generator=g), torch.randn(*shape, generator=g)).cuda()
+        assert z.conj().imag.is_neg()
+        return z.conj().imag
+
+    ids, off = torch.tensor([1, 0, 4, -1], device="cuda"), torch.tensor([0, 2, 5], device="cuda")
+    for D in (1, 6):
+        w, gate, x, h0, dh, dlast = negated(5, D), negated(5, D), negated(5, D), negated(2, D), negated(5, D), negated(2, D)
+        plainly = [t.clone().resolve_neg() for t in (w, gate, x, h0, dh, dlast)]
+
+        def work(w, gate, x, h0, dh, dlast):
+            w, gate, x, h0 = (t.detach().requires_grad_(True) for t in (w, gate, x, h0))
+            e = S.embed(w, ids)
+            h, last = S.gated_scan(gate, x, off, h0)
+            out = [e, *torch.autograd.grad(e, [w], dh[:4]), h, last, *torch.autograd.grad([h, last], [gate, x, h0], [dh, dlast])]
+            state = torch.ones(5, D, device="cuda")
+            with torch.no_grad():
+                return out + [S.gated_step(gate, x, state), state, dvae_amd.optim.orthogonalize(x)]
+
+        if D == 1:  # (rows whose elements do not lie side by side are refused in a table)
+            assert all(torch.equal(a, b) for a, b in zip(work(w, gate, x, h0, dh, dlast), work(*plainly)))
+        else:
+            assert all(torch.equal(a, b) for a, b in zip(work(plainly[0], gate, x, h0, dh, dlast), work(*plainly)))
+    state = negated(5, 1)
+    with pytest.raises(ValueError, match="negated"):
+        S.gated_step(torch.ones(5, 1, device="cuda"), torch.ones(5, 1, device="cuda"), state)
+    with pytest.raises(ValueError, match="negated"):
+        dvae_amd.optim.orthogonalize(torch.ones(5, 1, device="cuda"), out=state)
