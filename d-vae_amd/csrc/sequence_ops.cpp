@@ -212,10 +212,25 @@ std::tuple<Tensor, Tensor> scan(const Tensor& gate, const Tensor& x, const Maybe
     return {h, last};
 }
 
+// whether two tensors may share memory: by the addresses between their first and last elements
+bool may_overlap(const Tensor& a, const Tensor& b) {
+    auto span = [](const Tensor& t) {
+        int64_t last = 0;
+        for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+        const char* from = (const char*)t.data_ptr();
+        return std::make_pair(from, from + (last + 1) * t.element_size());
+    };
+    if (a.numel() == 0 || b.numel() == 0) return false;
+    const auto [a0, a1] = span(a);
+    const auto [b0, b1] = span(b);
+    return a0 < b1 && b0 < a1;
+}
+
 Tensor step(const Tensor& gate, const Tensor& x, const Tensor& state, const Maybe& slots) {
     no_tangent("gated_step", gate, x, state);
     const int32_t B = size32("gated_step: rows", x.size(0)), D = size32("gated_step: channels", x.size(1));
-    const Rows g(gate), y(x);
+    // rows that lie in the pool itself are read before any state is written
+    const Rows g(may_overlap(gate, state) ? gate.clone() : gate), y(may_overlap(x, state) ? x.clone() : x);
     const int64_t P = state.size(0);
     Tensor h = at::empty(x.sizes(), at::TensorOptions(x.scalar_type()).device(x.device()));
     enqueue("dvae_scan_step", x.device(), p_dvae_scan_step, g.p(), g.ld, y.p(), y.ld, (float*)state.data_ptr(), P > 1 ? state.stride(0) : (int64_t)D, P,

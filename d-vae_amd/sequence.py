@@ -112,7 +112,7 @@ def gated_step(gate, x, state, slots=None):
     """One token of each of B sequences: gate, x [B, D]; returns h [B, D] in x's type and updates `state` [P, D] (float32)
     in place at the rows `slots` [B] (int32 / int64, B at most 65536; default: row b has state b).  A slot outside [0, P)
     marks a padding row: its h is zero and no state changes.  Rows that name the same slot advance it one after the other,
-    in their order.
+    in their order.  gate and x may lie in the pool itself: they are read before it is written.
     For serving: not differentiable, inputs that need gradients are refused outside torch.no_grad()."""
     out = (_ops or _native()).usual_step(gate, x, state, slots)
     if out is not None:

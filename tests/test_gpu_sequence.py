@@ -702,3 +702,22 @@ def test_views_of_negated_elements():
         S.gated_step(torch.ones(5, 1, device="cuda"), torch.ones(5, 1, device="cuda"), state)
     with pytest.raises(ValueError, match="negated"):
         dvae_amd.optim.orthogonalize(torch.ones(5, 1, device="cuda"), out=state)
+
+
+def test_gated_step_on_rows_of_the_pool_itself():
+    g = gen(51)
+    P, D = 20000, 96  # more rows than run at a time
+    pool, gate = torch.randn(P, D, generator=g).cuda(), torch.randn(P, D, generator=g).cuda()
+    slots = torch.arange(P).flip(0).cuda()
+    want = pool.clone()
+    h = S.gated_step(gate, pool, want, slots)
+    got = pool.clone()
+    assert torch.equal(S.gated_step(gate, got, got, slots), h) and torch.equal(got, want)
+    want = pool.clone()
+    h = S.gated_step(pool[:5000], gate[:5000], want, slots[:5000])
+    got = pool.clone()
+    assert torch.equal(S.gated_step(got[:5000], gate[:5000], got, slots[:5000]), h) and torch.equal(got, want)
+    both = torch.cat([pool, gate], 1)  # states and gates side by side, in one range of addresses
+    h = S.gated_step(gate, pool.clone(), pool, slots)
+    assert torch.equal(S.gated_step(both[:, D:], both[:, :D], both[:, :D], slots), h) and torch.equal(both[:, :D], pool)
+    assert torch.equal(both[:, D:], gate)
