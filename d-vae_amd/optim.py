@@ -90,7 +90,7 @@ def orthogonalize(updates, steps=5, coefficients=QUINTIC, out=None, products="fu
     every product in one launch.  coefficients: (a, b, c), or one such triple for each step; a set that lets a singular value
     leave [-2, 2] is refused.  out: where to write (same shapes and type; matrices may be their own outputs, or each other's),
     default new tensors.  A zero matrix gives zeros, one with a NaN or an infinity NaN.  Not differentiable (it acts on updates):
-    inputs that need gradients are refused outside torch.no_grad().
+    inputs and outputs that need gradients are refused outside torch.no_grad().
 
     Accuracy of float32, rounded once to the matrices' type.  products="half" (bfloat16 only): matrices with both sides of at
     least 512 multiply operands of 11 bits, for a third of the work; their error is then of the order of the result's own
@@ -104,7 +104,7 @@ def orthogonalize(updates, steps=5, coefficients=QUINTIC, out=None, products="fu
     steps, abc = _iteration(steps, coefficients)
     if not mats:
         return []
-    if torch.is_grad_enabled() and any(torch.is_tensor(g) and g.requires_grad for g in mats):
+    if torch.is_grad_enabled() and any(torch.is_tensor(g) and g.requires_grad for g in mats + (outs if out is not None else [])):
         raise ValueError("orthogonalize is not differentiable: call it under torch.no_grad()")
     if forward_ad._current_level >= 0 and any(torch.is_tensor(g) and forward_ad.unpack_dual(g).tangent is not None
                                               for g in mats + (outs if out is not None else [])):

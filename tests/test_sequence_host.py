@@ -251,3 +251,15 @@ def test_what_no_launch_can_hold_is_refused_before_the_first_one():
         assert "too many" in rc(name, *args, 30, 1 << 26, 64, 0, None)  # one tile
         assert "too many" in rc(name, *args, 0, 1 << 26, 64, 0, None)
     assert "too many" in rc("dvae_scan_step", p, 1 << 13, p, 1 << 13, p, 1 << 13, 1 << 24, None, 0, p, 1 << 24, 1 << 13, 0, None)
+
+
+def test_orthogonalize_refuses_an_output_that_needs_a_gradient():
+    """it would keep the gradient of what it held before"""
+    m, leaf = torch.ones(3, 4), torch.ones(3, 4, requires_grad=True)
+    for out in (leaf, leaf * 2):
+        with pytest.raises(ValueError, match="no_grad"):
+            dvae_amd.optim.orthogonalize(m, out=out)
+        with pytest.raises(ValueError, match="no_grad"):
+            dvae_amd.optim.orthogonalize([m, m], out=[m.clone(), out])
+        with torch.no_grad(), pytest.raises(L.DvaeHipError, match="no CPU fallback"):
+            dvae_amd.optim.orthogonalize(m, out=out)
