@@ -65,3 +65,63 @@ def test_gradients_of_masked_rows_are_finite(dtype):
     assert not dg[closed.cuda()].any()  # z (1 - z) is 0 in 32 bits, whatever the state before
     # a masked row: G = dh exactly, (prev - x) z (1 - z) off by its roundings alone, a few u relative (and u |h| of prev)
     close(dg[rows.cuda()], ref[2][rows], ref[2][rows].abs() * 32 * U + 2 * tol_h, "dgate of masked rows")
+
+
+# ------------------------------------------------------------------------------------ states that stay over many tiles of rows
+
+LONG = [([3077], 0, 0), ([1500, 0, 3, 1574], 7, 5), ([2600, 477], 0, 0)]
+
+
+def long_memory(k, dim, dtype):
+    """every channel keeps its own retention between 0.3 and 0.9995; what comes first (h0, early x) and last (dlast) is large.
+    More than 20 tiles of rows in either direction."""
+    lengths, front, behind = LONG[k]
+    dt, g = DT[dtype], gen(10 * k + dim)
+    off = [front]
+    for n in lengths:
+        off.append(off[-1] + n)
+    N, Sn = off[-1] + behind, len(lengths)
+    z = torch.linspace(0.9995, 0.3, dim).double()
+    gate = (torch.log(z / (1 - z)) + 0.1 * torch.randn(N, dim, generator=g)).to(dt)
+    x = torch.randn(N, dim, generator=g).clamp(-3, 3)
+    x[front:front + 100] = 3 * torch.sign(x[:1])
+    h0 = 3 * torch.sign(torch.randn(Sn, dim, generator=g))
+    dh, dlast = torch.randn(N, dim, generator=g).to(dt), 30 * torch.sign(torch.randn(Sn, dim, generator=g))
+    return off, gate, x.to(dt), h0, dh, dlast
+
+
+def long_bounds(off, gate, big):
+    """what h and last, and G may be off by (the head of the file), channel by channel"""
+    mem = (1 / (1 - torch.sigmoid(gate.double()).max(0).values)).clamp(max=max(b - a for a, b in zip(off, off[1:])))
+    return (8 * mem + 32) * U * 3.0, (8 * mem + 32) * U * big
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("dim", [1, 66, 129])
+@pytest.mark.parametrize("k", range(len(LONG)))
+def test_states_and_gradients_that_stay_over_many_tiles(k, dim, dtype):
+    off, gate, x, h0, dh, dlast = long_memory(k, dim, dtype)
+    ref = plain_scan(gate.double(), x.double(), off, h0.double(), dh.double(), dlast.double())
+    leaves = [gate.cuda().requires_grad_(True), x.cuda().requires_grad_(True), h0.cuda().requires_grad_(True)]
+    h, last = S.gated_scan(leaves[0], leaves[1], torch.tensor(off).cuda(), leaves[2])
+    dg, dx, dh0 = torch.autograd.grad([h, last], leaves, [dh.cuda(), dlast.cuda()])
+    tol_h, tol_G = long_bounds(off, gate, ref[5])
+    close(h, ref[0], tol_h, "h")
+    close(last, ref[1], tol_h, "last")
+    close(dx, ref[3], tol_G + 4 * U * ref[5], "dx")
+    close(dg, ref[2], (tol_G * 6 + ref[5] * tol_h + 32 * U * ref[5] * 6) / 4, "dgate")
+    close(dh0, ref[4], tol_G, "dh0")
+    alone = S.gated_scan(gate.cuda(), x.cuda(), torch.tensor(off).cuda(), h0.cuda())  # without what the backward pass keeps
+    assert torch.equal(alone[0], h) and torch.equal(alone[1], last)
+
+
+def test_the_gradient_of_h0_comes_back_over_the_whole_sequence():
+    g = gen(60)
+    T, D = 700, 40
+    gate = torch.full((2, T, D), 6.0) + 0.5 * torch.randn(2, T, D, generator=g)
+    h0 = torch.zeros(2, D, device="cuda", requires_grad=True)
+    h, last = S.gated_scan(gate.cuda(), torch.zeros(2, T, D, device="cuda"), h0=h0)
+    dh0, = torch.autograd.grad(last.sum(), [h0])
+    want = torch.sigmoid(gate.double()).prod(1)
+    assert want.min() > 0.05
+    close(dh0, want, (8 * T + 32) * U, "dh0")
