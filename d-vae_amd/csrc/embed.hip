@@ -12,7 +12,8 @@
 //   2. the sorted list is cut into chunks of EC tokens, one wave per chunk and column slab, whatever the tokens' counts (a
 //      hot token is spread over as many waves as it fills chunks).  A run of equal tokens inside one chunk is summed in
 //      registers and written once; a run that crosses a chunk's border leaves an fp32 partial per chunk;
-//   3. the partials of each crossing run are added in chunk order.
+//   3. the partials of each crossing run are added by the waves of one workgroup, each every so many of them in chunk order, and
+//      the waves' sums in wave order: the same order every time.
 // Rows that no token names are zeroed by further workgroups of launch 2, which find the tokens of their row range in the
 // sorted list, so every row of dW is written exactly once.
 //
@@ -66,8 +67,8 @@ __global__ __launch_bounds__(256) void embed_fwd_kernel(const T* __restrict__ w,
 }
 
 // --------------------------------------------------------------------------------------------------- sorting by token
-// Radix sort, 8 bits a pass, least significant first; every pass is stable: the rows of a token are added in the order of
-// their positions.  Bound by latency: up to SMALL_N tokens one workgroup does all passes, beyond that a pass is two launches.  Each wave takes 512 consecutive items in
+// Radix sort, 8 bits a pass, least significant first; every pass is stable: equal tokens stay in the order of
+// their positions, so that sums do not vary.  Bound by latency: up to SMALL_N tokens one workgroup does all passes, beyond that a pass is two launches.  Each wave takes 512 consecutive items in
 // eight rounds of 64: the lanes with equal digits find each other by eight ballots, a lane's rank is the wave's count of
 // its digit so far plus the number of such lanes below it.
 __device__ __forceinline__ int wave_rank(unsigned digit, bool live, volatile int* cnt) {

@@ -32,16 +32,18 @@
 // in (17 to 21 bytes a cycle measured with all of them loading, whatever the depth; loads alone are 28 of the 29 us of the
 // ENAS model's products X X^T and 35 of its update's 41), and with large tiles the power: the clock is 2.0 GHz where loads and
 // MFMAs run together, 2.5 with either alone.  So a product takes the largest tile that still keeps the CUs busy:
-//   256 x 256, one workgroup per CU, where the last round of them is nearly full: update at 4096 x 4096 bf16 142 us (0.97 PFLOP/s)
+//   256 x 256, one workgroup per CU, where the last round of them is nearly full: update at 4096 x 4096 350 to 370 us (1.1 to 1.2
+//     PFLOP/s of MFMAs), half products 140 to 155 us (0.89 to 0.98 PFLOP/s; the epilogue is 40 us of either)
 //   192 x 192 for symmetric products where their rounds cover less area than those of 128 x 128: 253 tiles are one round at
-//     4096 x 4096 (78 us), 528 of 128 x 128 two and a bit (120 us)
-//   128 x 128 from 3/4 of a tile per CU on (3000 x 3000 bf16: 1130 -> 990 us a call against 64 x 64; from 1/2 on the ENAS set
-//     would lose: 537 -> 677)
+//     4096 x 4096 (185 to 215 us; half products 76 to 92), 528 of 128 x 128 two and a bit (half products 120 us)
+//   128 x 128 from 3/4 of a tile per CU on (3000 x 3000: fp32 2600 -> 2220 us a call against 64 x 64, half products 1130 -> 990;
+//     from 1/2 on the ENAS set would lose: 537 -> 677)
 //   64 x 64; at most one per CU: four groups of waves share the sum (1024 x 1024: 242 us a call)
 //   32 x 32, at most one per CU: the direct kernel (501 x 501: 155 -> 128 us a call; 768 x 768 would lose: 211 -> 232)
 //
 // Launches.  The matrices of a call go through each product together, one grid over all their tiles: an optimiser step on a
-// model's many small matrices is 17 launches, whatever their number (up to 32 per group).
+// model's many small matrices is 17 launches, whatever their number (up to 32 per group).  The coefficients are checked before
+// the first of them in a few operations a step (0.5 us a call).
 #include "common.h"
 #include "dvae_hip.h"
 #include "seq_common.h"

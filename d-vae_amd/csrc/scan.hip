@@ -17,7 +17,7 @@
 // states, products and sums are fp32; outputs are rounded once.
 //
 // One pass over the data in either direction (forward 3, backward 5 matrices of memory traffic), tiles chained through
-// look_back.  Measured on 131072 x 1024 bf16: forward 225 us (3.6 TB/s), backward 367 us (3.7 TB/s), where a large copy
+// look_back.  Measured on 131072 x 1024 bf16: forward 230 us (3.5 TB/s), backward 369 us (3.6 TB/s), where a large copy
 // reaches 4.9.  With the look-back left out they take 187 and 272: what a tile waits for is two trips to device memory, its
 // neighbours' maps and back, about 5 us of the 28 (17) that it lives, whatever the length of the chain: a second level of
 // look-back over groups of 8 tiles, and other waves to publish than those that wait, made 223 and 354 of it, and 1 us more of a prompt.
@@ -117,7 +117,7 @@ __device__ __forceinline__ float both(float A, float before) { return begins(A) 
 constexpr int LOOK = 8;
 constexpr unsigned long long UNSET = ~0ull;
 constexpr long FILL_BLOCKS = 2048;  // at most, before a pass
-constexpr int SPINS = 1 << 22;  // never reached: every tile waits for earlier tickets only; then NaN rather than a hang
+constexpr int SPINS = 1 << 22;  // never reached: every tile waits for earlier tickets only; else the states from there on are NaN, not a hang
 __device__ __forceinline__ void publish(unsigned long long* at, float A, float B) {
     const unsigned long long w = ((unsigned long long)__float_as_uint(A) << 32) | __float_as_uint(B);
     __hip_atomic_store(at, w == UNSET ? w ^ 1 : w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -499,7 +499,7 @@ __global__ __launch_bounds__(TRB / RW * 64) void scan_bwd_kernel(ScanParams p) {
 
 // Before a pass over several tiles: nothing is published yet, ticket 0 is next; and the sequences without rows, by the
 // workgroups behind `fill_blocks`.  A single tile per slab has nothing to wait for: no tickets, no look-back, and the
-// sequences without rows are taken by workgroups behind the tiles' (100 rows of 501 floats: 9.2 -> 6.6 us).
+// sequences without rows are taken by workgroups behind the tiles' (100 rows of 501 floats: 9.2 -> 6.9 us).
 __global__ __launch_bounds__(256) void scan_begin_kernel(ulonglong2* __restrict__ words, long pairs, unsigned* __restrict__ ticket,
                                                          int fill_blocks, Rows q, const float* __restrict__ from,
                                                          float* __restrict__ to, int D) {
@@ -597,7 +597,7 @@ static int scan_check(const char* who, int64_t rows, int64_t seqs, const void* o
     DVAE_REQUIRE(rows >= 0 && rows < (1LL << 40), "%s: %lld rows are not supported", who, (long long)rows);
     DVAE_REQUIRE(seqs >= 0 && seqs < (1LL << 31), "%s: %lld sequences are not supported", who, (long long)seqs);
     DVAE_REQUIRE(D >= 1 && D <= (1 << 20), "%s: %d channels are not in 1 .. 2^20", who, D);
-    // (a wave addresses its 32 rows with 32-bit byte offsets)
+    // (a wave addresses its 16 rows with 32-bit byte offsets)
     DVAE_REQUIRE(ld_most <= (1 << 23), "%s: a row stride of %lld elements is not supported", who, (long long)ld_most);
     DVAE_REQUIRE(off || (seqs > 0 ? rows % seqs == 0 : rows == 0), "%s: %lld rows are not %lld sequences of one length", who,
                  (long long)rows, (long long)seqs);

@@ -54,8 +54,8 @@ def _native():
 def embed(weight, ids, scale=1.0):
     """scale * weight[ids]: `weight` [V, D] with its elements side by side in a row, `ids` int32 / int64 of any shape;
     returns [*ids.shape, D].  A token outside [0, V) (padding) gives a row of zeros and takes no part in the gradient.
-    The gradient of `weight` is dense, summed in float32 in the order of the tokens' positions and rounded once; it does
-    not vary from run to run."""
+    The gradient of `weight` is dense (up to 2^28 - 32 tokens), summed in float32 in an order that depends on the tokens alone
+    and rounded once; it does not vary from run to run."""
     out = (_ops or _native()).usual_embed(weight, ids, scale)
     if out is not None:
         return out

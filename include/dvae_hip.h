@@ -474,7 +474,8 @@ int dvae_embed_bwd(const void* dout, int64_t ld_dout, const void* ids, int32_t i
  * row for all; at most 2^23); h [rows][D] contiguous, rounded once; last [seqs][D] fp32: the state after each sequence (h0
  * where it is empty).  rows times D / 64, rounded up, stays below 2^30 - 128, and there are less than 2^26 - 8192 sequences
  * (without off and with rows: any number).  Rows of no sequence give zeros.  states: dvae_scan_state_floats() floats that the backward pass reads (NULL if
- * there is none); ws: dvae_scan_ws_bytes() bytes, 16-byte aligned, for this call alone. */
+ * there is none); ws: dvae_scan_ws_bytes() bytes, 16-byte aligned, for this call alone.  Workgroups wait for earlier ones
+ * that have begun; the waits are bounded, and one that ran out (no cause is known) would leave NaN, as in the chains above. */
 int64_t dvae_scan_state_floats(int64_t rows, int32_t D);
 int64_t dvae_scan_ws_bytes(int64_t rows, int32_t D);
 int dvae_scan_fwd(const void* gate, int64_t ld_gate, const void* x, int64_t ld_x, const void* off, int32_t off_i64,
