@@ -94,7 +94,7 @@ def orthogonalize(updates, steps=5, coefficients=QUINTIC, out=None, products="fu
 
     Accuracy of float32, rounded once to the matrices' type.  products="half" (bfloat16 only): matrices with both sides of at
     least 512 multiply operands of 11 bits, for a third of the work; their error is then of the order of the result's own
-    rounding and adds to it.  What other matrices a call has changes a result by the order of its sums alone (float32)."""
+    rounding and adds to it.  What other matrices a call has changes a result in the last bits of float32 alone."""
     one = torch.is_tensor(updates)
     mats = [updates] if one else list(updates)
     if out is not None:
@@ -346,6 +346,11 @@ class FlatAdam(torch.optim.Optimizer):
             self.extra.load_state_dict(sd["extra"])
 
 
+def _of_matrices(key):
+    """a value of FlatMuon's group of matrices as an attribute"""
+    return property(lambda self: self.param_groups[0][key], lambda self, value: self.param_groups[0].update({key: value}))
+
+
 class FlatMuon(FlatAdam):
     """Muon for the weight matrices, Adam for everything else, on FlatAdam's flat buffers: the momentum of a matrix is
     orthogonalised (`orthogonalize`, all matrices of the model together) before it is applied.  The arguments are those of
@@ -398,8 +403,7 @@ class FlatMuon(FlatAdam):
         if fn not in ("original", "match_rms_adamw"):
             raise ValueError("adjust_lr_fn must be 'original' or 'match_rms_adamw'")
 
-    ns_steps = property(lambda self: self.param_groups[0]["ns_steps"])
-    ns_coefficients = property(lambda self: self.param_groups[0]["ns_coefficients"])
+    ns_steps, ns_coefficients = _of_matrices("ns_steps"), _of_matrices("ns_coefficients")
 
     def _set_factor(self):
         """the learning-rate factors of the matrices, for every 64 elements of the flat buffers; 0 elsewhere"""

@@ -359,3 +359,22 @@ def test_flat_muon_refuses_an_iteration_before_anything_moves():
     opt.param_groups[0]["ns_coefficients"] = O.QUINTIC
     opt.step()
     assert opt.steps == 1 and not torch.equal(kept[0], opt.flat_p)
+
+
+def test_flat_muon_iteration_can_be_set_as_an_attribute():
+    model, ga = model_and_batch()
+    opt = O.FlatMuon(model)
+    opt.ns_steps, opt.ns_coefficients = 2, (1.5, -0.5, 0.0)
+    opt.zero_grad()
+    grads_of(model, ga, torch.randn(24, 16, generator=gen(13)))
+    before = [p.detach().double().cpu() for p in opt.reducer.params]
+    grads = [p.grad.double().cpu().clone() for p in opt.reducer.params]
+    opt.step()
+    for name, p, b, d in zip(opt.reducer.names, opt.reducer.params, before, grads):
+        if name in opt.matrices:
+            rows, cols = d.shape
+            f = 0.02 * max(1.0, rows / cols) ** 0.5
+            o = plain(d + 0.95 * (0.05 * d - d), 2, (1.5, -0.5, 0.0))  # u = g + mu (m - g), m = (1 - mu) g
+            # (sup |p'| is 1.5 here: 1 + 1.5 steps' errors; the momentum's and the update's roundings as above)
+            slack = f * float(o.norm()) * 2.5 * (16 * 2.0 ** -22 + 8 * 2.0 ** -24) + 3 * 2.0 ** -24 * float(b.norm())
+            assert float((p.detach().double().cpu() - (b - f * o)).norm()) <= slack, name
