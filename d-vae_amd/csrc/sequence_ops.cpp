@@ -212,7 +212,8 @@ std::tuple<Tensor, Tensor> scan(const Tensor& gate, const Tensor& x, const Maybe
     return {h, last};
 }
 
-// whether two tensors may share memory: by the addresses between their first and last elements
+// whether two matrices may share memory: by the addresses between their first and last elements, and columns beside each other
+// in rows of one stride are told apart
 bool may_overlap(const Tensor& a, const Tensor& b) {
     auto span = [](const Tensor& t) {
         int64_t last = 0;
@@ -223,7 +224,13 @@ bool may_overlap(const Tensor& a, const Tensor& b) {
     if (a.numel() == 0 || b.numel() == 0) return false;
     const auto [a0, a1] = span(a);
     const auto [b0, b1] = span(b);
-    return a0 < b1 && b0 < a1;
+    if (a0 >= b1 || b0 >= a1) return false;
+    const int64_t ld = a.stride(0) * a.element_size();
+    if (ld <= 0 || a.element_size() != b.element_size() || a.stride(0) != b.stride(0) || (a.size(1) > 1 && a.stride(1) != 1) ||
+        (b.size(1) > 1 && b.stride(1) != 1))
+        return true;
+    const int64_t apart = ((b0 - a0) % ld + ld) % ld;  // where a row of b begins in a's rows
+    return apart < a.size(1) * a.element_size() || apart + b.size(1) * b.element_size() > ld;
 }
 
 Tensor step(const Tensor& gate, const Tensor& x, const Tensor& state, const Maybe& slots) {

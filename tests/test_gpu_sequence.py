@@ -721,3 +721,16 @@ def test_gated_step_on_rows_of_the_pool_itself():
     h = S.gated_step(gate, pool.clone(), pool, slots)
     assert torch.equal(S.gated_step(both[:, D:], both[:, :D], both[:, :D], slots), h) and torch.equal(both[:, :D], pool)
     assert torch.equal(both[:, D:], gate)
+    parts = torch.cat([want, gate, gate], 1)  # states, gates and candidates beside each other, at an odd place, read where they lie
+    wide = torch.zeros(P, 3 * D + 1, device="cuda")
+    wide[:, 1:] = parts
+    for flip in (False, True):
+        st, ga, xx = want.clone(), gate.clone(), gate.clone()
+        h = S.gated_step(ga, xx, st, slots)
+        cols = [wide[:, 1:D + 1], wide[:, D + 1:2 * D + 1], wide[:, 2 * D + 1:]]
+        wide[:, 1:] = parts
+        if flip:
+            cols = cols[::-1]
+            cols[0].copy_(want), cols[1].copy_(gate), cols[2].copy_(gate)
+        assert torch.equal(S.gated_step(cols[1], cols[2], cols[0], slots), h) and torch.equal(cols[0], st)
+        assert torch.equal(cols[1], gate) and torch.equal(cols[2], gate)
