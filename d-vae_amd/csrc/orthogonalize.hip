@@ -8,8 +8,17 @@
 // S = 2^13: 22 bits, with an absolute floor of 2^-38.  A product is three MFMAs, hi hi + hi lo + lo hi, accumulated in
 // fp32; the dropped lo lo is 2^-22 relative, as the planes' own rounding.  That is fp32 accuracy at 1/3 of the fp16 rate:
 // against 64 bits the result is 7e-7 off at 501 x 501 and 3e-6 at 4096 x 4096, where the same iteration in fp32 is 2.2e-6 and 5e-6.
-// With few rows the roundings average out less (8 to 16 rows: up to 1.5e-6, 1.8 times fp32's own error), so up to 64 rows, and
-// wherever the direct kernel runs, lo lo is added (up to 1.2e-6, 1.5 times); latency bounds those products and hides it.
+// With few rows the roundings average out less.  So
+//   - up to 64 rows, and wherever the direct kernel runs, lo lo is added (latency bounds those products and hides it);
+//   - up to 64 rows B is kept as B + f, f = -(b + c), with X <- (a - f) X + (B + f) X: where the singular values have come near 1, B
+//     is near -f, and its rounding and the cancellation with a X are what is left (with many rows, small singular values leave
+//     entries near 0 in B, which a shift would round worse);
+//   - the sums of X X^T, over whole rows of X, are held in parts on 64 x 64 tiles and in the direct kernel: the products with a
+//     second plane apart, hi hi in two or eight (one by one in fp32 9 x 1883 beside larger matrices was 2.7e-6 off and 9 x 20000
+//     8.5e-6, where the fp32 iteration is 1.1e-6 and 3.5e-6; now 1.1e-6 and 0.9e-6; no time, the MFMAs are as many), and matrices
+//     of up to 384 rows take 64 x 64 tiles there also in sets whose others take larger ones (five launches more: 60 us of 1400
+//     with two 2048 x 2048 and three of few rows).
+// Against the fp32 iteration's own error over random shapes and sets: median 0.9 of it up to 20 rows, 0.7 up to 65, 0.6 up to 400.
 // G is scaled by a power of two, exactly; the rest of the division by its norm (a factor r in (1, 2]) goes into the
 // coefficients of the first step: a r, b r^3, c r^5.
 //
@@ -57,6 +66,7 @@ typedef float nsf32x16 __attribute__((ext_vector_type(16)));
 typedef float nsf32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int NS_GROUP = 32;          // matrices per launch
+constexpr int NS_FEW = 384;           // rows up to which the long sums of X X^T are held apart; see the head of the file
 constexpr int NS_PARTS = 256;         // partial sums of a norm
 constexpr float NS_S = 8192.f;        // 2^13
 
@@ -76,7 +86,7 @@ struct NsGroup {
     char* ws;
     double* parts;  // [count][NS_PARTS]
     float* r;       // [count]
-    float a, b, c;
+    float a, b, c, shift;  // of the step; what B of matrices with few rows is shifted by
 };
 
 __host__ __device__ inline int ns_pad(int v, int tb) { return (v + tb - 1) / tb * tb; }
@@ -269,6 +279,7 @@ __device__ __forceinline__ void ns_out8(const NsMat& m, int dtype, int row, int 
 template <int TB, int WN, int KG, int PL, int NB, int MODE>
 __global__ __launch_bounds__(128 * WN * KG) void ns_product_kernel(NsGroup p, int from, int first) {
     constexpr int TM = TB / 64, TN = TB / WN / 32, NT = 128 * WN;
+    constexpr bool SUMS = TB == 64 && PL == 2 && MODE == NS_GRAM;  // three sums of an output instead of one
     constexpr int LR = NT / 8, PASSES = TB / LR;  // 16 bytes per thread and pass: LR rows of one block
     constexpr int OPERAND = TB * 128, LOADS = 2 * PASSES;
     constexpr int TP = TB + 4;                    // row pitch of the output in LDS, floats; 64 rows at a time
@@ -294,7 +305,7 @@ __global__ __launch_bounds__(128 * WN * KG) void ns_product_kernel(NsGroup p, in
     const char* b_rows = base + ns_offset(mp, np, PL, MODE == NS_GRAM ? from : MODE == NS_POLY ? 4 : from + 1) + (long)tj * TB * pitch;
     const int blocks = (int)(pitch / 128), stages = (blocks + KG - 1) / KG;
 
-    const bool all_four = m.m() <= 64;  // lo lo too
+    const bool few = PL == 2 && m.m() <= 64;  // lo lo too, and B shifted
     const int col0 = tj * TB;
     const bool mirror = MODE == NS_STEP || ((MODE == NS_GRAM || MODE == NS_POLY) && ti != tj);  // a diagonal tile is its own mirror
     const char* src = base + ns_offset(mp, np, PL, MODE == NS_POLY ? 4 : from);
@@ -329,6 +340,9 @@ __global__ __launch_bounds__(128 * WN * KG) void ns_product_kernel(NsGroup p, in
         for (int j = 0; j < TN; ++j)
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+    nsf32x16 odd, cross;  // SUMS: of every other 16 columns, and of the products with a second plane
+#pragma unroll
+    for (int r = 0; r < 16; ++r) odd[r] = cross[r] = 0.f;
     const int wm = wave / WN, wn = wave % WN;
     // A wave's load writes 1 KB of LDS in the order of its lanes: 8 rows of 128 bytes.  Chunk c of row r goes to place
     // c ^ (r / 2 mod 8), so that the 16 rows that a read of a fragment takes at a time lie on different banks.
@@ -407,15 +421,17 @@ __global__ __launch_bounds__(128 * WN * KG) void ns_product_kernel(NsGroup p, in
             if (PIPED) __builtin_amdgcn_sched_barrier(0);
             auto mma = [&](int qa, int qb, int i) {
 #pragma unroll
-                for (int j = 0; j < TN; ++j)
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[h & 1][qa][i], fb[h & 1][qb][j], acc[i][j], 0, 0, 0);
+                for (int j = 0; j < TN; ++j) {
+                    nsf32x16& sum = SUMS && qa + qb > 0 ? cross : SUMS && (h & 1) ? odd : acc[i][j];
+                    sum = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[h & 1][qa][i], fb[h & 1][qb][j], sum, 0, 0, 0);
+                }
             };
 #pragma unroll
             for (int q = 0; q < PRODUCTS; ++q)
 #pragma unroll
                 for (int i = 0; i < TM; ++i) {
                     if (mine) {
-                        if (PL == 2 && q == 0 && all_four) mma(PL - 1, PL - 1, i);
+                        if (PL == 2 && q == 0 && few) mma(PL - 1, PL - 1, i);
                         mma(PL == 2 && q == 0, PL == 2 && q == 1, i);
                     }
                     if (PIPED) {
@@ -429,6 +445,7 @@ __global__ __launch_bounds__(128 * WN * KG) void ns_product_kernel(NsGroup p, in
         }
         b = after;
     }
+    if (SUMS) acc[0][0] += odd + cross;
     if (MODE != NS_GRAM && !FROM_START && !FROM_LAST)
 #pragma unroll
         for (int n = 0; n < UNITS; ++n) fetch(0, n);
@@ -439,7 +456,8 @@ __global__ __launch_bounds__(128 * WN * KG) void ns_product_kernel(NsGroup p, in
     // c ^ 8 (q / 8 mod 8): rows are read 8 columns at a time and columns 8 rows at a time, both from all banks.
     // Lane l of an MFMA block holds column l & 31 and rows (r & 3) + 8 (r >> 2) + 4 (l >> 5).
     const float r = first ? p.r[k] : 1.f;
-    const float from_src = MODE == NS_GRAM ? 0.f : (MODE == NS_POLY ? p.b * r * r * r : p.a * r) / NS_S;
+    const float shift = few ? p.shift : 0.f;
+    const float from_src = MODE == NS_GRAM ? 0.f : (MODE == NS_POLY ? p.b * r * r * r : (p.a - shift) * r) / NS_S;
     const float from_acc = (MODE == NS_POLY ? p.c * r * r * r * r * r : 1.f) / (NS_S * NS_S);
     const bool wide = m.rows <= m.cols;  // else the rows of out are the columns of X
     auto place = [](int row, int c) { return row * TP + (c ^ (row & 56)); };
@@ -470,6 +488,10 @@ __global__ __launch_bounds__(128 * WN * KG) void ns_product_kernel(NsGroup p, in
             if (MODE != NS_GRAM) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[e] = fmaf((float)src_hi[n][e] + (float)src_lo[n][e], from_src, v[e]);
+                if (MODE == NS_POLY && few)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (row_of(i, row) == col0 + c8 + e) v[e] += shift * r;
                 if (i + 1 < TM) fetch(i + 1, n);
             }
             if ((MODE != NS_GRAM || KG > 1) && (MODE == NS_LAST ? !wide : mirror))
@@ -563,8 +585,8 @@ __global__ __launch_bounds__(512) void ns_small_kernel(NsGroup p, int from, int 
 #pragma unroll
     for (int e = 0; e < 16; ++e) part[wave][((e & 3) + 8 * (e >> 2) + 4 * (lane >> 5)) * TP + (lane & 31)] = acc[e] + cross[e];
     __syncthreads();
-    const float r = first ? p.r[k] : 1.f;
-    const float from_src = MODE == NS_GRAM ? 0.f : (MODE == NS_POLY ? p.b * r * r * r : p.a * r) / NS_S;
+    const float r = first ? p.r[k] : 1.f, shift = PL == 2 && m.m() <= 64 ? p.shift : 0.f;
+    const float from_src = MODE == NS_GRAM ? 0.f : (MODE == NS_POLY ? p.b * r * r * r : (p.a - shift) * r) / NS_S;
     const float from_acc = (MODE == NS_POLY ? p.c * r * r * r * r * r : 1.f) / (NS_S * NS_S);
     const bool mirror = MODE == NS_STEP || ((MODE == NS_GRAM || MODE == NS_POLY) && ti != tj);
     if (threadIdx.x < 128) {
@@ -575,6 +597,7 @@ __global__ __launch_bounds__(512) void ns_small_kernel(NsGroup p, int from, int 
 #pragma unroll
             for (int w = 0; w < W; ++w) t += part[w][row * TP + c8 + e];
             v[e] = fmaf((float)src_hi[e] + (float)src_lo[e], from_src, t * from_acc);
+            if (MODE == NS_POLY && ti * 32 + row == tj * 32 + c8 + e) v[e] += shift * r;
             part[0][row * TP + c8 + e] = v[e];
         }
         if (MODE != NS_LAST) {
@@ -690,11 +713,12 @@ extern "C" int dvae_orthogonalize(const dvae_matrix_desc* mats, int32_t count, i
     // p(s) = a s + b s^3 + c s^5 is [0, max |p|] again in absolute values; with l = s^2 the maximum is at the end or where
     // a + 3 b l + 5 c l^2 = 0, that of B's |b l + c l^2| at the end or at l = -b / 2 c.
     double most = 1;
+    float shift[32];
     for (int t = 0; t < steps; ++t) {
         const double a = coefficients[3 * t], b = coefficients[3 * t + 1], c = coefficients[3 * t + 2], end = most * most;
         auto p_at = [&](double l) { return fabs((a + b * l + c * l * l) * sqrt(l)); };
-        auto b_at = [&](double l) { return fabs(b * l + c * l * l); };
-        double big = b_at(end);
+        auto b_at = [&](double l) { return b * l + c * l * l; };
+        double low = fmin(0, b_at(end)), high = fmax(0, b_at(end));
         most = p_at(end);
         const double d = 9 * b * b - 20 * a * c;
         // (both roots of the quadratic without cancellation; infinite ones, as with c = 0, lie outside)
@@ -702,11 +726,14 @@ extern "C" int dvae_orthogonalize(const dvae_matrix_desc* mats, int32_t count, i
         for (int i = 0; i < 3; ++i) {
             if (!(roots[i] > 0 && roots[i] < end)) continue;
             if (i < 2) most = fmax(most, p_at(roots[i]));
-            else big = fmax(big, b_at(roots[i]));
+            else low = fmin(low, b_at(roots[i])), high = fmax(high, b_at(roots[i]));
         }
+        const double big = fmax(-low, high);
         DVAE_REQUIRE(most < 1.95, "orthogonalize: with the coefficients of step %d singular values leave [-2, 2]", t);
         // (the first step's B carries r <= 2)
         DVAE_REQUIRE(big * (t == 0 ? 2 : 1) < 7.5, "orthogonalize: the coefficients b and c of step %d are too large", t);
+        shift[t] = (float)-(b + c);
+        if (!(fmax(-(low + shift[t]), high + shift[t]) * (t == 0 ? 2 : 1) < 7.5)) shift[t] = 0;
     }
     if (count == 0) return DVAE_OK;
     DVAE_REQUIRE(ws && (uintptr_t)ws % 16 == 0, "orthogonalize: the workspace must be 16-byte aligned");
@@ -761,10 +788,11 @@ extern "C" int dvae_orthogonalize(const dvae_matrix_desc* mats, int32_t count, i
         else hipLaunchKernelGGL((ns_split_kernel<1>), dim3(split), dim3(256), 0, s, p);
         DVAE_LAUNCH_CHECK();
 #define NS_LAUNCH(TB, WN, KG, PL, NB, MODE, grid) \
-    hipLaunchKernelGGL((ns_product_kernel<TB, WN, KG, PL, NB, MODE>), dim3(grid), dim3(128 * WN * KG), 0, s, p, 2 * (t & 1), t == 0)
-#define NS_SMALL(PL, MODE, grid) hipLaunchKernelGGL((ns_small_kernel<PL, MODE>), dim3(grid), dim3(512), 0, s, p, 2 * (t & 1), t == 0)
-#define NS_PRODUCT(MODE, size, grid)                                                      \
+    hipLaunchKernelGGL((ns_product_kernel<TB, WN, KG, PL, NB, MODE>), dim3(grid), dim3(128 * WN * KG), 0, s, group, 2 * (t & 1), t == 0)
+#define NS_SMALL(PL, MODE, grid) hipLaunchKernelGGL((ns_small_kernel<PL, MODE>), dim3(grid), dim3(512), 0, s, group, 2 * (t & 1), t == 0)
+#define NS_PRODUCT(set, MODE, size, grid)                                                 \
     do {                                                                                  \
+        const NsGroup& group = set;                                                       \
         if (p.planes == 2) {                                                              \
             if (size == 3) NS_LAUNCH(256, 4, 1, 2, 2, MODE, grid);                        \
             else if (size == 4) NS_LAUNCH((MODE == NS_GRAM || MODE == NS_POLY ? 192 : 128), 2, 1, 2, (MODE == NS_GRAM || MODE == NS_POLY ? 3 : 2), MODE, grid); \
@@ -782,14 +810,35 @@ extern "C" int dvae_orthogonalize(const dvae_matrix_desc* mats, int32_t count, i
         }                                                                                 \
         DVAE_LAUNCH_CHECK();                                                              \
     } while (0)
+        // X X^T of matrices with few rows in sets that take larger tiles: apart, on 64 x 64 tiles
+        NsGroup most_of = p, few = p;
+        int most_tiles = square[sq], few_tiles = 0;
+        most_of.count = few.count = 0;
+        if (p.planes == 2 && sq >= 2) {
+            most_tiles = 0;
+            for (int i = 0; i < n; ++i) {
+                const bool is_few = p.mat[i].m() <= NS_FEW;
+                NsGroup& group = is_few ? few : most_of;
+                int& tiles = is_few ? few_tiles : most_tiles;
+                group.mat[group.count] = p.mat[i];
+                group.mat[group.count++].tile0 = tiles;
+                const int mt = cdiv(ns_pad(p.mat[i].m(), p.pad), side[is_few ? 1 : sq]);
+                tiles += mt * (mt + 1) / 2;
+            }
+        }
         for (int t = 0; t < steps; ++t) {
             p.a = coefficients[3 * t]; p.b = coefficients[3 * t + 1]; p.c = coefficients[3 * t + 2];
+            p.shift = few.shift = most_of.shift = shift[t];
             place(square0[sq]);
-            NS_PRODUCT(NS_GRAM, sq, square[sq]);
-            NS_PRODUCT(NS_POLY, sq, square[sq]);
+            if (few_tiles == 0) NS_PRODUCT(p, NS_GRAM, sq, square[sq]);
+            else {
+                NS_PRODUCT(few, NS_GRAM, 1, few_tiles);
+                if (most_tiles > 0) NS_PRODUCT(most_of, NS_GRAM, sq, most_tiles);
+            }
+            NS_PRODUCT(p, NS_POLY, sq, square[sq]);
             place(update0[up]);
-            if (t + 1 < steps) NS_PRODUCT(NS_STEP, up, update[up]);
-            else NS_PRODUCT(NS_LAST, up, update[up]);
+            if (t + 1 < steps) NS_PRODUCT(p, NS_STEP, up, update[up]);
+            else NS_PRODUCT(p, NS_LAST, up, update[up]);
         }
 #undef NS_PRODUCT
 #undef NS_LAUNCH

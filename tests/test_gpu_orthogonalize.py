@@ -136,3 +136,40 @@ def test_outputs_in_the_place_of_other_inputs():
     want = O.orthogonalize([large, small], products="half")
     O.orthogonalize([mine[:, :512], mine[:, 512:]], out=[mine[:, 511:], mine[:, :511]], products="half")
     assert torch.equal(mine[:, 511:], want[0]) and torch.equal(mine[:, :511], want[1])
+
+
+LARGE = [(1312, 1785), (619, 1766), (790, 578), (500, 542)]
+LONG_SETS = [[(9, 1883)] + LARGE, [(9, 1883), (17, 690), (11, 267), (30, 1500), (8, 2048), (56, 501), (64, 2000), (100, 2000)] + LARGE,
+             [(9, 20000), (40, 9000), (100, 20000), (300, 20000)] + LARGE, [(300, 8192)] * 32, [(250, 4000)] * 32,
+             [(2048, 2048)] * 2 + [(9, 1883), (30, 2000), (2000, 9), (384, 3000), (385, 3000)], [(4096, 4096), (9, 1883)], [(9, 20000)], [(300, 20000)]]
+
+
+@pytest.mark.parametrize("k", range(len(LONG_SETS)))
+def test_few_rows_with_long_sums_keep_float32_accuracy_in_every_set(k):
+    """An entry of X X^T is a sum over a whole row, and where there are few rows its rounding is not averaged over many: added up
+    one by one in float32 it was up to 3.6 times as far off as the float32 iteration, in some sets.  Its parts are summed
+    apart; half as much again as the float32 iteration loses is allowed, or 16 of its half steps."""
+    for seed in range(2):
+        g = torch.Generator(device="cuda")
+        g.manual_seed(seed)
+        for kind in ("noise", "spiked"):
+            mats = [torch.randn(m, n, generator=g, device="cuda") for m, n in LONG_SETS[k]]
+            if kind == "spiked":
+                mats = [a + 3 * torch.randn(a.shape[0], 4, generator=g, device="cuda") @ torch.randn(4, a.shape[1], generator=g, device="cuda") for a in mats]
+            for m, o in list(zip(mats, O.orthogonalize(mats)))[:8]:
+                want = plain(m).cpu()
+                got, mine = off(o, want), off(plain(m, dtype=torch.float32), want)
+                assert got <= max(1.5 * mine, 2.0 ** -20), (kind, tuple(m.shape), got, mine)
+
+
+@pytest.mark.parametrize("shape", [(1, 40), (3, 50), (8, 80), (9, 84), (16, 300), (64, 90), (65, 90), (600, 12)])
+def test_few_rows_with_other_coefficients(shape):
+    """B of up to 64 rows is held shifted, unless the coefficients leave no room for that (the last two sets, whose singular values
+    stay below 1); limits as at the head of the file"""
+    m = matrix(shape, 0, 8)
+    for abc, steps in (((1.5, -0.5, 0.0), 3), ((2.0, -1.5, 0.5), 8), ([(3.4445, -4.7750, 2.0315), (2.0, -1.5, 0.5)], 2), ((1.0, 0.0, 0.0), 2),
+                       ([(0.5, 0.0, 0.0), (3.8, -6.8, -1.3)], 2), ([(0.4, 0.0, 0.0), (1.36, 7.15, 2.38), (1.5, -0.5, 0.0)], 3)):
+        want = plain(m, steps, abc).cpu()
+        for given in ([m], [m] + [matrix((200, 300), 0, k) for k in range(9)]):  # by itself and on larger tiles
+            got = O.orthogonalize(given, steps=steps, coefficients=abc)[0]
+            assert off(got, want) <= 8 * max(off(plain(m, steps, abc, dtype=torch.float32), want), 2.0 ** -22), (abc, len(given))
